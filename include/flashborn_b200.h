@@ -368,6 +368,119 @@ typedef struct fb_xent_args {
 FB_API int fb_xent_fwd(const fb_xent_args* args, void* stream);
 FB_API int fb_xent_bwd(const fb_xent_args* args, void* stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Generating from a trained model: a paged key-value cache, attention of one new token per
+ * sequence over it, and what fills it (additions to ABI version 4; no earlier struct changed).
+ *
+ * Pages: k and v are (num_pages, kv_heads, page_size, head_dim) with element strides, innermost 1.
+ * Token t of sequence s lives in page table[s][t / page_size], row t % page_size.
+ *
+ *   fb_paged_born_fwd   a_j = max(0, scale_h <q, k_j>),  p_j = a_j^2,  for the keys j of
+ *                       [max(0, len - window), len) (window 0: all of them)
+ *                       out = (sum_j p_j v_j) / (sum_j p_j + eps);  no key with p_j > 0: out = 0
+ * Query head h reads kv head h / (heads / kv_heads).  lens are the cache lengths, the new token
+ * included; a length outside [0, max_pages * page_size] is clamped to it.  A table entry outside
+ * [0, num_pages) holds no keys.  What a page holds past its sequence's length is never used, NaN
+ * included; a NaN key that is used gives a NaN row.
+ * scale: device vector of 1 or heads floats, or NULL for scale_value.
+ * ------------------------------------------------------------------------------------------ */
+typedef struct fb_paged_args {
+  int32_t seqs, heads, kv_heads, head_dim;
+  int32_t dtype;       /* q, k, v and out */
+  int32_t page_size, num_pages, max_pages; /* max_pages: table columns */
+  int32_t window_size; /* 0 = no window */
+  float eps;
+  float scale_value;
+  int32_t scale_numel;
+  const float* scale;
+  const void* q;       int64_t q_stride[3];   /* (seqs, heads, head_dim) */
+  const void* k;       int64_t k_stride[4];
+  const void* v;       int64_t v_stride[4];
+  void* out;           int64_t out_stride[3]; /* (seqs, heads, head_dim) */
+  const int32_t* table; int64_t table_stride; /* elements between the table's rows */
+  const int32_t* lens;
+  void* workspace;     size_t workspace_bytes;
+} fb_paged_args;
+
+FB_API size_t fb_paged_workspace_size(const fb_paged_args* args);
+FB_API int fb_paged_born_fwd(const fb_paged_args* args, void* stream);
+
+/* New tokens into the cache: row n of qkv holds (heads + 2 kv_heads) heads of head_dim: Q, K, V.
+ *   Q, K heads: rotated by the angles of row positions[n] of cos / sin (as fb_qkv_prologue_fwd),
+ *               then x / sqrt(sum x^2 + eps);   V: copied
+ * q receives the Q heads, (tokens, heads, head_dim) contiguous; K and V go to slot slots[n] =
+ * page * page_size + row of the pages.  A slot outside the pages stores nothing (padding); a
+ * position outside [0, rope_rows) gives NaN q and K.  Two tokens with one slot race.  k_out and v_out
+ * (both or neither), (tokens, kv_heads, head_dim) contiguous, receive K and V as well. */
+typedef struct fb_paged_write_args {
+  int64_t tokens;
+  int32_t heads, kv_heads, head_dim;
+  int32_t dtype;
+  int32_t page_size, num_pages, rope_rows;
+  float eps;
+  const void* qkv;  int64_t qkv_stride; /* elements between rows */
+  const float* cos; const float* sin;   /* (rope_rows, head_dim / 2) contiguous */
+  const int64_t* positions;
+  const int64_t* slots;
+  void* k;          int64_t k_stride[4];
+  void* v;          int64_t v_stride[4];
+  void* q;
+  void* k_out;
+  void* v_out;
+} fb_paged_write_args;
+
+FB_API int fb_paged_qkv_write(const fb_paged_write_args* args, void* stream);
+
+/* Log probabilities of given tokens, with entropy and the top_k alternatives of each row:
+ *   lse = log sum_c exp(x_c);  logp = x_t - lse;  entropy = lse - sum_c p_c x_c
+ *   top: the top_k largest x_c, equal ones by lowest index, NaN above everything: x_c - lse, c
+ * -inf columns have no probability; a row with nothing but them, a +inf or a NaN is NaN, and so is
+ * the logp of a target outside [0, vocab).  logp, entropy, lse, top_logp fp32; top_index int64.
+ *   backward   grad_c = g_logp ([c == t] - p_c) + sum_i g_top_i ([c == top_i] - p_c)
+ *                       - g_entropy p_c (log p_c + entropy)
+ * Any of g_logp, g_entropy, g_top may be NULL (zero).  top_k <= FB_MAX_TOP_K. */
+#define FB_MAX_TOP_K 64
+typedef struct fb_logprob_args {
+  int64_t rows;
+  int32_t vocab, dtype, top_k;
+  const void* logits;     int64_t ld;      /* elements between rows */
+  const int64_t* targets;
+  float* logp;
+  float* entropy;
+  float* lse;
+  float* top_logp;        /* (rows, top_k) contiguous */
+  int64_t* top_index;
+  const float* g_logp;
+  const float* g_entropy;
+  const float* g_top;     /* (rows, top_k) contiguous */
+  void* grad;             int64_t grad_ld; /* the logits' type */
+} fb_logprob_args;
+
+FB_API int fb_logprob_fwd(const fb_logprob_args* args, void* stream);
+FB_API int fb_logprob_bwd(const fb_logprob_args* args, void* stream);
+
+/* The global norm of many gradient tensors, and clipping:
+ *   norm = sqrt(sum over all tensors of g^2);  c = min(1, max_norm / (norm + eps));  out = c g
+ * The arrays of `count` entries are host memory, read during the call.  grads[i] and out[i] are
+ * dense tensors of numel[i] elements of type dtype[i] and out_dtype[i] (the same, or FB_F32).
+ * out[i] == grads[i] scales in place, and then nothing is written when c is 1.  out NULL: the norm
+ * alone.  A NaN gradient gives a NaN norm and NaN outputs; squares are summed in fp32 per thread and
+ * in fp64 across threads.  norm: device fp32 scalar. */
+typedef struct fb_clip_args {
+  int32_t count;
+  const void* const* grads;
+  void* const* out;
+  const int64_t* numel;
+  const int32_t* dtype;
+  const int32_t* out_dtype;
+  float max_norm, eps;
+  float* norm;
+  void* workspace; size_t workspace_bytes;
+} fb_clip_args;
+
+FB_API size_t fb_clip_workspace_size(const fb_clip_args* args);
+FB_API int fb_clip_grad_norm(const fb_clip_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -8,23 +8,35 @@ signatures and tensor layout so callers swap it in unchanged (see ``swap``).
 from .kernels import (
     HAS_TRITON,
     IS_HIP,
+    TokenLogprobs,
+    clip_grad_norm_,
     complex_phase_born_attention,
     flash_born_attention,
     flash_born_attention_token_major,
     flash_purified_born_attention,
     get_flash_born_launch_meta,
     get_rdna4_autotune_configs,
+    grad_norm,
+    paged_born_attention,
+    paged_qkv_write,
     paired_heads_born_attention,
+    token_logprobs,
 )
 
 __all__ = [
     "HAS_TRITON",
     "IS_HIP",
+    "TokenLogprobs",
+    "clip_grad_norm_",
     "complex_phase_born_attention",
     "flash_born_attention",
     "flash_born_attention_token_major",
     "flash_purified_born_attention",
     "get_flash_born_launch_meta",
     "get_rdna4_autotune_configs",
+    "grad_norm",
+    "paged_born_attention",
+    "paged_qkv_write",
     "paired_heads_born_attention",
+    "token_logprobs",
 ]

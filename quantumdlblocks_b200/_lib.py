@@ -23,6 +23,7 @@ FB_ERR_WORKSPACE = 7
 FB_ERR_NO_DEVICE = 8
 FB_ERR_UNSUPPORTED = 9
 FB_ERR_SCRATCH_LIMIT = 10
+FB_MAX_TOP_K = 64
 FB_STATIC_SCRATCH_BYTES = 16 * 1024 * 1024
 
 FB_F32, FB_F16, FB_BF16 = 0, 1, 2
@@ -30,6 +31,7 @@ FB_PATH_AUTO, FB_PATH_TCGEN05, FB_PATH_GENERAL = 0, 1, 2
 
 _I64x4 = ctypes.c_int64 * 4
 _I64x2 = ctypes.c_int64 * 2
+_I64x3 = ctypes.c_int64 * 3
 
 
 class FbAttnArgs(ctypes.Structure):
@@ -124,6 +126,59 @@ class FbHeadsArgs(ctypes.Structure):
     ]
 
 
+class FbPagedArgs(ctypes.Structure):
+    """Mirror of ``fb_paged_args`` (attention of one new token per sequence over a paged cache)."""
+    _fields_ = [
+        ("seqs", ctypes.c_int32), ("heads", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("page_size", ctypes.c_int32), ("num_pages", ctypes.c_int32), ("max_pages", ctypes.c_int32),
+        ("window_size", ctypes.c_int32), ("eps", ctypes.c_float), ("scale_value", ctypes.c_float),
+        ("scale_numel", ctypes.c_int32), ("scale", ctypes.c_void_p),
+        ("q", ctypes.c_void_p), ("q_stride", _I64x3),
+        ("k", ctypes.c_void_p), ("k_stride", _I64x4),
+        ("v", ctypes.c_void_p), ("v_stride", _I64x4),
+        ("out", ctypes.c_void_p), ("out_stride", _I64x3),
+        ("table", ctypes.c_void_p), ("table_stride", ctypes.c_int64), ("lens", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class FbPagedWriteArgs(ctypes.Structure):
+    """Mirror of ``fb_paged_write_args`` (new tokens' Q, K, V, the last two into the cache)."""
+    _fields_ = [
+        ("tokens", ctypes.c_int64), ("heads", ctypes.c_int32), ("kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32), ("dtype", ctypes.c_int32),
+        ("page_size", ctypes.c_int32), ("num_pages", ctypes.c_int32), ("rope_rows", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("qkv", ctypes.c_void_p), ("qkv_stride", ctypes.c_int64), ("cos", ctypes.c_void_p), ("sin", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p), ("slots", ctypes.c_void_p),
+        ("k", ctypes.c_void_p), ("k_stride", _I64x4), ("v", ctypes.c_void_p), ("v_stride", _I64x4),
+        ("q", ctypes.c_void_p), ("k_out", ctypes.c_void_p), ("v_out", ctypes.c_void_p),
+    ]
+
+
+class FbLogprobArgs(ctypes.Structure):
+    """Mirror of ``fb_logprob_args`` (log probabilities of given tokens)."""
+    _fields_ = [
+        ("rows", ctypes.c_int64), ("vocab", ctypes.c_int32), ("dtype", ctypes.c_int32), ("top_k", ctypes.c_int32),
+        ("logits", ctypes.c_void_p), ("ld", ctypes.c_int64), ("targets", ctypes.c_void_p),
+        ("logp", ctypes.c_void_p), ("entropy", ctypes.c_void_p), ("lse", ctypes.c_void_p),
+        ("top_logp", ctypes.c_void_p), ("top_index", ctypes.c_void_p),
+        ("g_logp", ctypes.c_void_p), ("g_entropy", ctypes.c_void_p), ("g_top", ctypes.c_void_p),
+        ("grad", ctypes.c_void_p), ("grad_ld", ctypes.c_int64),
+    ]
+
+
+class FbClipArgs(ctypes.Structure):
+    """Mirror of ``fb_clip_args`` (global gradient norm and clipping)."""
+    _fields_ = [
+        ("count", ctypes.c_int32), ("grads", ctypes.c_void_p), ("out", ctypes.c_void_p), ("numel", ctypes.c_void_p),
+        ("dtype", ctypes.c_void_p), ("out_dtype", ctypes.c_void_p),
+        ("max_norm", ctypes.c_float), ("eps", ctypes.c_float), ("norm", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
 # Every symbol the header declares, with its ctypes signature.
 _PARGS = ctypes.POINTER(FbAttnArgs)
 _PQKV = ctypes.POINTER(FbQkvArgs)
@@ -156,6 +211,13 @@ SIGNATURES = {
     "fb_combine_terms": (ctypes.c_int, [ctypes.POINTER(FbCombineArgs), ctypes.c_void_p]),
     "fb_delta_terms": (ctypes.c_int, [ctypes.POINTER(FbDeltaArgs), ctypes.c_void_p]),
     "fb_xent_bwd": (ctypes.c_int, [_PXENT, ctypes.c_void_p]),
+    "fb_paged_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(FbPagedArgs)]),
+    "fb_paged_born_fwd": (ctypes.c_int, [ctypes.POINTER(FbPagedArgs), ctypes.c_void_p]),
+    "fb_paged_qkv_write": (ctypes.c_int, [ctypes.POINTER(FbPagedWriteArgs), ctypes.c_void_p]),
+    "fb_logprob_fwd": (ctypes.c_int, [ctypes.POINTER(FbLogprobArgs), ctypes.c_void_p]),
+    "fb_logprob_bwd": (ctypes.c_int, [ctypes.POINTER(FbLogprobArgs), ctypes.c_void_p]),
+    "fb_clip_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(FbClipArgs)]),
+    "fb_clip_grad_norm": (ctypes.c_int, [ctypes.POINTER(FbClipArgs), ctypes.c_void_p]),
 }
 
 _lock = threading.Lock()

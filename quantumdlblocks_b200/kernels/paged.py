@@ -1,0 +1,182 @@
+"""Generating from a trained flash-Born GPT: Born attention over a paged key-value cache.
+
+The reference trains its GPTs but has no cache; a model that answers token by token needs one.
+Two native ops (no gradient, CUDA only, like every op here):
+
+  ``paged_qkv_write``       new tokens' fused projection -> Q (RoPE + L2 normalisation), with K (the
+                            same) and V stored into their slots of the cache's pages
+  ``paged_born_attention``  one new query per sequence against its cached keys: the framework's Born
+                            attention ``O = sum p v / (sum p + eps)``, ``p = relu(scale q.k)^2``
+
+The pages are ``(num_pages, kv_heads, page_size, head_dim)`` tensors: a page is a batch entry of the
+framework's ``(B, H, T, D)`` layout.  Sequence s keeps its token t in page ``block_table[s, t // page_size]``,
+row ``t % page_size``; ``slots`` of the write are ``page * page_size + row``.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from .. import _lib
+from .flash_born import _DTYPE_CODE, _stream_handle
+
+__all__ = ["paged_born_attention", "paged_qkv_write"]
+
+_I64x3, _I64x4 = _lib._I64x3, _lib._I64x4
+
+
+def _check_pages(what: str, x: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor) -> None:
+    if not (x.is_cuda and k_pages.is_cuda and v_pages.is_cuda):
+        raise RuntimeError(f"{what} (B200): CUDA tensors required; there is no CPU path")
+    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape:
+        raise ValueError(f"{what}: pages must be two (num_pages, kv_heads, page_size, head_dim) tensors of one shape; "
+                         f"got {tuple(k_pages.shape)}, {tuple(v_pages.shape)}")
+    if x.dtype not in _DTYPE_CODE or k_pages.dtype != x.dtype or v_pages.dtype != x.dtype:
+        raise ValueError(f"{what}: one dtype of float32 / float16 / bfloat16 for all; got {x.dtype}, {k_pages.dtype}, "
+                         f"{v_pages.dtype}")
+    if k_pages.shape[3] > 1 and (k_pages.stride(3) != 1 or v_pages.stride(3) != 1):
+        raise ValueError(f"{what}: pages must have a unit inner stride (they are not copied)")
+    if torch.is_grad_enabled() and (x.requires_grad or k_pages.requires_grad or v_pages.requires_grad):
+        raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad()")
+
+
+def _check_devices(what: str, device: torch.device, *tensors: torch.Tensor) -> None:
+    for t in tensors:
+        if t.device != device:
+            raise RuntimeError(f"{what}: all tensors must be on {device}; got one on {t.device}")
+
+
+def _page_strides(t: torch.Tensor):
+    s = t.stride()
+    return _I64x4(s[0], s[1], s[2], 1)
+
+
+def paged_born_attention(
+    q: torch.Tensor,
+    k_pages: torch.Tensor,
+    v_pages: torch.Tensor,
+    block_table: torch.Tensor,
+    seq_lens: torch.Tensor,
+    scale: float | torch.Tensor,
+    eps: float = 1e-12,
+    window_size: int = 0,
+) -> torch.Tensor:
+    """Born attention of one new token per sequence: ``out (S, H, D)`` in q's dtype.
+
+    q is ``(S, H, D)`` (the head_dim up to 256); k_pages, v_pages ``(num_pages, Hkv, page_size, D)`` of q's
+    dtype with H a multiple of Hkv (query head h reads kv head ``h // (H // Hkv)``) and any strides but the
+    inner one; block_table ``(S, max_pages)`` int32; seq_lens ``(S,)`` int32 cache lengths, the new token
+    included.  ``scale`` and ``eps`` are those of ``flash_born_attention`` (scale: float, or a tensor of 1 or
+    H elements); ``window_size > 0`` keeps the last ``window_size`` keys.  A sequence without keys (or whose
+    keys all have zero weight) gives zeros.  Lengths past ``max_pages * page_size`` are cut to it, and a table
+    entry outside the pages holds no keys.  What pages hold past a sequence's length is never used.
+    """
+    _check_pages("paged_born_attention", q, k_pages, v_pages)
+    if q.dim() != 3:
+        raise ValueError(f"paged_born_attention: q must be (S, H, D); got {tuple(q.shape)}")
+    S, H, D = q.shape
+    P, Hkv, page, Dk = k_pages.shape
+    if Dk != D or D < 1 or D > 256 or Hkv < 1 or H < 1 or H % Hkv != 0 or page < 1:
+        raise ValueError(f"paged_born_attention: q {tuple(q.shape)} does not fit pages {tuple(k_pages.shape)} "
+                         "(the same head_dim in [1, 256], heads a multiple of kv_heads)")
+    if block_table.dim() != 2 or block_table.shape[0] != S or block_table.dtype != torch.int32:
+        raise ValueError(f"paged_born_attention: block_table must be ({S}, max_pages) int32; got "
+                         f"{tuple(block_table.shape)} {block_table.dtype}")
+    if seq_lens.shape != (S,) or seq_lens.dtype != torch.int32:
+        raise ValueError(f"paged_born_attention: seq_lens must be ({S},) int32; got {tuple(seq_lens.shape)} "
+                         f"{seq_lens.dtype}")
+    if not eps >= 0.0 or window_size < 0:
+        raise ValueError(f"paged_born_attention: eps and window_size must not be negative; got {eps}, {window_size}")
+    device = q.device
+    _check_devices("paged_born_attention", device, k_pages, v_pages, block_table, seq_lens)
+    a = _lib.FbPagedArgs()
+    if isinstance(scale, torch.Tensor):
+        sc = scale.detach().reshape(-1).to(device=device, dtype=torch.float32).contiguous()
+        if sc.numel() not in (1, H):
+            raise ValueError(f"scale must have 1 or H={H} elements, got {sc.numel()}")
+        a.scale, a.scale_numel = sc.data_ptr(), sc.numel()
+    else:
+        a.scale_value = float(scale)
+    qc = q if D == 1 or q.stride(2) == 1 else q.contiguous()
+    table = block_table if block_table.shape[1] <= 1 or block_table.stride(1) == 1 else block_table.contiguous()
+    lens = seq_lens.contiguous()
+    out = torch.empty((S, H, D), dtype=q.dtype, device=device)
+    a.seqs, a.heads, a.kv_heads, a.head_dim = S, H, Hkv, D
+    a.dtype = _DTYPE_CODE[q.dtype]
+    a.page_size, a.num_pages, a.max_pages = page, P, table.shape[1]
+    a.window_size, a.eps = int(window_size), float(eps)
+    s = qc.stride()
+    a.q, a.q_stride = qc.data_ptr(), _I64x3(s[0], s[1], 1)
+    a.k, a.k_stride = k_pages.data_ptr(), _page_strides(k_pages)
+    a.v, a.v_stride = v_pages.data_ptr(), _page_strides(v_pages)
+    a.out, a.out_stride = out.data_ptr(), _I64x3(H * D, D, 1)
+    a.table, a.table_stride, a.lens = table.data_ptr(), table.stride(0), lens.data_ptr()
+    lib = _lib.load()
+    need = lib.fb_paged_workspace_size(ctypes.byref(a))
+    if need:
+        ws = torch.empty(need, dtype=torch.uint8, device=device)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), need
+    with torch.cuda.device(device):
+        _lib.check(lib.fb_paged_born_fwd(ctypes.byref(a), _stream_handle(device)), "paged Born attention")
+    return out
+
+
+def paged_qkv_write(
+    qkv: torch.Tensor,
+    cos: torch.Tensor,
+    sin: torch.Tensor,
+    positions: torch.Tensor,
+    slots: torch.Tensor,
+    k_pages: torch.Tensor,
+    v_pages: torch.Tensor,
+    heads: int,
+    eps: float = 1e-12,
+    return_kv: bool = False,
+) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Q of new tokens, their K and V stored in the cache: ``q (N, H, D)``, or ``(q, k, v)``.
+
+    qkv is ``(N, (H + 2 Hkv) D)``, a fused projection's rows (Q heads, then K heads, then V heads); ``cos`` /
+    ``sin`` are the fp32 ``rope_tables``, ``positions (N,)`` each token's row of them.  Q and K are turned and
+    L2-normalised as ``qkv_rope_l2norm`` does, V is copied; K and V go to ``slots (N,)`` of the pages (changed in
+    place), Q is returned.  A slot outside the pages (-1, say) stores nothing; a position outside the tables
+    gives NaN Q and K; two tokens must not share a slot.  ``return_kv=True`` also returns K and V
+    ``(N, Hkv, D)``, for the prompt's own attention.  head_dim is even, up to 256.
+    """
+    _check_pages("paged_qkv_write", qkv, k_pages, v_pages)
+    P, Hkv, page, D = k_pages.shape
+    if qkv.dim() != 2 or D < 2 or D > 256 or D % 2 or Hkv < 1 or page < 1 or heads < 1 or heads % Hkv != 0 \
+            or qkv.shape[1] != (heads + 2 * Hkv) * D:
+        raise ValueError(f"paged_qkv_write: qkv must be (N, (H + 2 Hkv) D) with H={heads} a multiple of Hkv={Hkv} and "
+                         f"D={D} even, at most 256; got {tuple(qkv.shape)}")
+    N = qkv.shape[0]
+    if positions.shape != (N,) or slots.shape != (N,) or positions.is_floating_point() or slots.is_floating_point():
+        raise ValueError(f"paged_qkv_write: positions and slots must be ({N},) integers; got {tuple(positions.shape)} "
+                         f"{positions.dtype}, {tuple(slots.shape)} {slots.dtype}")
+    if cos.dim() != 2 or cos.shape[1] != D // 2 or sin.shape != cos.shape or cos.dtype != torch.float32 \
+            or sin.dtype != torch.float32:
+        raise ValueError(f"paged_qkv_write: rope tables must be two (rows, {D // 2}) float32; got {tuple(cos.shape)} "
+                         f"{cos.dtype}, {tuple(sin.shape)} {sin.dtype}")
+    if not eps >= 0.0:
+        raise ValueError(f"paged_qkv_write: eps must not be negative; got {eps}")
+    device = qkv.device
+    _check_devices("paged_qkv_write", device, k_pages, v_pages, cos, sin, positions, slots)
+    x = qkv if qkv.stride(1) == 1 else qkv.contiguous()
+    cos, sin = cos.contiguous(), sin.contiguous()
+    positions, slots = positions.to(torch.int64).contiguous(), slots.to(torch.int64).contiguous()
+    q = torch.empty((N, heads, D), dtype=qkv.dtype, device=device)
+    a = _lib.FbPagedWriteArgs()
+    a.tokens, a.heads, a.kv_heads, a.head_dim = N, heads, Hkv, D
+    a.dtype = _DTYPE_CODE[qkv.dtype]
+    a.page_size, a.num_pages, a.rope_rows, a.eps = page, P, cos.shape[0], float(eps)
+    a.qkv, a.qkv_stride = x.data_ptr(), x.stride(0)
+    a.cos, a.sin, a.positions, a.slots = cos.data_ptr(), sin.data_ptr(), positions.data_ptr(), slots.data_ptr()
+    a.k, a.k_stride = k_pages.data_ptr(), _page_strides(k_pages)
+    a.v, a.v_stride = v_pages.data_ptr(), _page_strides(v_pages)
+    a.q = q.data_ptr()
+    if return_kv:
+        k, v = (torch.empty((N, Hkv, D), dtype=qkv.dtype, device=device) for _ in range(2))
+        a.k_out, a.v_out = k.data_ptr(), v.data_ptr()
+    with torch.cuda.device(device):
+        _lib.check(_lib.load().fb_paged_qkv_write(ctypes.byref(a), _stream_handle(device)), "paged QKV write")
+    return (q, k, v) if return_kv else q

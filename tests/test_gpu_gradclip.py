@@ -1,0 +1,151 @@
+"""GPU: the global gradient norm over many tensors, and clipping, against 64-bit sums: mixed types and
+odd sizes, unaligned and permuted tensors, empty ones, more tensors than one launch takes, NaN and inf."""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import serving_ref as ref
+from quantumdlblocks_b200 import clip_grad_norm_, grad_norm
+from quantumdlblocks_b200.kernels import flash_born as fbm
+
+pytestmark = pytest.mark.gpu
+
+if not torch.cuda.is_available():
+    pytest.skip("CUDA device required", allow_module_level=True)
+
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+
+
+def make(sizes, dtypes, seed=0, std=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return [(torch.randn(n, generator=g, device="cuda") * std * (1 + i % 3)).to(dtypes[i % len(dtypes)])
+            for i, n in enumerate(sizes)]
+
+
+def check(norm, got, want_norm, want):
+    assert fbm.device_status() == (0, 0)
+    assert norm.shape == () and norm.dtype == F32
+    # squares and their sums round in fp32 within a thread (at most a few hundred of them), fp64 beyond
+    assert abs(float(norm) - want_norm) <= 1e-5 * want_norm
+    for o, w in zip(got, want):
+        tol = (1.01 * ref.ROUND[o.dtype] + 2e-5) * w.abs() + (6e-8 if o.dtype == F16 else 0.0)
+        assert bool(((o.double() - w).abs() <= tol).all())
+
+
+SIZES = [[1], [5], [0, 3, 0], [1024], [4096, 1, 4097, 33], [100_003, 17, 65536, 0, 999], [1_000_001] * 3,
+         [1] * 700, list(range(1, 400)), [3_000_000]]
+
+
+@pytest.mark.parametrize("dtypes", [[F32], [BF16], [F16], [F32, BF16, F16]], ids=["fp32", "bf16", "fp16", "mixed"])
+@pytest.mark.parametrize("sizes", SIZES, ids=lambda s: f"{len(s)}x{max(s)}")
+@pytest.mark.parametrize("to", ["in place", "out", "out fp32"])
+def test_clip_matches_formula(sizes, dtypes, to):
+    grads = make(sizes, dtypes)
+    full, _ = ref.clip(grads, math.inf)
+    for max_norm in (0.25 * full, 4.0 * full):
+        want_norm, want = ref.clip(grads, max_norm)
+        gs = [g.clone() for g in grads]
+        out = None if to == "in place" else [torch.full_like(g, 7.0, dtype=F32 if to == "out fp32" else g.dtype) for g in gs]
+        norm = clip_grad_norm_(gs, max_norm, out=out)
+        check(norm, gs if out is None else out, want_norm, want)
+        if out is not None or max_norm > full:
+            assert all(torch.equal(a, b) for a, b in zip(gs, grads))
+    assert abs(float(grad_norm(grads)) - full) <= 1e-5 * full
+    assert torch.equal(grad_norm(grads), grad_norm(grads))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("start", [1, 2, 3, 5])
+def test_unaligned_tensors(start, dtype):
+    """Views that start anywhere in their storage; what lies around them stays as it was."""
+    store = torch.randn(30_011, device="cuda").to(dtype)
+    old = store.clone()
+    cuts = [(start, start + 1), (start + 7, start + 1003), (2000 + start, 29_000 + start)]
+    gs = [store[a:b] for a, b in cuts]
+    want_norm, want = ref.clip(gs, 1.5)
+    check(clip_grad_norm_(gs, 1.5), gs, want_norm, want)
+    inside = torch.zeros(30_011, dtype=torch.bool, device="cuda")
+    for a, b in cuts:
+        inside[a:b] = True
+    assert torch.equal(store[~inside], old[~inside])
+    # into buffers aligned otherwise
+    gs = [old[a:b] for a, b in cuts]
+    out = [torch.zeros(b - a + 1, device="cuda")[1:] for a, b in cuts]
+    check(clip_grad_norm_(gs, 1.5, out=out), out, want_norm, want)
+
+
+def test_permuted_and_strided_tensors():
+    a = torch.randn(6, 40, 8, device="cuda").permute(2, 0, 1)  # dense in another order
+    b = torch.randn(64, 32, device="cuda").t()
+    for x in (a, b):
+        want_norm, want = ref.clip([x], 1.0)
+        y = x.clone(memory_format=torch.preserve_format)
+        check(clip_grad_norm_([y], 1.0), [y], want_norm, want)
+    with pytest.raises(ValueError):
+        clip_grad_norm_([torch.randn(8, 8, device="cuda")[:, ::2]], 1.0)
+    with pytest.raises(ValueError):
+        clip_grad_norm_([torch.randn(1, 8, device="cuda").expand(4, 8)], 1.0)
+    got = grad_norm([torch.randn(8, 8, device="cuda")[:, ::2].fill_(2.0)])
+    assert float(got) == float(torch.tensor(4.0 * 32).sqrt())
+
+
+def test_not_a_number_and_infinity():
+    gs = make([100, 50], [F32])
+    gs[1][7] = math.nan
+    norm = clip_grad_norm_(gs, 1.0)
+    assert norm.isnan() and all(g.isnan().all() for g in gs)
+    gs = make([100, 50], [F32])
+    gs[0][3] = math.inf
+    norm = clip_grad_norm_(gs, 1.0)
+    assert norm.isinf() and gs[0][3].isnan() and torch.all(gs[1] == 0)
+    gs = [torch.zeros(10, device="cuda")]
+    assert float(clip_grad_norm_(gs, 1.0)) == 0.0 and torch.all(gs[0] == 0)
+    gs = make([100], [F32])
+    clip_grad_norm_(gs, 0.0)
+    assert torch.all(gs[0] == 0)
+
+
+def test_long_tensor_past_32_bits():
+    """More than 2^31 elements in one tensor."""
+    n = (1 << 31) + 12_345
+    g = torch.zeros(n, dtype=BF16, device="cuda")
+    g[0], g[(1 << 31) - 1], g[1 << 31], g[n - 1] = 1.0, 2.0, 2.0, 4.0
+    norm = clip_grad_norm_([g], 1.0)
+    assert abs(float(norm) - 5.0) <= 1e-5
+    for i, x in ((0, 1.0), ((1 << 31) - 1, 2.0), (1 << 31, 2.0), (n - 1, 4.0)):
+        assert abs(float(g[i]) - x / 5.0) <= x / 5.0 * 2.0 ** -8
+    assert int((g != 0).sum()) == 4
+
+
+def test_runs_on_the_current_stream():
+    gs = make([5000, 300], [F32])
+    want_norm, want = ref.clip(gs, 1.0)
+    new = [torch.zeros_like(g) for g in gs]
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)
+        for a, b in zip(new, gs):
+            a.copy_(b)
+        norm = clip_grad_norm_(new, 1.0)
+    side.synchronize()
+    check(norm, new, want_norm, want)
+
+
+def test_refusals():
+    g = torch.ones(8, device="cuda")
+    for args in (([], 1.0), ([g], -1.0), ([g], math.nan), ([g.double()], 1.0), ([g.int()], 1.0)):
+        with pytest.raises(ValueError):
+            clip_grad_norm_(*args)
+    for out in ([], [g, g], [torch.ones(7, device="cuda")], [g.half()], [torch.ones(8, 2, device="cuda")[:, 0]]):
+        with pytest.raises(ValueError):
+            clip_grad_norm_([g], 1.0, out=out)
+    with pytest.raises(ValueError):
+        clip_grad_norm_([g], 1.0, eps=-1.0)
+    with pytest.raises(RuntimeError):
+        clip_grad_norm_([g.cpu()], 1.0)
+    with pytest.raises(RuntimeError):
+        clip_grad_norm_([g], 1.0, out=[g.cpu()])

@@ -1,0 +1,250 @@
+"""GPU: log probabilities of given tokens with entropy and top alternatives, forward and gradient,
+against the 64-bit formulas and differences: odd vocabularies, strided rows, ties, -inf columns and rows,
+NaN and +inf, targets out of range."""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import serving_ref as ref
+from quantumdlblocks_b200 import token_logprobs
+from quantumdlblocks_b200.kernels import flash_born as fbm
+
+pytestmark = pytest.mark.gpu
+
+if not torch.cuda.is_available():
+    pytest.skip("CUDA device required", allow_module_level=True)
+
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+TYPES = pytest.mark.parametrize("dtype", [BF16, F16, F32], ids=["bf16", "fp16", "fp32"])
+
+
+def make(N, V, dtype, masked=0, seed=0, std=3.0):
+    g = torch.Generator().manual_seed(seed + N + V)
+    x = (torch.randn(N, V, generator=g) * std).to(dtype)
+    if masked:
+        x[:, V - masked:] = -math.inf
+    t = torch.randint(0, V - masked, (N,), generator=g)
+    return x.cuda(), t.cuda()
+
+
+def check_forward(r, x, t, K):
+    assert fbm.device_status() == (0, 0)
+    logp, ent, top, order = ref.logprobs(x, t, K)
+    big = float(x.float()[x.float().isfinite()].abs().max()) if x.float().isfinite().any() else 1.0
+    # x - lse rounds at the size of its terms; the sum of exponentials has a relative error of a few roundings
+    for got, want, tol in ((r.logp, logp, 1e-6 * (8 + 2 * big)), (r.entropy, ent, 1e-5 * (1 + math.log(x.shape[1]))),
+                           (r.top_logp, top, 1e-6 * (8 + 2 * big))):
+        assert got.dtype == F32 and got.shape == want.shape
+        assert torch.equal(got.isnan(), want.isnan()), (got, want)
+        inf = want.isinf()
+        assert torch.equal(got[inf].double(), want[inf])
+        fin = want.isfinite()
+        if fin.any():
+            assert float((got.double() - want)[fin].abs().max()) <= tol
+    assert r.top_index.dtype == torch.int64 and torch.equal(r.top_index, order)
+
+
+SHAPES = [(1, 1, 0), (3, 2, 0), (5, 7, 3), (2, 64, 0), (37, 259, 59), (4, 1000, 333), (3, 4099, 0), (2, 50257, 0),
+          (2, 50304, 47), (1, 131075, 0), (200, 513, 0)]
+
+
+@TYPES
+@pytest.mark.parametrize("N,V,masked", SHAPES)
+@pytest.mark.parametrize("K", [0, 1, 5, 20, 64])
+def test_forward_matches_formula(N, V, masked, K, dtype):
+    K = min(K, V)
+    x, t = make(N, V, dtype, masked)
+    r = token_logprobs(x, t, top_k=K)
+    check_forward(r, x, t, K)
+
+
+@TYPES
+def test_ties_go_to_the_lowest_index(dtype):
+    for V in (100, 5000, 50257):
+        x = torch.zeros(3, V, dtype=dtype, device="cuda")  # all equal
+        x[1, V // 2:] = 1.0  # half of them equal and above
+        x[2, ::7] = 2.0
+        x[2, 5] = -0.0  # equal to 0
+        t = torch.tensor([0, V - 1, 7], device="cuda")
+        for K in (1, 33, 64):
+            check_forward(token_logprobs(x, t, top_k=K), x, t, K)
+
+
+@TYPES
+@pytest.mark.parametrize("pattern", ["sorted", "reversed", "one thread's", "clustered"])
+def test_top_where_the_largest_lie_together(pattern, dtype):
+    """The largest values next to one another, or at any fixed distance: no split of a row may count on their spread."""
+    V, K = 40000, 40
+    base = torch.linspace(-4, 0, V).to(dtype).cuda()
+    x = torch.stack([base if pattern == "sorted" else base.flip(0)] * 2)
+    if pattern in ("one thread's", "clustered"):
+        x = torch.full((12, V), -1.0, dtype=dtype, device="cuda")
+        for i, step in enumerate([1, 8, 32, 64, 128, 256, 512, 1024, 2048, 4096, 8192, 16384]):
+            cols = torch.arange(3, V, step, device="cuda") if pattern == "one thread's" else torch.arange(V // 2, V // 2 + 100, device="cuda")
+            x[i, cols] = 1.0 + torch.rand(len(cols), generator=torch.Generator(device="cuda").manual_seed(i), device="cuda").to(dtype)
+    t = torch.zeros(x.shape[0], dtype=torch.int64, device="cuda")
+    check_forward(token_logprobs(x, t, top_k=K), x, t, K)
+
+
+@TYPES
+def test_rows_without_a_distribution(dtype):
+    """All -inf, NaN, +inf: that row is NaN, and no other; the order still says what is there."""
+    V = 300
+    x, t = make(6, V, dtype)
+    x[1] = -math.inf
+    x[2, 17] = math.nan
+    x[3, 250] = math.inf
+    x[4, 5:] = -math.inf  # fewer finite columns than alternatives
+    t[4] = 2
+    for K in (0, 4, 9):
+        r = token_logprobs(x, t, top_k=K)
+        check_forward(r, x, t, K)
+        assert r.logp[1:4].isnan().all() and r.entropy[1:4].isnan().all()
+        assert r.logp[[0, 4, 5]].isfinite().all() and r.entropy[[0, 4, 5]].isfinite().all()
+    y = torch.full((2, V), -math.inf, dtype=dtype, device="cuda")
+    y[0, 3] = 0.5  # a certain token: log probability 0, entropy 0
+    y[1, 9] = math.nan  # NaN among nothing
+    r = token_logprobs(y, torch.tensor([3, 9], device="cuda"), top_k=2)
+    assert r.logp[0] == 0 and r.entropy[0] == 0 and r.top_index[0, 0] == 3 and r.top_logp[0, 1] == -math.inf
+    assert r.logp[1].isnan() and r.entropy[1].isnan() and r.top_index[1, 0] == 9
+
+
+@TYPES
+def test_strides_and_index_types(dtype):
+    x, t = make(9, 1003, dtype)
+    wide = torch.full((9, 1100), math.nan, dtype=dtype, device="cuda")
+    wide[:, 5:1008] = x
+    want = token_logprobs(x, t, top_k=3)
+    for view in (wide[:, 5:1008], x.t().contiguous().t()):  # unaligned rows further apart; columns strided
+        got = token_logprobs(view, t.to(torch.int32), top_k=3)
+        for a, b in zip(got, want):
+            torch.testing.assert_close(a, b, rtol=1e-6, atol=1e-6)
+    one = token_logprobs(x[:1].expand(4, 1003), t[:4], top_k=1)
+    check_forward(one, x[:1].expand(4, 1003), t[:4], 1)
+    empty = token_logprobs(x[:0], t[:0], top_k=2)
+    assert empty.logp.shape == (0,) and empty.top_index.shape == (0, 2)
+
+
+@TYPES
+@pytest.mark.parametrize("N,V,masked", [(1, 1, 0), (5, 7, 3), (37, 259, 59), (3, 4099, 0), (2, 50304, 47), (3, 50257, 0), (150, 640, 0)])
+@pytest.mark.parametrize("K", [0, 6])
+def test_gradient_matches_formula(N, V, masked, K, dtype):
+    K = min(K, V - masked)
+    x, t = make(N, V, dtype, masked)
+    g = torch.Generator(device="cuda").manual_seed(V)
+    gl, ge = (torch.randn(N, generator=g, device="cuda") for _ in range(2))
+    gt = torch.randn(N, K, generator=g, device="cuda")
+    leaf = x.clone().requires_grad_(True)
+    r = token_logprobs(leaf, t, top_k=K)
+    assert not r.top_index.requires_grad
+    (got,) = torch.autograd.grad([r.logp, r.entropy, r.top_logp], [leaf], [gl, ge, gt])
+    assert fbm.device_status() == (0, 0) and got.dtype == dtype and got.shape == x.shape
+    want = ref.logprobs_grad(x, t, r.top_index, gl, ge, gt)
+    # p has the relative error of exp over x - lse (1e-5 at these sizes); its factor is at most `size`
+    size = (gl.abs() + gt.abs().sum(1) + ge.abs() * (30 + math.log(V))).double()[:, None]
+    p = torch.softmax(x.double(), dim=1)
+    tol = ref.ROUND[dtype] * 1.01 * want.abs() + 2e-5 * size * p + 3e-7 * size + (6e-8 if dtype == F16 else 0.0)
+    assert bool(((got.double() - want).abs() <= tol).all())
+    if masked:
+        assert torch.all(got[:, V - masked:] == 0)
+
+
+@TYPES
+def test_each_gradient_alone_and_strided(dtype):
+    x, t = make(11, 515, dtype, 13)
+    g = torch.randn(11, 3, device="cuda")
+    zero, none = torch.zeros(11, device="cuda"), torch.zeros(11, 4, device="cuda")
+    wide = torch.zeros(11, 600, dtype=dtype, device="cuda")
+    wide[:, 1:516] = x
+    for which in range(3):
+        for base in (x, wide[:, 1:516]):
+            leaf = base.detach().requires_grad_(True)
+            r = token_logprobs(leaf, t, top_k=4)
+            out, up = [(r.logp, g[:, 0]), (r.entropy, g[:, 1]), (r.top_logp, g[:, 2:].expand(11, 4))][which]
+            (got,) = torch.autograd.grad([out], [leaf], [up])
+            args = [zero, zero, none]
+            args[which] = up
+            want = ref.logprobs_grad(x, t, r.top_index, *args)
+            size = float(up.abs().sum(-1).max() if which == 2 else up.abs().max()) * 40
+            assert bool(((got.double() - want).abs() <= ref.ROUND[dtype] * 1.01 * want.abs() + 2e-5 * size * torch.softmax(x.double(), 1) + 3e-7 * size).all())
+
+
+def test_gradient_matches_differences():
+    """d/dh of L(x + h d) at 0 in float32 through the op itself: L rounds at about 1e-6 |L|, the second-order
+    term falls with h^2; h = 2e-2 leaves both under 1e-3."""
+    x, t = make(6, 777, F32, 20, std=1.5)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    gl, ge = (torch.randn(6, generator=g, device="cuda") for _ in range(2))
+    gt = torch.randn(6, 3, generator=g, device="cuda")
+    leaf = x.clone().requires_grad_(True)
+    r = token_logprobs(leaf, t, top_k=3)
+    order = r.top_index.clone()
+    (dx,) = torch.autograd.grad([r.logp, r.entropy, r.top_logp], [leaf], [gl, ge, gt])
+    d = torch.randn(x.shape, generator=g, device="cuda")
+
+    def loss(y):
+        r = token_logprobs(y, t, top_k=0)
+        # the alternatives as fixed columns: their order changes along d, their derivative is that of the columns
+        cols = torch.stack([token_logprobs(y, order[:, i]).logp for i in range(3)], dim=1)
+        return ((gl * r.logp).double().sum() + (ge * r.entropy).double().sum() + (gt * cols).double().sum())
+
+    h = 2e-2
+    slope = float((loss(x + h * d.where(x.isfinite(), 0.0)) - loss(x - h * d.where(x.isfinite(), 0.0))) / (2 * h))
+    want = float((dx.double() * d.double()).sum())
+    assert abs(slope - want) <= 2e-3 * max(1.0, abs(want)), (slope, want)
+
+
+@TYPES
+def test_targets_out_of_range(dtype):
+    x, t = make(5, 130, dtype)
+    t[1], t[3] = -100, 130
+    leaf = x.clone().requires_grad_(True)
+    r = token_logprobs(leaf, t)
+    assert torch.equal(r.logp.isnan().cpu(), torch.tensor([False, True, False, True, False])) and r.entropy.isfinite().all()
+    g = torch.tensor([1.0, 0.0, 2.0, 1.0, 0.0], device="cuda")
+    (dx,) = torch.autograd.grad([r.logp], [leaf], [g])
+    # a row whose logp is not used gets no gradient; one that is used gets NaN, as its logp is
+    assert torch.all(dx[[1, 4]] == 0) and dx[3].isnan().all() and dx[[0, 2]].isfinite().all()
+
+
+@TYPES
+def test_gradient_of_rows_without_a_distribution(dtype):
+    x, t = make(4, 97, dtype)
+    x[1] = -math.inf
+    x[2, 3] = math.nan
+    leaf = x.clone().requires_grad_(True)
+    r = token_logprobs(leaf, t)
+    (dx,) = torch.autograd.grad([r.logp.sum() + r.entropy.sum()], [leaf])
+    assert dx[1:3].isnan().all() and dx[[0, 3]].isfinite().all()
+
+
+def test_runs_on_the_current_stream_and_repeats():
+    x, t = make(64, 5003, BF16)
+    want = token_logprobs(x, t, top_k=7)
+    y = torch.zeros_like(x)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)
+        y.copy_(x)
+        got = token_logprobs(y, t, top_k=7)
+        got = [a.clone() for a in got]
+    side.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+def test_refusals():
+    x, t = make(4, 64, BF16)
+    for kw in (dict(logits=x[0]), dict(logits=x.double()), dict(logits=x.to(torch.int32)), dict(logits=x[:, :0]),
+               dict(targets=t[:3]), dict(targets=t.float()), dict(targets=t > 1), dict(top_k=-1), dict(top_k=65)):
+        with pytest.raises(ValueError):
+            token_logprobs(**{**dict(logits=x, targets=t), **kw})
+    with pytest.raises(ValueError):
+        token_logprobs(x[:, :5], t % 5, top_k=6)
+    for kw in (dict(logits=x.cpu()), dict(targets=t.cpu())):
+        with pytest.raises(RuntimeError):
+            token_logprobs(**{**dict(logits=x, targets=t), **kw})

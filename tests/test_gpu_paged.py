@@ -1,0 +1,360 @@
+"""GPU: Born attention of one new token over a paged cache, and the kernel that fills the cache, against
+the 64-bit formulas: lengths of zero and one, pages that end inside a tile, grouped heads, windows, strided
+pages and queries, table entries and page rows that must not be used (NaN in them), offsets past 32 bits."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+import serving_ref as ref
+from quantumdlblocks_b200 import paged_born_attention, paged_qkv_write
+from quantumdlblocks_b200.kernels import flash_born as fbm
+from quantumdlblocks_b200.kernels.prologue import qkv_rope_l2norm, rope_tables
+
+pytestmark = pytest.mark.gpu
+
+if not torch.cuda.is_available():
+    pytest.skip("CUDA device required", allow_module_level=True)
+
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+
+
+def make_cache(lens, Hkv, D, page, dtype, seed=0, token_major=False, spare=2, width=None):
+    """Pages in random order; NaN wherever no token is; unused table entries far out of range."""
+    g = torch.Generator().manual_seed(seed)
+    count = [-(-n // page) for n in lens]
+    P = sum(count) + spare
+    shape = (P, page, Hkv, D) if token_major else (P, Hkv, page, D)
+    k, v = (torch.full(shape, float("nan"), dtype=dtype) for _ in range(2))
+    if token_major:
+        k, v = k.transpose(1, 2), v.transpose(1, 2)
+    order = torch.randperm(P, generator=g).tolist()
+    table = torch.full((len(lens), max(1, *count) if width is None else width), 1 << 30, dtype=torch.int32)
+    for s, n in enumerate(lens):
+        for i in range(count[s]):
+            pg, rows = order.pop(), min(page, n - i * page)
+            table[s, i] = pg
+            x = torch.randn(Hkv, rows, D, generator=g)
+            k[pg, :, :rows] = (x / x.norm(dim=-1, keepdim=True)).to(dtype)
+            v[pg, :, :rows] = torch.randn(Hkv, rows, D, generator=g).to(dtype)
+    # .cuda() keeps the strides of the transposed view
+    return k.cuda(), v.cuda(), table.cuda(), torch.tensor(lens, dtype=torch.int32, device="cuda")
+
+
+def make_q(S, H, D, dtype, seed=1):
+    x = torch.randn(S, H, D, generator=torch.Generator().manual_seed(seed))
+    return (x / x.norm(dim=-1, keepdim=True)).to(dtype).cuda()
+
+
+def check(got, want, v, dtype):
+    assert fbm.device_status() == (0, 0)
+    err = (got.double() - want).abs()
+    worst = float((err - ref.attention_bound(want, v, dtype)).max()) if err.numel() else 0.0
+    assert worst <= 0.0, (worst, float(err.max()))
+
+
+CASES = [
+    # H, Hkv, D, page, lens, window
+    (16, 16, 64, 16, [1], 0),
+    (16, 16, 64, 16, [0, 1, 15, 16, 17, 31, 100, 1024], 0),
+    (4, 1, 64, 64, [0, 0, 0], 0),
+    (8, 2, 128, 16, [129, 1, 640, 0, 255], 0),
+    (8, 1, 128, 64, [5000], 0),
+    (5, 5, 64, 1, [7, 40], 0),
+    (6, 3, 64, 24, [300, 77, 24, 25], 0),
+    (20, 1, 64, 16, [333, 16], 0),
+    (40, 2, 128, 32, [95, 2000], 0),
+    (16, 1, 64, 128, [127, 128, 129, 1500], 0),
+    (6, 3, 64, 24, [300, 77, 0, 25], 1),
+    (4, 4, 128, 16, [3000, 10, 400], 384),
+    (3, 3, 64, 16, [1000, 3], 5000),
+    (6, 2, 48, 24, [0, 100, 700], 0),
+    (2, 1, 20, 16, [50, 1], 0),
+    (3, 3, 7, 5, [33, 6], 4),
+    (4, 2, 256, 16, [70, 300], 0),
+    (9, 3, 80, 32, [640, 31], 100),
+    (1, 1, 1, 3, [10], 0),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32], ids=["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("case", CASES, ids=lambda c: "-".join(str(x) for x in c[:4]) + f"-n{max(c[4])}-w{c[5]}")
+def test_paged_attention_matches_formula(case, dtype):
+    H, Hkv, D, page, lens, window = case
+    k, v, table, n = make_cache(lens, Hkv, D, page, dtype)
+    q = make_q(len(lens), H, D, dtype)
+    scale = torch.linspace(4.0, 10.0, H, device="cuda")
+    got = paged_born_attention(q, k, v, table, n, scale, window_size=window)
+    assert got.shape == q.shape and got.dtype == dtype
+    check(got, ref.paged_attention(q, k, v, table, lens, scale, window=window), v, dtype)
+    # the same call again gives the same bits
+    assert torch.equal(got, paged_born_attention(q, k, v, table, n, scale, window_size=window))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32], ids=["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("H,Hkv,D,page", [(8, 4, 64, 16), (4, 4, 128, 48), (4, 2, 40, 16)])
+def test_strides_and_scale_forms(H, Hkv, D, page, dtype):
+    lens = [200, 33, 1]
+    k, v, table, n = make_cache(lens, Hkv, D, page, dtype, token_major=True)
+    assert not k.is_contiguous()
+    wide = make_q(len(lens), H, 2 * D + 3, dtype)
+    for q in (wide[:, :, :D], wide[:, :, 1:D + 1], wide[:, :, ::2][:, :, :D]):  # aligned, unaligned, inner stride 2
+        for scale, per_head in ((8.0, [8.0] * H), (torch.tensor(6.5, device="cuda"), [6.5] * H),
+                                (torch.linspace(1, 9, H, device="cuda").view(1, H, 1, 1), torch.linspace(1, 9, H).tolist())):
+            want = ref.paged_attention(q, k, v, table, lens, per_head, eps=1e-3)
+            check(paged_born_attention(q, k, v, table, n, scale, eps=1e-3), want, v, dtype)
+    # a table whose columns are strided, and lengths that are
+    t2 = table.repeat_interleave(2, dim=1)[:, ::2]
+    n2 = n.repeat_interleave(3)[::3]
+    q = wide[:, :, :D]
+    want = ref.paged_attention(q, k, v, table, lens, [8.0] * H)
+    check(paged_born_attention(q, k, v, t2, n2, 8.0), want, v, dtype)
+
+
+@pytest.mark.parametrize("dtype,D", [(BF16, 64), (F16, 128), (F32, 64), (BF16, 48)])
+def test_unaligned_pages(dtype, D):
+    """Pages whose base and rows are not 16-byte aligned."""
+    lens, page, Hkv = [150, 20], 16, 2
+    k, v, table, n = make_cache(lens, Hkv, D, page, dtype)
+    P = k.shape[0]
+    store = torch.full((2, P * Hkv * page * (D + 1) + 1), float("nan"), dtype=dtype, device="cuda")
+    views = [s[1:].view(P, Hkv, page, D + 1)[..., :D] for s in store]
+    views[0].copy_(k)
+    views[1].copy_(v)
+    q = make_q(2, 4, D, dtype)
+    want = ref.paged_attention(q, k, v, table, lens, [8.0] * 4)
+    check(paged_born_attention(q, views[0], views[1], table, n, 8.0), want, v, dtype)
+
+
+@pytest.mark.parametrize("dtype,D", [(BF16, 64), (F32, 64)])
+def test_out_of_range_lengths_and_table_entries(dtype, D):
+    """Lengths past the table are cut to it, negative ones are empty; entries outside the pages hold no keys."""
+    k, v, table, n = make_cache([64, 64, 64, 64], 2, D, 16, dtype)
+    table[1, 1], table[2, 0], table[2, 3] = -1, k.shape[0], 1 << 30
+    q = make_q(4, 4, D, dtype)
+    lens = torch.tensor([1 << 30, 64, 50, -5], dtype=torch.int32, device="cuda")
+    got = paged_born_attention(q, k, v, table, lens, 8.0)
+    check(got, ref.paged_attention(q, k, v, table, lens.tolist(), [8.0] * 4), v, dtype)
+    assert torch.all(got[3] == 0)
+    # no table columns, or no pages at all: no keys
+    assert torch.all(paged_born_attention(q, k, v, table[:, :0], lens, 8.0) == 0)
+    assert torch.all(paged_born_attention(q, k[:0], v[:0], table, lens, 8.0) == 0)
+    assert paged_born_attention(q[:0], k, v, table[:0], lens[:0], 8.0).shape == (0, 4, D)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32], ids=["bf16", "fp16", "fp32"])
+def test_keys_without_weight_nan_and_inf(dtype):
+    """A row of non-positive overlaps is 0 (eps 0 included); a NaN key that is used makes its heads NaN, and no others."""
+    D, page = 64, 16
+    k, v, table, n = make_cache([40, 40], 2, D, page, dtype)
+    q = make_q(2, 4, D, dtype)
+    pages = table[0, :3].long()
+    k[pages, 0] = -q[0, 0].clone()  # every overlap of (sequence 0, head 0) negative
+    q[0, 1] = q[0, 0]
+    for eps in (1e-12, 0.0):
+        got = paged_born_attention(q, k, v, table, n, 8.0, eps=eps)
+        assert torch.all(got[0, :2] == 0)
+        check(got, ref.paged_attention(q, k, v, table, [40, 40], [8.0] * 4, eps=eps), v, dtype)
+    k[table[1, 0].long(), 1, 3] = float("nan")
+    got = paged_born_attention(q, k, v, table, n, 8.0)
+    assert torch.isnan(got[1, 2:]).all() and torch.isfinite(got[0]).all() and torch.isfinite(got[1, :2]).all()
+    k[table[1, 0].long(), 1, 3] = 0.0
+    v[table[1, 0].long(), 1, 4] = float("inf")
+    got = paged_born_attention(q, k, v, table, n, 8.0)
+    assert not torch.isfinite(got[1, 2:]).all() and torch.isfinite(got[1, :2]).all()
+
+
+def test_large_scores_keep_fp16_finite():
+    """p = a^2 far above fp16's largest value (65504), and far below its smallest."""
+    k, v, table, n = make_cache([100, 7], 1, 64, 16, F16)
+    q = make_q(2, 2, 64, F16)
+    for scale in (2000.0, 1e-6):
+        want = ref.paged_attention(q, k, v, table, [100, 7], [scale] * 2, eps=0.0)
+        got = paged_born_attention(q, k, v, table, n, scale, eps=0.0)
+        check(got, want, v, F16)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "fp32"])
+def test_offsets_past_32_bits(dtype):
+    """Pages whose element offsets pass 2^31, used through the table's last entries."""
+    Hkv, page, D = 8, 64, 128
+    per = Hkv * page * D
+    P = (1 << 31) // per + 20
+    k, v = (torch.empty((P, Hkv, page, D), dtype=dtype, device="cuda") for _ in range(2))
+    last = torch.arange(P - 5, P, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn(5, Hkv, page, D, generator=g, device="cuda")
+    k[last], v[last] = (x / x.norm(dim=-1, keepdim=True)).to(dtype), torch.randn(5, Hkv, page, D, generator=g, device="cuda").to(dtype)
+    table = last.flip(0).to(torch.int32)[None]
+    q = make_q(1, 8, D, dtype)
+    got = paged_born_attention(q, k, v, table, torch.tensor([300], dtype=torch.int32, device="cuda"), 8.0)
+    rows = last.flip(0).long()
+    want = ref.paged_attention(q, k[rows], v[rows], torch.arange(5, device="cuda")[None], [300], [8.0] * 8)
+    check(got, want, v[rows], dtype)
+    # and the write reaches them
+    qkv = torch.randn(2, 3 * 8 * D, generator=g, device="cuda").to(dtype)
+    cos, sin = rope_tables(4, D, device="cuda")
+    slots = torch.tensor([P * page - 1, P * page], device="cuda")
+    paged_qkv_write(qkv, cos, sin, torch.tensor([0, 1], device="cuda"), slots, k, v, 8)
+    assert torch.equal(v[P - 1, :, page - 1], qkv[0].view(24, D)[16:])
+
+
+def test_runs_on_the_current_stream():
+    """Inputs made on a side stream are used there: the call is ordered behind them, and the result too."""
+    lens = [700, 900]
+    k, v, table, n = make_cache(lens, 4, 64, 16, BF16)
+    q = make_q(2, 8, 64, BF16)
+    want = ref.paged_attention(q, k, v, table, lens, [8.0] * 8)
+    k0, q0 = k.clone(), torch.zeros_like(q)
+    k.fill_(float("nan"))
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)
+        k.copy_(k0)
+        q0.copy_(q)
+        got = paged_born_attention(q0, k, v, table, n, 8.0)
+        got = got * 1
+    side.synchronize()
+    check(got, want, v, BF16)
+
+
+def test_decode_replays_from_a_graph():
+    """Captured once, replayed with other lengths and other keys in the same buffers."""
+    lens = [300, 1, 77]
+    k, v, table, n = make_cache(lens, 2, 64, 16, BF16, width=40)
+    q = make_q(3, 4, 64, BF16)
+    paged_born_attention(q, k, v, table, n, 8.0)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = paged_born_attention(q, k, v, table, n, 8.0)
+    for now in (lens, [17, 0, 600]):
+        k2, v2, t2, n2 = make_cache(now, 2, 64, 16, BF16, seed=sum(now), width=40, spare=60 - sum(-(-x // 16) for x in now))
+        P = min(k.shape[0], k2.shape[0])
+        assert int(t2[t2 < (1 << 30)].max()) < 60
+        if k.shape[0] < 60:  # the captured buffers hold fewer pages: keep the first problem only
+            if now is not lens:
+                break
+            graph.replay()
+            check(out, ref.paged_attention(q, k, v, table, now, [8.0] * 4), v, BF16)
+            continue
+        k[:P].copy_(k2[:P])
+        v[:P].copy_(v2[:P])
+        table.copy_(t2)
+        n.copy_(n2)
+        graph.replay()
+        check(out, ref.paged_attention(q, k, v, table, now, [8.0] * 4), v, BF16)
+
+
+# ------------------------------------------------------------------------------------------
+# the write
+# ------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [BF16, F16, F32], ids=["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("N,H,Hkv,D,page", [(1, 16, 16, 64, 16), (37, 8, 2, 128, 64), (5, 3, 3, 48, 24), (130, 4, 1, 64, 1),
+                                            (9, 2, 2, 2, 7), (4, 6, 3, 20, 16), (3, 4, 4, 256, 16), (0, 4, 2, 64, 16)])
+@pytest.mark.parametrize("layout", ["plain", "strided"])
+def test_write_matches_formula(N, H, Hkv, D, page, layout, dtype):
+    g = torch.Generator().manual_seed(N + D)
+    P = -(-max(N, 1) // page) + 2
+    width = (H + 2 * Hkv) * D
+    qkv = (torch.randn(N, width + 5, generator=g) * 2).to(dtype).cuda()
+    qkv = qkv[:, 3:3 + width] if layout == "strided" else qkv[:, :width].contiguous()
+    shape = (P, page, Hkv, D) if layout == "strided" else (P, Hkv, page, D)
+    k, v = (torch.randn(shape, generator=g).to(dtype).cuda() for _ in range(2))
+    if layout == "strided":
+        k, v = k.transpose(1, 2), v.transpose(1, 2)
+    cos, sin = rope_tables(50, D, device="cuda")
+    pos = torch.randint(0, 50, (N,), generator=g).cuda()
+    slots = torch.randperm(P * page, generator=g)[:N].cuda()
+    if N > 3:
+        slots[1], slots[2], pos[3] = -1, P * page, 50
+    want = ref.qkv_write(qkv, cos, sin, pos, slots, k, v, H)
+    before = (k.clone(), v.clone())
+    q, k_new, v_new = paged_qkv_write(qkv, cos, sin, pos, slots, k, v, H, return_kv=True)
+    assert fbm.device_status() == (0, 0)
+    for got, w in zip((q, k_new, k), (want[0], want[1], want[3])):
+        # fp32 arithmetic on unit vectors, then one rounding
+        bad = (got.double() - w).abs() > 1.01 * ref.ROUND[dtype] * w.abs() + 2e-5
+        assert not bad.any() and torch.equal(got.isnan(), w.isnan())
+    assert torch.equal(v.double(), want[4]) and torch.equal(v_new.double(), want[2])
+    # slots that no token went to are as they were
+    free = torch.ones(P * page, dtype=torch.bool, device="cuda")
+    free[slots[(slots >= 0) & (slots < P * page)]] = False
+    for now, old in zip((k, v), before):
+        assert torch.equal(now.transpose(1, 2).reshape(P * page, -1)[free], old.transpose(1, 2).reshape(P * page, -1)[free])
+    # the other index types, and the form that returns Q alone
+    q2 = paged_qkv_write(qkv, cos, sin, pos.to(torch.int32), slots.to(torch.int32), k, v, H)
+    assert torch.equal(q2.nan_to_num(9.0), q.nan_to_num(9.0))
+
+
+def test_write_then_attend_is_the_prompt_attention():
+    """Tokens written one at a time and attended one at a time give the rows of the causal prompt attention."""
+    T, H, D, page = 70, 4, 64, 16
+    g = torch.Generator().manual_seed(5)
+    qkv = torch.randn(T, 3 * H * D, generator=g).to(BF16).cuda()
+    cos, sin = rope_tables(T, D, device="cuda")
+    k, v = (torch.full((8, H, page, D), float("nan"), dtype=BF16, device="cuda") for _ in range(2))
+    table = torch.tensor([[6, 1, 3, 0, 7]], dtype=torch.int32, device="cuda")
+    rows = []
+    for t in range(T):
+        slot = table[0, t // page].long()[None] * page + t % page
+        q = paged_qkv_write(qkv[t:t + 1], cos, sin, torch.tensor([t], device="cuda"), slot, k, v, H)
+        rows.append(paged_born_attention(q, k, v, table, torch.tensor([t + 1], dtype=torch.int32, device="cuda"), 8.0))
+    got = torch.cat(rows)
+    q, kk, vv = qkv_rope_l2norm(qkv[None], cos, sin, H)
+    want = fbm.flash_born_attention(q, kk, vv, 8.0)[0].transpose(0, 1)
+    assert float((got.float() - want.float()).abs().max()) <= 2e-2 * float(want.float().abs().max())
+
+
+# ------------------------------------------------------------------------------------------
+# refusals
+# ------------------------------------------------------------------------------------------
+def test_attention_refusals():
+    k, v, table, n = make_cache([20, 5], 2, 64, 16, BF16)
+    q = make_q(2, 4, 64, BF16)
+
+    def call(**kw):
+        a = dict(q=q, k_pages=k, v_pages=v, block_table=table, seq_lens=n, scale=8.0)
+        a.update(kw)
+        return paged_born_attention(**a)
+
+    call()
+    for kw in (dict(q=q[0]), dict(q=q.float()), dict(q=q.double()), dict(q=q[:, :3]), dict(q=q[:, :, :32]),
+               dict(k_pages=k[:1]), dict(k_pages=k.float(), v_pages=v.float()), dict(v_pages=v.transpose(2, 3)),
+               dict(k_pages=k[..., ::2], v_pages=v[..., ::2], q=q[..., :32]),
+               dict(block_table=table.long()), dict(block_table=table[:1]), dict(block_table=table[0]),
+               dict(seq_lens=n.long()), dict(seq_lens=n[:1]), dict(scale=torch.ones(3, device="cuda")),
+               dict(eps=-1.0), dict(eps=float("nan")), dict(window_size=-1)):
+        with pytest.raises(ValueError):
+            call(**kw)
+    for kw in (dict(q=q.cpu()), dict(k_pages=k.cpu()), dict(block_table=table.cpu()), dict(seq_lens=n.cpu()),
+               dict(q=q.clone().requires_grad_(True))):
+        with pytest.raises(RuntimeError):
+            call(**kw)
+    with torch.no_grad():
+        call(q=q.clone().requires_grad_(True))
+
+
+def test_write_refusals():
+    cos, sin = rope_tables(10, 64, device="cuda")
+    k, v = (torch.zeros((2, 2, 16, 64), dtype=BF16, device="cuda") for _ in range(2))
+    qkv = torch.zeros((3, 8 * 64), dtype=BF16, device="cuda")
+    i = torch.arange(3, device="cuda")
+
+    def call(**kw):
+        a = dict(qkv=qkv, cos=cos, sin=sin, positions=i, slots=i, k_pages=k, v_pages=v, heads=4)
+        a.update(kw)
+        return paged_qkv_write(**a)
+
+    call()
+    for kw in (dict(qkv=qkv[0]), dict(qkv=qkv[:, :64]), dict(qkv=qkv.float()), dict(heads=3), dict(heads=0),
+               dict(positions=i[:2]), dict(slots=i.float()), dict(cos=cos[:, :5]), dict(sin=sin[:4]),
+               dict(cos=cos.double(), sin=sin.double()), dict(v_pages=v[:1]), dict(eps=-1.0),
+               dict(k_pages=k[..., ::2], v_pages=v[..., ::2])):
+        with pytest.raises(ValueError):
+            call(**kw)
+    for kw in (dict(qkv=qkv.cpu()), dict(v_pages=v.cpu()), dict(slots=i.cpu()), dict(cos=cos.cpu()),
+               dict(qkv=qkv.clone().requires_grad_(True))):
+        with pytest.raises(RuntimeError):
+            call(**kw)

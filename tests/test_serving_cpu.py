@@ -1,0 +1,186 @@
+"""The serving and policy-training operators without a GPU: struct layouts against the header, host-side
+validation status codes, refusal of CPU tensors, and the plain 64-bit formulas of their GPU tests against
+torch's own functions."""
+from __future__ import annotations
+
+import ctypes
+import math
+import os
+import shutil
+import subprocess
+
+import pytest
+import torch
+
+import serving_ref as ref
+from quantumdlblocks_b200 import (_lib, clip_grad_norm_, grad_norm, paged_born_attention, paged_qkv_write,
+                                  token_logprobs)
+
+HEADER = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "flashborn_b200.h")
+STRUCTS = {"fb_paged_args": _lib.FbPagedArgs, "fb_paged_write_args": _lib.FbPagedWriteArgs,
+           "fb_logprob_args": _lib.FbLogprobArgs, "fb_clip_args": _lib.FbClipArgs}
+
+
+@pytest.mark.skipif(shutil.which("gcc") is None, reason="gcc needed for the layout probe")
+def test_struct_layouts_match_header(tmp_path):
+    src = ["#include <stdio.h>", "#include <stddef.h>", f'#include "{HEADER}"', "int main(void){"]
+    for name, cls in STRUCTS.items():
+        src.append(f'printf("{name} size %zu\\n", sizeof({name}));')
+        src += [f'printf("{name} {f[0]} %zu\\n", offsetof({name}, {f[0]}));' for f in cls._fields_]
+    src += [f'printf("x top_k %d\\n", FB_MAX_TOP_K);', "return 0;}"]
+    c, exe = tmp_path / "probe.c", tmp_path / "probe"
+    c.write_text("\n".join(src))
+    subprocess.run(["gcc", "-std=c99", str(c), "-o", str(exe)], check=True)
+    out = subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.split("\n")
+    got = {tuple(line.split()[:2]): int(line.split()[2]) for line in out if line.strip()}
+    assert got.pop(("x", "top_k")) == _lib.FB_MAX_TOP_K
+    for name, cls in STRUCTS.items():
+        assert got.pop((name, "size")) == ctypes.sizeof(cls)
+        for f in cls._fields_:
+            assert got.pop((name, f[0])) == getattr(cls, f[0]).offset, (name, f[0])
+
+
+FAKE = 0x10000  # never dereferenced: validation fails, or nothing is launched
+
+
+def paged(**kw):
+    a = _lib.FbPagedArgs()
+    a.seqs, a.heads, a.kv_heads, a.head_dim, a.dtype = 2, 4, 2, 64, _lib.FB_BF16
+    a.page_size, a.num_pages, a.max_pages, a.eps, a.scale_value = 16, 8, 4, 1e-12, 8.0
+    for n in ("q", "k", "v", "out", "table", "lens"):
+        setattr(a, n, FAKE)
+    a.q_stride = a.out_stride = _lib._I64x3(256, 64, 1)
+    a.k_stride = a.v_stride = _lib._I64x4(2048, 1024, 64, 1)
+    a.table_stride = 4
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(head_dim=0), _lib.FB_ERR_SHAPE), (dict(head_dim=257), _lib.FB_ERR_SHAPE), (dict(seqs=-1), _lib.FB_ERR_SHAPE),
+    (dict(heads=5), _lib.FB_ERR_SHAPE), (dict(kv_heads=0), _lib.FB_ERR_SHAPE), (dict(page_size=0), _lib.FB_ERR_SHAPE),
+    (dict(page_size=1 << 20, max_pages=1 << 20), _lib.FB_ERR_SHAPE), (dict(dtype=3), _lib.FB_ERR_DTYPE),
+    (dict(window_size=-1), _lib.FB_ERR_ARG), (dict(eps=-1.0), _lib.FB_ERR_ARG), (dict(eps=math.nan), _lib.FB_ERR_ARG),
+    (dict(scale=FAKE, scale_numel=3), _lib.FB_ERR_ARG), (dict(q=None), _lib.FB_ERR_ARG), (dict(k=None), _lib.FB_ERR_ARG),
+    (dict(table=None), _lib.FB_ERR_ARG), (dict(lens=None), _lib.FB_ERR_ARG), (dict(out=None), _lib.FB_ERR_ARG),
+    (dict(k_stride=_lib._I64x4(2048, 1024, 64, 2)), _lib.FB_ERR_ALIGN),
+    (dict(v_stride=_lib._I64x4(2048, -1, 64, 1)), _lib.FB_ERR_ALIGN), (dict(seqs=0), _lib.FB_OK),
+])
+def test_paged_attention_validation(kw, code):
+    assert _lib.load().fb_paged_born_fwd(ctypes.byref(paged(**kw)), None) == code
+
+
+def test_null_arguments():
+    lib = _lib.load()
+    for name in ("fb_paged_born_fwd", "fb_paged_qkv_write", "fb_logprob_fwd", "fb_logprob_bwd", "fb_clip_grad_norm"):
+        assert getattr(lib, name)(None, None) == _lib.FB_ERR_ARG
+    assert lib.fb_paged_workspace_size(None) == 0 and lib.fb_clip_workspace_size(None) == 0
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(head_dim=63), _lib.FB_ERR_SHAPE), (dict(head_dim=258), _lib.FB_ERR_SHAPE), (dict(tokens=-1), _lib.FB_ERR_SHAPE),
+    (dict(heads=3), _lib.FB_ERR_SHAPE), (dict(dtype=9), _lib.FB_ERR_DTYPE), (dict(cos=None), _lib.FB_ERR_ARG),
+    (dict(slots=None), _lib.FB_ERR_ARG), (dict(k=None), _lib.FB_ERR_ARG), (dict(k_out=FAKE), _lib.FB_ERR_ARG),
+    (dict(eps=-1.0), _lib.FB_ERR_ARG), (dict(qkv_stride=-5), _lib.FB_ERR_ALIGN), (dict(tokens=0), _lib.FB_OK),
+])
+def test_paged_write_validation(kw, code):
+    a = _lib.FbPagedWriteArgs()
+    a.tokens, a.heads, a.kv_heads, a.head_dim, a.dtype = 3, 4, 2, 64, _lib.FB_F16
+    a.page_size, a.num_pages, a.rope_rows, a.eps, a.qkv_stride = 16, 8, 100, 1e-12, 512
+    for n in ("qkv", "cos", "sin", "positions", "slots", "k", "v", "q"):
+        setattr(a, n, FAKE)
+    a.k_stride = a.v_stride = _lib._I64x4(2048, 1024, 64, 1)
+    for k, v in kw.items():
+        setattr(a, k, v)
+    assert _lib.load().fb_paged_qkv_write(ctypes.byref(a), None) == code
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(rows=-1), _lib.FB_ERR_SHAPE), (dict(vocab=0), _lib.FB_ERR_SHAPE), (dict(ld=99), _lib.FB_ERR_SHAPE),
+    (dict(top_k=65), _lib.FB_ERR_SHAPE), (dict(top_k=-1), _lib.FB_ERR_SHAPE), (dict(vocab=5, top_k=6), _lib.FB_ERR_SHAPE),
+    (dict(dtype=-1), _lib.FB_ERR_DTYPE), (dict(logits=None), _lib.FB_ERR_ARG), (dict(logp=None), _lib.FB_ERR_ARG),
+    (dict(entropy=None), _lib.FB_ERR_ARG), (dict(top_index=None), _lib.FB_ERR_ARG), (dict(rows=0), _lib.FB_OK),
+])
+def test_logprob_validation(kw, code):
+    a = _lib.FbLogprobArgs()
+    a.rows, a.vocab, a.dtype, a.top_k, a.ld, a.grad_ld = 3, 100, _lib.FB_F32, 4, 100, 100
+    for n in ("logits", "targets", "logp", "entropy", "lse", "top_logp", "top_index"):
+        setattr(a, n, FAKE)
+    for k, v in kw.items():
+        setattr(a, k, v)
+    lib = _lib.load()
+    assert lib.fb_logprob_fwd(ctypes.byref(a), None) == code
+    if not kw:
+        assert lib.fb_logprob_bwd(ctypes.byref(a), None) == _lib.FB_ERR_ARG  # grad missing
+
+
+def test_clip_validation():
+    lib = _lib.load()
+
+    def call(n=2, numel=(4, 5), dtype=(0, 2), out_dtype=(0, 0), ptrs=(FAKE, FAKE), outs=(FAKE, FAKE), max_norm=1.0,
+             norm=FAKE, workspace=FAKE, bytes_less=0):
+        a = _lib.FbClipArgs()
+        keep = [(ctypes.c_void_p * 2)(*ptrs), (ctypes.c_void_p * 2)(*outs), (ctypes.c_int64 * 2)(*numel),
+                (ctypes.c_int32 * 2)(*dtype), (ctypes.c_int32 * 2)(*out_dtype)]
+        a.count, a.max_norm, a.eps, a.norm, a.workspace = n, max_norm, 1e-6, norm, workspace
+        a.grads, a.out, a.numel, a.dtype, a.out_dtype = (ctypes.cast(x, ctypes.c_void_p) for x in keep)
+        a.workspace_bytes = lib.fb_clip_workspace_size(ctypes.byref(a)) - bytes_less
+        return lib.fb_clip_grad_norm(ctypes.byref(a), None)
+
+    assert call(n=-1) == _lib.FB_ERR_SHAPE
+    assert call(numel=(4, -1)) == _lib.FB_ERR_SHAPE
+    assert call(dtype=(0, 7)) == _lib.FB_ERR_DTYPE
+    assert call(out_dtype=(1, 0)) == _lib.FB_ERR_DTYPE
+    assert call(ptrs=(FAKE, None)) == _lib.FB_ERR_ARG
+    assert call(outs=(FAKE, None)) == _lib.FB_ERR_ARG
+    assert call(max_norm=-1.0) == _lib.FB_ERR_ARG
+    assert call(norm=None) == _lib.FB_ERR_ARG
+    assert call(workspace=None) == _lib.FB_ERR_WORKSPACE
+    assert call(bytes_less=1) == _lib.FB_ERR_WORKSPACE
+
+
+def test_cpu_tensors_are_refused():
+    x = torch.zeros(2, 4, 64)
+    pages = torch.zeros(3, 4, 16, 64)
+    i = torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(RuntimeError):
+        paged_born_attention(x, pages, pages, i[:, None], i, 8.0)
+    with pytest.raises(RuntimeError):
+        paged_qkv_write(torch.zeros(2, 12 * 64), torch.zeros(5, 32), torch.zeros(5, 32), i, i, pages, pages, 4)
+    with pytest.raises(RuntimeError):
+        token_logprobs(torch.zeros(2, 10), torch.zeros(2, dtype=torch.int64))
+    with pytest.raises(RuntimeError):
+        clip_grad_norm_([torch.zeros(4)], 1.0)
+    with pytest.raises(RuntimeError):
+        grad_norm([torch.zeros(4)])
+
+
+def test_plain_formulas_against_torch():
+    """The 64-bit formulas that the GPU tests rest on, against torch's functions and autograd."""
+    g = torch.Generator().manual_seed(0)
+    x = torch.randn(5, 33, generator=g, dtype=torch.float64).requires_grad_(True)
+    t = torch.randint(0, 33, (5,), generator=g)
+    logp, ent, top, order = ref.logprobs(x, t, 4)
+    assert torch.allclose(-logp, torch.nn.functional.cross_entropy(x, t, reduction="none"))
+    dist = torch.distributions.Categorical(logits=x)
+    assert torch.allclose(ent, dist.entropy()) and torch.equal(order, x.topk(4).indices)
+    gl, ge, gt = torch.randn(5, generator=g), torch.randn(5, generator=g), torch.randn(5, 4, generator=g)
+    loss = (gl * dist.log_prob(t)).sum() + (ge * dist.entropy()).sum() + (gt * torch.log_softmax(x, 1).gather(1, order)).sum()
+    (want,) = torch.autograd.grad(loss, [x])
+    assert torch.allclose(ref.logprobs_grad(x, t, order, gl, ge, gt), want)
+    # attention: one sequence over pages in reverse order is the last row of the dense causal attention
+    from test_gpt_cpu import born_eager
+
+    q, k, v = (torch.randn(1, 2, 20, 8, generator=g) for _ in range(3))
+    dense = born_eager(q, k, v, 3.0)[0, :, -1].double()
+    pages = [y[0].reshape(2, 4, 5, 8).transpose(0, 1).flip(0).contiguous() for y in (k, v)]
+    table = torch.tensor([[3, 2, 1, 0]])
+    got = ref.paged_attention(q[0, :, -1][None], *pages, table, [20], [3.0, 3.0])[0]
+    assert torch.allclose(got, dense, atol=1e-5)
+    ps = [torch.randn(7, generator=g, requires_grad=True), torch.randn(3, 2, generator=g, requires_grad=True)]
+    for p in ps:
+        p.grad = torch.randn(p.shape, generator=g)
+    norm, want = ref.clip([p.grad for p in ps], 0.5)
+    assert abs(float(torch.nn.utils.clip_grad_norm_(ps, 0.5)) - norm) < 1e-5
+    assert all(torch.allclose(p.grad.double(), w, atol=1e-6) for p, w in zip(ps, want))
