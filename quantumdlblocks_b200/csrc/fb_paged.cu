@@ -224,8 +224,7 @@ __device__ __forceinline__ float half_lo(uint32_t w) { return __half2float(__ush
 __device__ __forceinline__ float half_hi(uint32_t w) { return __half2float(__ushort_as_half((unsigned short)(w >> 16))); }
 
 template <int D> struct TcShape {
-  static constexpr int kCopies = D / 16 + D / 16;       // 16-byte pieces per lane and stage: K, then V
-  static constexpr int kStageBytes = kCopies * 32 * 16;  // per warp: kSub keys and values
+  static constexpr int kStageBytes = 2 * kSub * D * 2;  // per warp: kSub keys, then their values
   static constexpr int kStages = D == 64 ? 4 : 3;
   static constexpr int kSmem = kWarps * kStages * kStageBytes;
   static constexpr int kCtasPerSm = D == 64 ? 3 : 2;
@@ -237,9 +236,11 @@ template <int D> struct TcShape {
 //              the same: it takes the 16-byte pieces at 32 j + 8 c
 //   O = P V    (B = V):  keys 2c, 2c + 1, 2c + 8, 2c + 9; column r of instruction (jj, e) is dimension
 //              64 jj + 8 r + e, so it takes the 16-byte pieces at 64 jj + 8 r and pairs two keys' words
-// and S's accumulator has P's operand layout.  So each lane reads exactly the bytes it copied itself:
-// the asynchronous copies' ring in shared memory is a longer register file, with no barrier, no bank
-// conflict and no swizzle, and kStages x kSub keys per warp are in flight.
+// and S's accumulator has P's operand layout: no transposing load, no exchange between lanes.  Each warp
+// has a ring of kStages x kSub keys and values of its own in shared memory and no barrier with the others.
+// Its copies take whole rows by neighbouring lanes (copied in the lanes' own order instead, a sector crossed
+// from L2 twice: 1.94 GB for 0.97 GB of keys).  Piece i of row t lies at i ^ 4 (t & 1) for keys, i ^ 2 ((t / 2) & 3)
+// for values: eight lanes' reads then fall on eight different bank groups.
 template <typename T, int D>
 __global__ void __launch_bounds__(kWarps * 32, TcShape<D>::kCtasPerSm) paged_born_tc(const PagedParams p) {
   using Sh = TcShape<D>;
@@ -248,8 +249,12 @@ __global__ void __launch_bounds__(kWarps * 32, TcShape<D>::kCtasPerSm) paged_bor
   __shared__ int64_t sh[kWarps];
   __shared__ float rz[kWarps * 16];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
-  uint8_t* ring = smem + warp * Sh::kStages * Sh::kStageBytes + lane * 16;
+  uint8_t* ring = smem + warp * Sh::kStages * Sh::kStageBytes;
   const uint32_t ring_s = (uint32_t)__cvta_generic_to_shared(ring);
+  constexpr int kRow = 2 * D;          // bytes
+  constexpr int kPieces = D / 8;       // per row
+  constexpr int kRows = 32 / kPieces;  // that one copy instruction takes
+  const int cp_row = lane / kPieces, cp_piece = lane % kPieces;
   float* red = reinterpret_cast<float*>(smem);
   constexpr int kRedWarp = Sh::kStages * Sh::kStageBytes / 4;
   static_assert(16 * (D + 4) <= kRedWarp, "a warp's sums fit its ring");
@@ -271,57 +276,38 @@ __global__ void __launch_bounds__(kWarps * 32, TcShape<D>::kCtasPerSm) paged_bor
       return table[p.page_shift >= 0 ? key >> p.page_shift : key / p.page];
     };
     auto issue = [&](int i, int pg) {
-      const uint32_t to = ring_s + (i % Sh::kStages) * Sh::kStageBytes;
       const int key0 = first + i * kTile;
       if (i < n) {
-        int64_t ko[2], vo[4];
-        bool kv[2], vv[4];
+        const uint32_t to = ring_s + (i % Sh::kStages) * Sh::kStageBytes;
+        const bool have = pg >= 0 && pg < p.pages;
+        int row0 = 0;
+        const T *ksrc = kbase + 8 * cp_piece, *vsrc = vbase + 8 * cp_piece;
         if (page_uniform) {
-          const bool have = pg >= 0 && pg < p.pages;
-          const int row0 = p.page_shift >= 0 ? key0 & (p.page - 1) : key0 % p.page;
-          const int64_t kp = (have ? pg : 0) * p.ks[0], vp = (have ? pg : 0) * p.vs[0];
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const int j = r + 8 * x;
-            kv[x] = have && key0 + j >= kk.lo && key0 + j < kk.hi;
-            ko[x] = kp + (row0 + j) * p.ks[2];
-          }
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const int j = 2 * c + (x & 1) + 8 * (x >> 1);
-            vv[x] = have && key0 + j >= kk.lo && key0 + j < kk.hi;
-            vo[x] = vp + (row0 + j) * p.vs[2];
+          row0 = p.page_shift >= 0 ? key0 & (p.page - 1) : key0 % p.page;
+          if (have) {
+            ksrc += pg * p.ks[0] + (row0 + cp_row) * p.ks[2];
+            vsrc += pg * p.vs[0] + (row0 + cp_row) * p.vs[2];
           }
         } else {
-          const int key = key0 + (lane & 15);
-          const int row = key % p.page;
-          const bool have = pg >= 0 && pg < p.pages;
-          const int packed = have ? pg : -1;
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const int j = r + 8 * x;
-            const int g = __shfl_sync(0xffffffffu, packed, j), w = __shfl_sync(0xffffffffu, row, j);
-            kv[x] = g >= 0;
-            ko[x] = kv[x] ? g * p.ks[0] + w * p.ks[2] : 0;
-          }
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const int j = 2 * c + (x & 1) + 8 * (x >> 1);
-            const int g = __shfl_sync(0xffffffffu, packed, j), w = __shfl_sync(0xffffffffu, row, j);
-            vv[x] = g >= 0;
-            vo[x] = vv[x] ? g * p.vs[0] + w * p.vs[2] : 0;
-          }
+          row0 = (key0 + (lane & 15)) % p.page;
         }
+        const int packed = have ? pg : -1;
 #pragma unroll
-        for (int x = 0; x < 2; ++x)
-#pragma unroll
-          for (int j = 0; j < D / 32; ++j)
-            copy16(to + (x * (D / 32) + j) * 512, kbase + (kv[x] ? ko[x] : 0) + 32 * j + 8 * c, kv[x]);
-#pragma unroll
-        for (int x = 0; x < 4; ++x)
-#pragma unroll
-          for (int jj = 0; jj < D / 64; ++jj)
-            copy16(to + (D / 16 + x * (D / 64) + jj) * 512, vbase + (vv[x] ? vo[x] : 0) + 64 * jj + 8 * r, vv[x]);
+        for (int x = 0; x < kSub / kRows; ++x) {
+          const int t = x * kRows + cp_row;
+          const T *kx = ksrc, *vx = vsrc;
+          bool ok = have;
+          if (page_uniform) {
+            ok = ok && key0 + t >= kk.lo && key0 + t < kk.hi;
+            if (ok) kx += x * kRows * p.ks[2], vx += x * kRows * p.vs[2];
+          } else {
+            const int g = __shfl_sync(0xffffffffu, packed, t), w = __shfl_sync(0xffffffffu, row0, t);
+            ok = g >= 0;
+            if (ok) kx += g * p.ks[0] + w * p.ks[2], vx += g * p.vs[0] + w * p.vs[2];
+          }
+          copy16(to + t * kRow + (cp_piece ^ 4 * (t & 1)) * 16, kx, ok);
+          copy16(to + kSub * kRow + t * kRow + (cp_piece ^ 2 * (t >> 1 & 3)) * 16, vx, ok);
+        }
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
@@ -361,7 +347,10 @@ __global__ void __launch_bounds__(kWarps * 32, TcShape<D>::kCtasPerSm) paged_bor
     int next = lookup(Sh::kStages - 1);
     for (int i = 0; i < n; ++i) {
       asm volatile("cp.async.wait_group %0;" ::"n"(Sh::kStages - 2) : "memory");
+      __syncwarp();  // the other lanes' copies have landed too
       const uint8_t* stage = ring + (i % Sh::kStages) * Sh::kStageBytes;
+      const uint8_t* kst = stage + r * kRow + c * 16;
+      const uint8_t* vst = stage + (kSub + 2 * c) * kRow + (r ^ 2 * c) * 16;
       float sacc[2][4];
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
@@ -369,7 +358,7 @@ __global__ void __launch_bounds__(kWarps * 32, TcShape<D>::kCtasPerSm) paged_bor
         for (int e = 0; e < 4; ++e) sacc[x][e] = 0.f;
 #pragma unroll
         for (int j = 0; j < D / 32; ++j) {
-          const uint4 w = *reinterpret_cast<const uint4*>(stage + (x * (D / 32) + j) * 512);
+          const uint4 w = *reinterpret_cast<const uint4*>(kst + 8 * x * kRow + 64 * (j ^ (r & 1)));
           mma_16816<T>(sacc[x], qf[2 * j], w.x, w.y);
           mma_16816<T>(sacc[x], qf[2 * j + 1], w.z, w.w);
         }
@@ -407,7 +396,7 @@ __global__ void __launch_bounds__(kWarps * 32, TcShape<D>::kCtasPerSm) paged_bor
           uint4 v[4];
 #pragma unroll
           for (int x = 0; x < 4; ++x)
-            v[x] = *reinterpret_cast<const uint4*>(stage + (D / 16 + x * (D / 64) + jj) * 512);
+            v[x] = *reinterpret_cast<const uint4*>(vst + ((x & 1) + 8 * (x >> 1)) * kRow + 128 * jj);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const uint32_t v0 = (&v[0].x)[e], v1 = (&v[1].x)[e], v2 = (&v[2].x)[e], v3 = (&v[3].x)[e];
@@ -438,7 +427,7 @@ __global__ void __launch_bounds__(kWarps * 32, TcShape<D>::kCtasPerSm) paged_bor
           uint4 v[4];
 #pragma unroll
           for (int x = 0; x < 4; ++x)
-            v[x] = *reinterpret_cast<const uint4*>(stage + (D / 16 + x * (D / 64) + jj) * 512);
+            v[x] = *reinterpret_cast<const uint4*>(vst + ((x & 1) + 8 * (x >> 1)) * kRow + 128 * jj);
 #pragma unroll
           for (int e = 0; e < 4; ++e)
 #pragma unroll
@@ -449,7 +438,8 @@ __global__ void __launch_bounds__(kWarps * 32, TcShape<D>::kCtasPerSm) paged_bor
             }
         }
       }
-      issue(i + Sh::kStages - 1, next);  // over the stage that the previous step has read
+      __syncwarp();
+      issue(i + Sh::kStages - 1, next);  // over the stage that every lane read in the previous step
       next = lookup(i + Sh::kStages);
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
