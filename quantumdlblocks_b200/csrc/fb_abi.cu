@@ -180,6 +180,8 @@ int run(const fb_attn_args* a, void* stream, bool purified, bool backward, bool 
 
 void set_last_launch_count(int n) { t_last_launches = n; }
 
+int* device_status_word(int* rc) { return status_ptr(rc); }
+
 cudaError_t set_smem_limit_once(const void* kernel, int smem) {
   static std::mutex mu;
   static std::map<std::pair<const void*, int>, int> done;  // (kernel, device) -> bytes set

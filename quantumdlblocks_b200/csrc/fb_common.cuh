@@ -225,6 +225,8 @@ bool tc_bwd64_supported(const Problem& p);  // fused backward (fb_tc_bwd64.cu), 
 int tc_bwd64(const Problem& p, cudaStream_t s, int* launches);
 size_t tc_bwd64_workspace(const Problem& p);
 void record_cuda_error(cudaError_t e);
+// the current device's status word {code, site}; nullptr and *rc on failure
+int* device_status_word(int* rc);
 void set_last_launch_count(int n);  // what fb_last_launch_count reports for this host thread
 // cudaFuncSetAttribute(MaxDynamicSharedMemorySize) for `kernel` on the current device, made once
 // per (kernel, device, size) and remembered (a failure is not), so that repeated launches spend

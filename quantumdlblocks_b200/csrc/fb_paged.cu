@@ -6,31 +6,31 @@
 //
 // The attention reads every key and value once and does 4 operations per element and query head:
 // HBM bandwidth bounds it.  Born weights need no running maximum, so a sequence's keys can be cut
-// anywhere and the pieces' (sum p v, sum p) just add.  The work is cut evenly whatever the lengths:
-// a unit is (sequence, kv head, up to HU query heads), its keys are tiles of kTile, all units' tiles
-// form one line, and CTA c of C takes the c-th C-th of it.  Lengths are read on the device (the host
-// knows only the table's width), so a call needs no synchronisation and replays from a graph.  A unit
-// inside one CTA's share is finished there; pieces of a unit that spans shares go to the workspace,
-// two slots per CTA, and a second kernel adds them in share order (the same bits every time).
+// anywhere and the pieces' (sum p v, sum p) just add.  The work is cut evenly whatever the lengths: a
+// unit is (sequence, kv head, up to HU query heads), its keys are cut into tiles, all units' tiles form
+// one line, and worker w of W (a warp of the tensor-core kernel, a CTA of the other) takes the w-th part
+// of it.  Lengths are read on the device (the host knows only the table's width), so a call needs
+// no synchronisation and replays from a graph.  A unit inside one worker's share is finished there;
+// pieces of a unit that spans shares go to the workspace, two slots per worker, and a second kernel adds
+// them in share order (the same bits every time).
 #include <cuda_runtime.h>
 
 #include <algorithm>
 #include <type_traits>
 
 #include "fb_common.cuh"
+#include "fb_sm100.cuh"
 
 namespace fb {
 namespace {
 
-constexpr int kWarps = 4;             // per CTA
-constexpr int kSub = 16;              // keys a warp takes at a time
-constexpr int kTile = kWarps * kSub;  // keys a CTA takes at a time
-constexpr int kJoinThreads = 256;
+constexpr int kWarps = 4;  // per CTA of the attention kernels
+constexpr int kThreads = kWarps * 32;
+constexpr int kSub = 16;   // keys a warp of the tensor-core kernel takes at a time
 
 struct PagedParams {
   int S, H, Hkv, G, D;
   int page, pages, width;  // page rows, pages, table columns
-  int page_shift;          // log2 of page where it is a power of two, else -1
   int window;
   float eps, scale_value;
   const float* scale;
@@ -47,8 +47,10 @@ struct PagedParams {
   int64_t table_stride;
   const int32_t* lens;
   int HU, chunks, U;  // query heads per unit, units per kv head, units per sequence
-  int C;              // CTAs that share the tiles
-  float* part;        // [C][2][HU][D] sums of p v, then [C][2][HU] sums of p
+  int tile;           // keys, a multiple of 2 kSub where units are cut
+  uint32_t W;         // workers that share the tiles (all units' tiles are below 2^31)
+  float* part;        // [W][2][HU][D] sums of p v, then [W][2][HU] sums of p
+  int* status;        // device status word
 };
 
 __device__ __forceinline__ float warp_sum(float v) {
@@ -61,414 +63,490 @@ __device__ __forceinline__ float warp_sum(float v) {
 // the tiles they take, counted from a multiple of kSub so that a warp's keys do not straddle pages
 // whose size is a multiple of it.  A sequence without keys has one (empty) tile: its zeros get written.
 struct Keys {
-  int lo, hi, base, tiles;
+  int lo, hi, base;
+  uint32_t tiles;
 };
 __device__ __forceinline__ Keys keys_of(const PagedParams& p, int s) {
   Keys k;
   k.hi = min(max(p.lens[s], 0), p.page * p.width);
   k.lo = p.window > 0 ? max(k.hi - p.window, 0) : 0;
   k.base = k.lo & ~(kSub - 1);
-  k.tiles = max((k.hi - k.base + kTile - 1) / kTile, 1);
+  k.tiles = max((uint32_t)(k.hi - k.base + p.tile - 1) / (uint32_t)p.tile, 1u);
   return k;
 }
 
 // relu that keeps a NaN
 __device__ __forceinline__ float relu(float x) { return x <= 0.f ? 0.f : x; }
 
-// The tiles of the sequences before `stop` (or of all: stop = S), summed by a whole block.  Per
-// sequence, to be multiplied by the units.
-template <int THREADS>
-__device__ int64_t tiles_before(const PagedParams& p, int stop, int64_t* sh) {
-  int64_t n = 0;
-  for (int s = threadIdx.x; s < stop; s += THREADS) n += keys_of(p, s).tiles;
+// Tiles of the sequences up to and including group i of N, a group being `per` sequences in a row:
+// pre[i], by a block of N threads.  Returns per.
+template <int N>
+__device__ int tile_prefix(const PagedParams& p, uint32_t* pre) {
+  __shared__ uint32_t warps[N / 32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, per = (p.S + N - 1) / N;
+  uint32_t n = 0;
+  for (int s = threadIdx.x * per; s < min(p.S, ((int)threadIdx.x + 1) * per); ++s) n += keys_of(p, s).tiles * p.U;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = n;
-  __syncthreads();
-  n = 0;
-#pragma unroll
-  for (int w = 0; w < THREADS / 32; ++w) n += sh[w];
-  return n;
-}
-
-// The sequence that holds tile t (in tiles per sequence, t below the total) and the tiles before it,
-// searched by the whole block, THREADS sequences at a time.
-template <int THREADS>
-__device__ void find_sequence(const PagedParams& p, int64_t t, int64_t* sh, int& seq, int64_t& before) {
-  __shared__ int found;
-  __shared__ int64_t found_before;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (threadIdx.x == 0) found = -1;
-  int64_t start = 0;
-  for (int s0 = 0; s0 < p.S; s0 += THREADS) {
-    const int s = s0 + threadIdx.x;
-    const int64_t n = s < p.S ? keys_of(p, s).tiles : 0;
-    int64_t incl = n;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t up = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += up;
-    }
-    __syncthreads();
-    if (lane == 31) sh[warp] = incl;
-    __syncthreads();
-    int64_t all = start;
-#pragma unroll
-    for (int w = 0; w < THREADS / 32; ++w) {
-      if (w < warp) incl += sh[w];
-      all += sh[w];
-    }
-    incl += start;
-    if (t < incl && t >= incl - n) {
-      found = s;
-      found_before = incl - n;
-    }
-    start = all;
-    if (t < all) break;  // the same for every thread
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t up = __shfl_up_sync(0xffffffffu, n, o);
+    if (lane >= o) n += up;
   }
+  if (lane == 31) warps[warp] = n;
   __syncthreads();
-  seq = found;
-  before = found_before;
-}
-
-// Where a piece's sums go: the result when it is the whole unit, else the CTA's slot in the workspace
-// (slot 1: the unit begins here and goes on in the next CTA; slot 0: it began before).  red holds each
-// warp's [HU][D + 4] sums of p v and rz its HU sums of p.
-template <typename T>
-__device__ void finish_piece(const PagedParams& p, const float* red, int red_warp, const float* rz, int s, int unit,
-                             bool whole, bool begins) {
-  const int kvh = unit / p.chunks, h0 = unit % p.chunks * p.HU, nh = min(p.HU, p.G - h0);
-  const int ld = p.D + 4;
-  const int64_t slot = (int64_t)blockIdx.x * 2 + (begins ? 1 : 0);
-  for (int i = threadIdx.x; i < nh * p.D; i += kWarps * 32) {
-    const int h = i / p.D, d = i % p.D;
-    float o = 0.f, z = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      o += red[w * red_warp + h * ld + d];
-      z += rz[w * p.HU + h];
-    }
-    if (whole) {
-      T* out = static_cast<T*>(p.out) + s * p.os[0] + (int64_t)(kvh * p.G + h0 + h) * p.os[1];
-      out[d] = from_f32<T>(z == 0.f ? 0.f : o / (z + p.eps));
-    } else {
-      p.part[(slot * p.HU + h) * p.D + d] = o;
-      if (d == 0) p.part[(int64_t)p.C * 2 * p.HU * p.D + slot * p.HU + h] = z;
-    }
-  }
+  for (int w = 0; w < N / 32; ++w)
+    if (w < warp) n += warps[w];
+  pre[threadIdx.x] = n;
+  __syncthreads();
+  return per;
 }
 
-// Walks the CTA's share of the tiles: piece(s, keys, unit, first tile, last tile + 1, whole, begins).
-template <typename F>
-__device__ __forceinline__ void walk_share(const PagedParams& p, int64_t* sh, F&& piece) {
-  const int64_t total = tiles_before<kWarps * 32>(p, p.S, sh) * p.U;
-  const int64_t C = min((int64_t)p.C, total);  // no empty shares
-  if (blockIdx.x >= C) return;
-  const int64_t t0 = total * blockIdx.x / C, t1 = total * (blockIdx.x + 1) / C;
-  int s;
-  int64_t first;
-  find_sequence<kWarps * 32>(p, t0 / p.U, sh, s, first);
-  first *= p.U;
-  Keys k = keys_of(p, s);
-  for (int64_t t = t0; t < t1;) {
-    while (t >= first + (int64_t)k.tiles * p.U) {
-      first += (int64_t)k.tiles * p.U;
+// The even cut of `total` tiles among the workers (no more of them than tiles): the first `more` shares
+// have `each` + 1 tiles, the others `each`.
+struct Shares {
+  uint32_t workers, each, more;
+  __device__ Shares(uint32_t total, uint32_t W) : workers(min(W, total)), each(total / workers), more(total % workers) {}
+  __device__ uint32_t start(uint32_t w) const { return w * each + min(w, more); }
+  __device__ uint32_t owner(uint32_t t) const {
+    const uint32_t big = more * (each + 1);
+    return t < big ? t / (each + 1) : more + (t - big) / each;
+  }
+};
+
+// One worker's share, piece by piece: the tiles [a, b) of a unit of sequence s.
+struct Walk {
+  uint32_t t, t1;  // the line's tiles still to come
+  uint32_t first;  // the first tile of sequence s
+  int s, unit;
+  uint32_t a, b;
+  Keys k;
+
+  // false: the worker has no share.  pre: tile_prefix's.
+  template <int N>
+  __device__ bool begin(const PagedParams& p, const uint32_t* pre, int per, uint32_t worker) {
+    const Shares sh(pre[N - 1], p.W);
+    if (worker >= sh.workers) return false;
+    t = sh.start(worker);
+    t1 = sh.start(worker + 1);
+    int g = 0;  // the group that holds tile t
+#pragma unroll
+    for (int step = N / 2; step > 0; step >>= 1)
+      if (pre[g + step - 1] <= t) g += step;
+    first = g > 0 ? pre[g - 1] : 0;
+    s = g * per;
+    k = keys_of(p, s);
+    piece(p);
+    return true;
+  }
+  __device__ void piece(const PagedParams& p) {
+    while (t - first >= k.tiles * p.U) {
+      first += k.tiles * p.U;
       k = keys_of(p, ++s);
     }
-    const int unit = (int)((t - first) / k.tiles), a = (int)((t - first) % k.tiles);
-    const int b = (int)min((int64_t)k.tiles, a + (t1 - t));
-    piece(s, k, unit, a, b, a == 0 && b == k.tiles, a == 0);
-    t += b - a;
+    unit = (int)((t - first) / k.tiles);
+    a = (t - first) % k.tiles;
+    b = min(k.tiles, a + (t1 - t));
   }
-}
+  // to the next piece; false after the last
+  __device__ bool next(const PagedParams& p) {
+    t += b - a;
+    if (t >= t1) return false;
+    piece(p);
+    return true;
+  }
+  __device__ int first_key(const PagedParams& p) const { return k.base + (int)a * p.tile; }
+  __device__ int end_key(const PagedParams& p) const { return b == k.tiles ? k.hi : k.base + (int)b * p.tile; }
+  __device__ bool whole() const { return a == 0 && b == k.tiles; }
+};
 
-// Page and row of a key; false where the table holds no page for it.
-__device__ __forceinline__ bool find_page(const PagedParams& p, const int32_t* table, int key, int& pg, int& row) {
-  const int i = p.page_shift >= 0 ? key >> p.page_shift : key / p.page;
-  pg = table[i];
-  row = key - i * p.page;
-  return pg >= 0 && pg < p.pages;
-}
+// A worker's two slots in the workspace: 1 for the piece of a unit that begins in its share and goes
+// on in the next, 0 for the one that began before.
+__device__ __forceinline__ int64_t slot_of(uint32_t worker, bool begins) { return (int64_t)worker * 2 + (begins ? 1 : 0); }
+__device__ __forceinline__ float* slot_z(const PagedParams& p) { return p.part + (int64_t)p.W * 2 * p.HU * p.D; }
 
 // ------------------------------------------------------------------------------------------
 // Tensor-core kernel: bf16 or fp16, D = 64 or 128, rows on 16-byte boundaries
 // ------------------------------------------------------------------------------------------
 template <typename T>
-__device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  if constexpr (sizeof(T) == 2 && std::is_same<T, __half>::value)
+__device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                          uint32_t b1) {
+  if constexpr (std::is_same<T, __half>::value)
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   else
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-__device__ __forceinline__ void mma_1688_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma_1688_tf32(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                              uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
 __device__ __forceinline__ void copy16(uint32_t to, const void* from, bool valid) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(valid ? 16 : 0) : "memory");
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(valid ? 16 : 0) : "memory");
 }
 
 __device__ __forceinline__ uint32_t f2_to_bf2(float lo, float hi) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
+__device__ __forceinline__ uint32_t f_to_tf32(float x) {
+  uint32_t b;
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(b) : "f"(x));
+  return b;
+}
 __device__ __forceinline__ float half_lo(uint32_t w) { return __half2float(__ushort_as_half((unsigned short)(w & 0xFFFFu))); }
 __device__ __forceinline__ float half_hi(uint32_t w) { return __half2float(__ushort_as_half((unsigned short)(w >> 16))); }
 
 template <int D> struct TcShape {
-  static constexpr int kStageBytes = 2 * kSub * D * 2;  // per warp: kSub keys, then their values
+  static constexpr int kHalves = D / 64;                  // 128-byte rows per key
+  static constexpr int kHalfBytes = kSub * 128;
+  static constexpr int kStageBytes = 2 * kHalves * kHalfBytes;  // per warp: kSub keys, then their values
   static constexpr int kStages = D == 64 ? 4 : 3;
-  static constexpr int kSmem = kWarps * kStages * kStageBytes;
   static constexpr int kCtasPerSm = D == 64 ? 3 : 2;
+  static constexpr int kSmem = kWarps * kStages * kStageBytes + 1024;  // + alignment of the swizzle
 };
 
-// Rows of the matrix instructions are the unit's query heads (up to 16), so a key is read once for all
-// of them.  Lane (r = lane / 4, c = lane % 4) of a warp needs, of kSub keys,
-//   S = Q K^T  (B = K^T):  keys r and r + 8, and of them any dimensions as long as Q's fragment has
-//              the same: it takes the 16-byte pieces at 32 j + 8 c
-//   O = P V    (B = V):  keys 2c, 2c + 1, 2c + 8, 2c + 9; column r of instruction (jj, e) is dimension
-//              64 jj + 8 r + e, so it takes the 16-byte pieces at 64 jj + 8 r and pairs two keys' words
-// and S's accumulator has P's operand layout: no transposing load, no exchange between lanes.  Each warp
-// has a ring of kStages x kSub keys and values of its own in shared memory and no barrier with the others.
-// Its copies take whole rows by neighbouring lanes (copied in the lanes' own order instead, a sector crossed
-// from L2 twice: 1.94 GB for 0.97 GB of keys).  Piece i of row t lies at i ^ 4 (t & 1) for keys, i ^ 2 ((t / 2) & 3)
-// for values: eight lanes' reads then fall on eight different bank groups.
-template <typename T, int D>
-__global__ void __launch_bounds__(kWarps * 32, TcShape<D>::kCtasPerSm) paged_born_tc(const PagedParams p) {
+// What the two loaders need of the ring's next step: a cursor that runs kStages - 1 steps ahead of the
+// computation, across the pieces of the share.
+struct Feed {
+  Walk w;
+  bool more;
+  int key, end;      // next step's first key, the piece's end
+  int page_i, row;   // page of `key` in the table, and its row
+  int32_t ahead[2];  // lane l: the table's entries page0 + l and page0 + 32 + l
+  int page0;
+};
+
+// Rows of the matrix instructions are the unit's query heads, so a key is read once for all of them.
+// A warp takes kSub = 16 keys at a time.  Lane (r = lane / 4, c = lane % 4) needs of them
+//   S = Q K^T  (B = K^T):  two keys, and of them any dimensions as long as Q's fragment has the same: it takes
+//              the 16-byte pieces 4 j + c.  Column r of instruction x is key 8 x + r / 2 + 4 (r % 2).
+//   O = P V    (B = V):  S's accumulator already is P's operand for keys c, c + 4, c + 8, c + 12.  Column r of
+//              instruction (jj, e) is dimension 64 jj + 8 (r / 2 + 4 (r % 2)) + e: it takes that 16-byte piece
+//              of four keys and pairs their words.
+// No transposing load and no exchange between lanes.  Both orders are chosen for the 128-byte swizzle that the
+// copies write (piece i of row t at i ^ (t % 8)): eight lanes' reads fall on eight different bank groups.
+//
+// Up to 8 heads (PACK), rows 8-15 of P's operand are the rest that rounding P to 16 bits leaves, in the
+// same instructions; with 9 to 16 heads the rest takes instructions of its own.  P of one rounding would add
+// as much error as the rounding of the result does (measured: 2.3e-3 of the result against 1.6e-3).
+//
+// Each warp has a ring of kStages x 16 keys and values in shared memory and is its own producer: one lane asks
+// TMA for a step's boxes (TMA; pages of a multiple of 16 rows), or all lanes copy rows (any other page).
+// No barrier between warps; the ring runs on into the next piece while one is finished.
+template <typename T, int D, bool PACK, bool TMA>
+__global__ void __launch_bounds__(kThreads, TcShape<D>::kCtasPerSm)
+    paged_born_tc(const PagedParams p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
   using Sh = TcShape<D>;
   constexpr bool kHalf = std::is_same<T, __half>::value;
-  extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ int64_t sh[kWarps];
-  __shared__ float rz[kWarps * 16];
+  constexpr int kHeads = PACK ? 1 : 2;  // that a lane has: r, and r + 8
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  __shared__ uint32_t pre[kThreads];
+  __shared__ uint64_t bars[kWarps * Sh::kStages];
+  __shared__ int abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
-  uint8_t* ring = smem + warp * Sh::kStages * Sh::kStageBytes;
-  const uint32_t ring_s = (uint32_t)__cvta_generic_to_shared(ring);
-  constexpr int kRow = 2 * D;          // bytes
-  constexpr int kPieces = D / 8;       // per row
-  constexpr int kRows = 32 / kPieces;  // that one copy instruction takes
-  const int cp_row = lane / kPieces, cp_piece = lane % kPieces;
-  float* red = reinterpret_cast<float*>(smem);
-  constexpr int kRedWarp = Sh::kStages * Sh::kStageBytes / 4;
-  static_assert(16 * (D + 4) <= kRedWarp, "a warp's sums fit its ring");
-  const bool page_uniform = p.page % kSub == 0;  // a warp's keys are rows of one page
+  uint8_t* ring = sm100::smem_align1024(smem_raw) + warp * Sh::kStages * Sh::kStageBytes;
+  const uint32_t ring_s = sm100::smem_u32(ring);
+  uint64_t* bar = bars + warp * Sh::kStages;
 
   asm volatile("griddepcontrol.launch_dependents;");
-  walk_share(p, sh, [&](int s, const Keys& kk, int unit, int ta, int tb, bool whole, bool begins) {
-    const int kvh = unit / p.chunks, h0 = unit % p.chunks * p.HU, nh = min(p.HU, p.G - h0);
-    const int32_t* table = p.table + s * p.table_stride;
-    const T* kbase = static_cast<const T*>(p.k) + kvh * p.ks[1];
-    const T* vbase = static_cast<const T*>(p.v) + kvh * p.vs[1];
-    const int first = kk.base + ta * kTile + warp * kSub;  // this warp's first key
-    const int n = kk.hi > first ? min(tb - ta, (kk.hi - first + kTile - 1) / kTile) : 0;  // its steps
+  if constexpr (TMA) {
+    if (threadIdx.x == 0) {
+      asm volatile("prefetch.tensormap [%0];" ::"l"(&kmap));
+      asm volatile("prefetch.tensormap [%0];" ::"l"(&vmap));
+    }
+    if (lane == 0) {
+      for (int i = 0; i < Sh::kStages; ++i) sm100::mbar_init(bar + i, 1);
+      sm100::fence_mbar_init();
+    }
+    if (threadIdx.x == 0) abort_flag = 0;
+  }
+  const int per = tile_prefix<kThreads>(p, pre);  // and the barriers' initialisation is visible
+  const uint32_t worker = blockIdx.x * kWarps + warp;
+  Walk w;
+  if (!w.begin<kThreads>(p, pre, per, worker)) return;
 
-    // page of the step's first key (page_uniform) or of key lane & 15
-    auto lookup = [&](int i) -> int {
-      const int key = first + i * kTile + (page_uniform ? 0 : lane & 15);
-      if (i >= n || key >= kk.hi || (!page_uniform && key < kk.lo)) return -1;
-      return table[p.page_shift >= 0 ? key >> p.page_shift : key / p.page];
-    };
-    auto issue = [&](int i, int pg) {
-      const int key0 = first + i * kTile;
-      if (i < n) {
-        const uint32_t to = ring_s + (i % Sh::kStages) * Sh::kStageBytes;
-        const bool have = pg >= 0 && pg < p.pages;
-        int row0 = 0;
-        const T *ksrc = kbase + 8 * cp_piece, *vsrc = vbase + 8 * cp_piece;
-        if (page_uniform) {
-          row0 = p.page_shift >= 0 ? key0 & (p.page - 1) : key0 % p.page;
-          if (have) {
-            ksrc += pg * p.ks[0] + (row0 + cp_row) * p.ks[2];
-            vsrc += pg * p.vs[0] + (row0 + cp_row) * p.vs[2];
-          }
-        } else {
-          row0 = (key0 + (lane & 15)) % p.page;
+  // ---- the feed
+  Feed f;
+  f.w = w;
+  f.more = true;
+  auto entries = [&](int i) -> int32_t {  // lane's table entry, out of range where it has none
+    return i < p.width ? p.table[f.w.s * p.table_stride + i] : -1;
+  };
+  auto feed_piece = [&]() {
+    f.key = f.w.first_key(p);
+    f.end = f.w.end_key(p);
+    f.page_i = f.key / p.page;
+    f.row = f.key - f.page_i * p.page;
+    if constexpr (TMA) {
+      f.page0 = f.page_i;
+      f.ahead[0] = entries(f.page0 + lane);
+      f.ahead[1] = entries(f.page0 + 32 + lane);
+    }
+  };
+  // the feed's step into stage `st` (nothing after the last)
+  auto feed = [&](int st) {
+    while (f.more && f.key >= f.end) {  // pieces without keys have no steps
+      f.more = f.w.next(p);
+      if (f.more) feed_piece();
+    }
+    if (f.more) {
+      const int unit = f.w.unit, kvh = unit / p.chunks;
+      if constexpr (TMA) {
+        if (f.page_i - f.page0 >= 32) {
+          f.page0 += 32;
+          f.ahead[0] = f.ahead[1];
+          f.ahead[1] = entries(f.page0 + 32 + lane);
         }
-        const int packed = have ? pg : -1;
+        int pg = __shfl_sync(0xffffffffu, f.ahead[0], f.page_i - f.page0);
+        if (pg < 0 || pg >= p.pages) pg = p.pages;  // outside the map: the box is filled with zeros
+        if (lane == 0) {
+          uint8_t* to = ring + st * Sh::kStageBytes;
+          sm100::mbar_arrive_expect_tx(bar + st, Sh::kStageBytes);
+#pragma unroll
+          for (int h = 0; h < Sh::kHalves; ++h) {
+            sm100::tma_load_4d(to + h * Sh::kHalfBytes, &kmap, bar + st, 64 * h, f.row, kvh, pg);
+            sm100::tma_load_4d(to + (Sh::kHalves + h) * Sh::kHalfBytes, &vmap, bar + st, 64 * h, f.row, kvh, pg);
+          }
+        }
+        f.row += kSub;
+        if (f.row >= p.page) {
+          f.row = 0;
+          ++f.page_i;
+        }
+      } else {
+        constexpr int kPieces = D / 8, kRows = 32 / kPieces;  // per row; that one copy instruction takes
+        const uint32_t to = ring_s + st * Sh::kStageBytes;
+        const int key = f.key + (lane & 15);
+        int pg = -1, row = 0;
+        if (key >= f.w.k.lo && key < f.w.k.hi) {
+          const int i = key / p.page;
+          pg = p.table[f.w.s * p.table_stride + i];
+          row = key - i * p.page;
+          if (pg >= p.pages) pg = -1;
+        }
+        const int piece = lane % kPieces;
+        const T* ks = static_cast<const T*>(p.k) + kvh * p.ks[1] + 8 * piece;
+        const T* vs = static_cast<const T*>(p.v) + kvh * p.vs[1] + 8 * piece;
 #pragma unroll
         for (int x = 0; x < kSub / kRows; ++x) {
-          const int t = x * kRows + cp_row;
-          const T *kx = ksrc, *vx = vsrc;
-          bool ok = have;
-          if (page_uniform) {
-            ok = ok && key0 + t >= kk.lo && key0 + t < kk.hi;
-            if (ok) kx += x * kRows * p.ks[2], vx += x * kRows * p.vs[2];
-          } else {
-            const int g = __shfl_sync(0xffffffffu, packed, t), w = __shfl_sync(0xffffffffu, row0, t);
-            ok = g >= 0;
-            if (ok) kx += g * p.ks[0] + w * p.ks[2], vx += g * p.vs[0] + w * p.vs[2];
-          }
-          copy16(to + t * kRow + (cp_piece ^ 4 * (t & 1)) * 16, kx, ok);
-          copy16(to + kSub * kRow + t * kRow + (cp_piece ^ 2 * (t >> 1 & 3)) * 16, vx, ok);
+          const int t = x * kRows + lane / kPieces;
+          const int g = __shfl_sync(0xffffffffu, pg, t), n = __shfl_sync(0xffffffffu, row, t);
+          const uint32_t at = to + (piece >> 3) * Sh::kHalfBytes + t * 128 + ((piece ^ t) & 7) * 16;
+          copy16(at, g >= 0 ? ks + g * p.ks[0] + n * p.ks[2] : ks, g >= 0);
+          copy16(at + Sh::kHalves * Sh::kHalfBytes, g >= 0 ? vs + g * p.vs[0] + n * p.vs[2] : vs, g >= 0);
         }
       }
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    };
-
-    // Q: heads r and r + 8 of the unit, zero where it has fewer
-    uint32_t qf[D / 16][4];
-    float sc[2];
+      f.key += kSub;
+    }
+    if constexpr (!TMA) asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  feed_piece();
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const int h = r + 8 * x;
-      const int head = kvh * p.G + h0 + h;
-      const T* q = static_cast<const T*>(p.q) + s * p.qs[0] + head * p.qs[1];
+  for (int i = 0; i < Sh::kStages - 1; ++i) feed(i);
+
+  const uint8_t* kst0 = ring + (r >> 1) * 128 + (r & 1) * 512 + (c ^ (r >> 1)) * 16;
+  const uint8_t* vst0 = ring + Sh::kHalves * Sh::kHalfBytes + c * 128 + ((r >> 1) ^ c) * 16;
+  int stage = 0;
+  uint32_t phase = 0;
+  do {
+    const int kvh = w.unit / p.chunks, h0 = w.unit % p.chunks * p.HU, nh = min(p.HU, p.G - h0);
+    const int head0 = kvh * p.G + h0;
+    // Q: heads r (and r + 8) of the unit, zero where it has fewer
+    uint32_t qf[D / 32][kHeads][4];
+    float sc[kHeads];
+#pragma unroll
+    for (int y = 0; y < kHeads; ++y) {
+      const int h = r + 8 * y;
+      const T* q = static_cast<const T*>(p.q) + w.s * p.qs[0] + (head0 + h) * p.qs[1];
 #pragma unroll
       for (int j = 0; j < D / 32; ++j) {
-        uint4 w = make_uint4(0, 0, 0, 0);
-        if (h < nh) w = *reinterpret_cast<const uint4*>(q + 32 * j + 8 * c);
-        qf[2 * j][x] = w.x;
-        qf[2 * j][2 + x] = w.y;
-        qf[2 * j + 1][x] = w.z;
-        qf[2 * j + 1][2 + x] = w.w;
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (h < nh) x = *reinterpret_cast<const uint4*>(q + 32 * j + 8 * c);
+        qf[j][y][0] = x.x, qf[j][y][1] = x.y, qf[j][y][2] = x.z, qf[j][y][3] = x.w;
       }
-      sc[x] = h < nh ? (p.scale ? p.scale[p.scale_per_head ? head : 0] : p.scale_value) : 0.f;
+      sc[y] = h < nh ? (p.scale ? p.scale[p.scale_per_head ? head0 + h : 0] : p.scale_value) : 0.f;
     }
-    float o[D / 8][4], z[2] = {0.f, 0.f};
+    float o[D / 8][4], z[kHeads];
 #pragma unroll
-    for (int i = 0; i < D / 8; ++i)
+    for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
+    for (int y = 0; y < kHeads; ++y) z[y] = 0.f;
 
-    {
-      int pg[Sh::kStages - 1];
-#pragma unroll
-      for (int i = 0; i < Sh::kStages - 1; ++i) pg[i] = lookup(i);
-#pragma unroll
-      for (int i = 0; i < Sh::kStages - 1; ++i) issue(i, pg[i]);
-    }
-    int next = lookup(Sh::kStages - 1);
-    for (int i = 0; i < n; ++i) {
-      asm volatile("cp.async.wait_group %0;" ::"n"(Sh::kStages - 2) : "memory");
-      __syncwarp();  // the other lanes' copies have landed too
-      const uint8_t* stage = ring + (i % Sh::kStages) * Sh::kStageBytes;
-      const uint8_t* kst = stage + r * kRow + c * 16;
-      const uint8_t* vst = stage + (kSub + 2 * c) * kRow + (r ^ 2 * c) * 16;
+    const int end = w.end_key(p);
+    for (int key0 = w.first_key(p); key0 < end; key0 += kSub) {
+      if constexpr (TMA) {
+        const sm100::WaitCtx wc{&abort_flag, p.status};
+        const bool landed = sm100::mbar_wait(bar + stage, phase, wc, 901);
+        if (!__all_sync(0xffffffffu, landed)) {  // give up: the copies in flight land before the CTA's memory goes
+          for (int i = 0; i < Sh::kStages; ++i) sm100::mbar_wait_drain(bar + i, i < stage ? phase ^ 1 : phase);
+          return;
+        }
+      } else {
+        asm volatile("cp.async.wait_group %0;" ::"n"(Sh::kStages - 2) : "memory");
+        __syncwarp();  // the other lanes' copies have landed too
+      }
+      const uint8_t* kst = kst0 + stage * Sh::kStageBytes;
+      const uint8_t* vst = vst0 + stage * Sh::kStageBytes;
       float sacc[2][4];
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sacc[x][e] = 0.f;
+        sacc[x][0] = sacc[x][1] = sacc[x][2] = sacc[x][3] = 0.f;
 #pragma unroll
         for (int j = 0; j < D / 32; ++j) {
-          const uint4 w = *reinterpret_cast<const uint4*>(kst + 8 * x * kRow + 64 * (j ^ (r & 1)));
-          mma_16816<T>(sacc[x], qf[2 * j], w.x, w.y);
-          mma_16816<T>(sacc[x], qf[2 * j + 1], w.z, w.w);
+          const uint4 k = *reinterpret_cast<const uint4*>(kst + (j >> 1) * Sh::kHalfBytes + x * 1024 + 64 * ((j ^ r) & 1));
+          mma_16816<T>(sacc[x], qf[j][0][0], PACK ? 0u : qf[j][kHeads - 1][0], qf[j][0][1],
+                       PACK ? 0u : qf[j][kHeads - 1][1], k.x, k.y);
+          mma_16816<T>(sacc[x], qf[j][0][2], PACK ? 0u : qf[j][kHeads - 1][2], qf[j][0][3],
+                       PACK ? 0u : qf[j][kHeads - 1][3], k.z, k.w);
         }
       }
-      // sacc[x][e]: head r + 8 (e / 2), key 8 x + 2 c + e % 2.  A key that does not count has K and V of
-      // zero; its weight is set to 0 as well, for a Q that is not finite.
-      float w[2][4];
-      const int key0 = first + i * kTile;
-      const bool edge = key0 < kk.lo || key0 + kSub > kk.hi;
+      // sacc[x][2 y + b]: head r + 8 y, key 8 x + 4 b + c.  Keys that do not count (before the window, past the
+      // length) may hold anything: their weight is 0, and so are their values.
+      const bool edge = key0 < w.k.lo || key0 + kSub > w.k.hi;
+      float wt[2][kHeads][2];
 #pragma unroll
       for (int x = 0; x < 2; ++x)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float a = relu(sacc[x][e] * sc[e >> 1]);
-          w[x][e] = a * a;
-          const int key = key0 + 8 * x + 2 * c + (e & 1);
-          if (edge && (key < kk.lo || key >= kk.hi)) w[x][e] = 0.f;
+        for (int y = 0; y < kHeads; ++y)
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            const float a = relu(sacc[x][2 * y + b] * sc[y]);
+            wt[x][y][b] = a * a;
+          }
+      bool counts[4];
+      if (edge) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int key = key0 + c + 4 * i;
+          counts[i] = key >= w.k.lo && key < w.k.hi;
+#pragma unroll
+          for (int y = 0; y < kHeads; ++y)
+            if (!counts[i]) wt[i >> 1][y][i & 1] = 0.f;
         }
+      }
+      auto load_v = [&](int i, int jj) {  // key c + 4 i
+        uint4 v = *reinterpret_cast<const uint4*>(vst + jj * Sh::kHalfBytes + i * 512 + 64 * ((i ^ r) & 1));
+        if (edge && !counts[i]) v = make_uint4(0, 0, 0, 0);
+        return v;
+      };
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int y = 0; y < kHeads; ++y) z[y] += wt[x][y][0] + wt[x][y][1];
       if constexpr (!kHalf) {
-        // P goes into the product as the sum of two bf16 numbers, 16 bits of it: one alone would add as much
-        // error as the rounding of the result does (measured: 2.3e-3 of the result against 1.6e-3)
-        uint32_t pf[4], pl[4];
+        uint32_t hi[2][kHeads], lo[2][kHeads];
 #pragma unroll
         for (int x = 0; x < 2; ++x)
 #pragma unroll
-          for (int y = 0; y < 2; ++y) {
-            const float w0 = w[x][2 * y], w1 = w[x][2 * y + 1];
-            const uint32_t b = f2_to_bf2(w0, w1);
-            pf[2 * x + y] = b;
-            pl[2 * x + y] = f2_to_bf2(w0 - __uint_as_float(b << 16), w1 - __uint_as_float(b & 0xFFFF0000u));
-            z[y] += w0 + w1;
+          for (int y = 0; y < kHeads; ++y) {
+            const uint32_t b = f2_to_bf2(wt[x][y][0], wt[x][y][1]);
+            hi[x][y] = b;
+            lo[x][y] = f2_to_bf2(wt[x][y][0] - __uint_as_float(b << 16), wt[x][y][1] - __uint_as_float(b & 0xFFFF0000u));
           }
 #pragma unroll
-        for (int jj = 0; jj < D / 64; ++jj) {
+        for (int jj = 0; jj < Sh::kHalves; ++jj) {
           uint4 v[4];
 #pragma unroll
-          for (int x = 0; x < 4; ++x)
-            v[x] = *reinterpret_cast<const uint4*>(vst + ((x & 1) + 8 * (x >> 1)) * kRow + 128 * jj);
+          for (int i = 0; i < 4; ++i) v[i] = load_v(i, jj);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t v0 = (&v[0].x)[e], v1 = (&v[1].x)[e], v2 = (&v[2].x)[e], v3 = (&v[3].x)[e];
-            const uint32_t even0 = __byte_perm(v0, v1, 0x5410), even1 = __byte_perm(v2, v3, 0x5410);
-            const uint32_t odd0 = __byte_perm(v0, v1, 0x7632), odd1 = __byte_perm(v2, v3, 0x7632);
-            mma_16816<T>(o[8 * jj + 2 * e], pf, even0, even1);
-            mma_16816<T>(o[8 * jj + 2 * e + 1], pf, odd0, odd1);
-            mma_16816<T>(o[8 * jj + 2 * e], pl, even0, even1);
-            mma_16816<T>(o[8 * jj + 2 * e + 1], pl, odd0, odd1);
+          for (int e = 0; e < 8; ++e) {
+            const uint32_t sel = e & 1 ? 0x7632 : 0x5410;
+            const uint32_t b0 = __byte_perm((&v[0].x)[e >> 1], (&v[1].x)[e >> 1], sel);
+            const uint32_t b1 = __byte_perm((&v[2].x)[e >> 1], (&v[3].x)[e >> 1], sel);
+            if constexpr (PACK) {
+              mma_16816<T>(o[8 * jj + e], hi[0][0], lo[0][0], hi[1][0], lo[1][0], b0, b1);
+            } else {
+              mma_16816<T>(o[8 * jj + e], hi[0][0], hi[0][kHeads - 1], hi[1][0], hi[1][kHeads - 1], b0, b1);
+              mma_16816<T>(o[8 * jj + e], lo[0][0], lo[0][kHeads - 1], lo[1][0], lo[1][kHeads - 1], b0, b1);
+            }
           }
         }
       } else {
         // fp16 cannot hold p = a^2 (a > 256 overflows it): P goes through TF32, fp16's 11 bits with fp32's
-        // range, in which V's values are exact.  Instruction x takes key 8 x + 2 c as its column c and
-        // 8 x + 2 c + 1 as c + 4.
-        uint32_t pf[2][4];
+        // range, in which V's values are exact.  Instruction x has key 8 x + c as its column c, 8 x + 4 + c as c + 4.
+        uint32_t hi[2][kHeads][2], lo[2][kHeads][2];
 #pragma unroll
         for (int x = 0; x < 2; ++x)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            uint32_t b;
-            asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(b) : "f"(w[x][e]));
-            pf[x][(e >> 1) + 2 * (e & 1)] = b;
-            z[e >> 1] += __uint_as_float(b);
-          }
+          for (int y = 0; y < kHeads; ++y)
 #pragma unroll
-        for (int jj = 0; jj < D / 64; ++jj) {
+            for (int b = 0; b < 2; ++b) {
+              hi[x][y][b] = f_to_tf32(wt[x][y][b]);
+              lo[x][y][b] = f_to_tf32(wt[x][y][b] - __uint_as_float(hi[x][y][b]));
+            }
+#pragma unroll
+        for (int jj = 0; jj < Sh::kHalves; ++jj) {
           uint4 v[4];
 #pragma unroll
-          for (int x = 0; x < 4; ++x)
-            v[x] = *reinterpret_cast<const uint4*>(vst + ((x & 1) + 8 * (x >> 1)) * kRow + 128 * jj);
+          for (int i = 0; i < 4; ++i) v[i] = load_v(i, jj);
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
+          for (int e = 0; e < 8; ++e)
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-              const uint32_t va = (&v[2 * x].x)[e], vb = (&v[2 * x + 1].x)[e];
-              mma_1688_tf32(o[8 * jj + 2 * e], pf[x], __float_as_uint(half_lo(va)), __float_as_uint(half_lo(vb)));
-              mma_1688_tf32(o[8 * jj + 2 * e + 1], pf[x], __float_as_uint(half_hi(va)), __float_as_uint(half_hi(vb)));
+              const uint32_t v0 = (&v[2 * x].x)[e >> 1], v1 = (&v[2 * x + 1].x)[e >> 1];
+              const uint32_t b0 = __float_as_uint(e & 1 ? half_hi(v0) : half_lo(v0));
+              const uint32_t b1 = __float_as_uint(e & 1 ? half_hi(v1) : half_lo(v1));
+              if constexpr (PACK) {
+                mma_1688_tf32(o[8 * jj + e], hi[x][0][0], lo[x][0][0], hi[x][0][1], lo[x][0][1], b0, b1);
+              } else {
+                constexpr int y = kHeads - 1;
+                mma_1688_tf32(o[8 * jj + e], hi[x][0][0], hi[x][y][0], hi[x][0][1], hi[x][y][1], b0, b1);
+                mma_1688_tf32(o[8 * jj + e], lo[x][0][0], lo[x][y][0], lo[x][0][1], lo[x][y][1], b0, b1);
+              }
             }
         }
       }
-      __syncwarp();
-      issue(i + Sh::kStages - 1, next);  // over the stage that every lane read in the previous step
-      next = lookup(i + Sh::kStages);
+      __syncwarp();  // every lane has read this stage's predecessor: the feed writes over it
+      feed(stage == 0 ? Sh::kStages - 1 : stage - 1);
+      if (++stage == Sh::kStages) {
+        stage = 0;
+        phase ^= 1;
+      }
     }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
-    __syncwarp();  // every lane has read its last stage before the sums go over the ring
 
-    // o[8 jj + e][.]: heads r, r + 8; dimensions 64 jj + 16 c + e and + 8.  Sums over the warps.
+    // o[8 jj + e][2 y + b]: dimension 64 jj + 32 b + 8 c + e of head r + 8 y (PACK: row 8 + r is head r's rest)
 #pragma unroll
-    for (int y = 0; y < 2; ++y) {
+    for (int y = 0; y < kHeads; ++y) {
       z[y] += __shfl_xor_sync(0xffffffffu, z[y], 1);
       z[y] += __shfl_xor_sync(0xffffffffu, z[y], 2);
       const int h = r + 8 * y;
-      if (h < nh) {
-        if (c == 0) rz[warp * p.HU + h] = z[y];
-        float* to = red + warp * kRedWarp + h * (D + 4) + 16 * c;
+      if (h >= nh) continue;
+      const bool whole = w.whole();
+      const bool none = z[y] == 0.f;  // no key with weight: 0, also where eps is 0
+      const float norm = none ? 1.f : z[y] + p.eps;
+      T* out = static_cast<T*>(p.out) + w.s * p.os[0] + (head0 + h) * p.os[1];
+      const int64_t slot = slot_of(worker, w.a == 0);
+      float* part = p.part + (slot * p.HU + h) * D;
 #pragma unroll
-        for (int jj = 0; jj < D / 64; ++jj)
+      for (int jj = 0; jj < Sh::kHalves; ++jj)
 #pragma unroll
-          for (int half = 0; half < 2; ++half)
+        for (int b = 0; b < 2; ++b) {
+          float x[8];
 #pragma unroll
-            for (int e = 0; e < 8; e += 4)
-              *reinterpret_cast<float4*>(to + 64 * jj + 8 * half + e) =
-                  make_float4(o[8 * jj + e][2 * y + half], o[8 * jj + e + 1][2 * y + half],
-                              o[8 * jj + e + 2][2 * y + half], o[8 * jj + e + 3][2 * y + half]);
-      }
+          for (int e = 0; e < 8; ++e) x[e] = PACK ? o[8 * jj + e][b] + o[8 * jj + e][2 + b] : o[8 * jj + e][2 * y + b];
+          const int d = 64 * jj + 32 * b + 8 * c;
+          if (whole) {
+            T t[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) t[e] = from_f32<T>(none ? 0.f : x[e] / norm);
+            uint4 packed;
+            memcpy(&packed, t, 16);
+            *reinterpret_cast<uint4*>(out + d) = packed;
+          } else {
+            *reinterpret_cast<float4*>(part + d) = make_float4(x[0], x[1], x[2], x[3]);
+            *reinterpret_cast<float4*>(part + d + 4) = make_float4(x[4], x[5], x[6], x[7]);
+          }
+        }
+      if (!whole && c == 0) slot_z(p)[slot * p.HU + h] = z[y];
     }
-    __syncthreads();
-    finish_piece<T>(p, red, kRedWarp, rz, s, unit, whole, begins);
-    __syncthreads();  // the sums are read before the ring and rz are written again
-  });
+  } while (w.next(p));
 }
 
 // ------------------------------------------------------------------------------------------
@@ -505,35 +583,36 @@ template <> struct Piece<__half, 8> {
 // Lane (r, c) takes key r of 8 and the pieces c, c + 4, ... of its row (VEC elements each, E = NI VEC of
 // them, E at least D / 4): a dot product is finished by two shuffles among four lanes, the four have the
 // weight, and each adds it times its own part of the value row.  The eight keys' sums meet at the end of the
-// piece.  HU query heads share a read of the row; a kv head with more is several units.
+// piece, the CTA's warps' too.  HU query heads share a read of the row; a kv head with more is several units.
 template <typename T, int VEC, int NI, int HU>
-__global__ void __launch_bounds__(kWarps * 32) paged_born_general(const PagedParams p) {
+__global__ void __launch_bounds__(kThreads) paged_born_general(const PagedParams p) {
   constexpr int E = NI * VEC;
-  extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ int64_t sh[kWarps];
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  __shared__ uint32_t pre[kThreads];
   __shared__ float rz[kWarps * HU];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
-  float* red = reinterpret_cast<float*>(smem);
-  const int red_warp = HU * (p.D + 4);
-  float* qsm = red + kWarps * red_warp;  // [HU][4 E] scaled queries, piece i of lane c at (i * 4 + c) VEC
+  const int ld = p.D + 4;
+  float* red = reinterpret_cast<float*>(smem_raw);  // [kWarps][HU][ld]
+  float* qsm = red + kWarps * HU * ld;              // [HU][4 E] queries, piece i of lane c at (i * 4 + c) VEC
 
   asm volatile("griddepcontrol.launch_dependents;");
-  walk_share(p, sh, [&](int s, const Keys& kk, int unit, int ta, int tb, bool whole, bool begins) {
-    const int kvh = unit / p.chunks, h0 = unit % p.chunks * p.HU, nh = min(p.HU, p.G - h0);
-    const int32_t* table = p.table + s * p.table_stride;
+  const int per = tile_prefix<kThreads>(p, pre);
+  Walk w;
+  if (!w.begin<kThreads>(p, pre, per, blockIdx.x)) return;
+  do {
+    const int kvh = w.unit / p.chunks, h0 = w.unit % p.chunks * HU, nh = min(HU, p.G - h0);
+    const int head0 = kvh * p.G + h0;
+    const int32_t* table = p.table + w.s * p.table_stride;
     const T* kbase = static_cast<const T*>(p.k) + kvh * p.ks[1];
     const T* vbase = static_cast<const T*>(p.v) + kvh * p.vs[1];
-    for (int i = threadIdx.x; i < HU * 4 * E; i += kWarps * 32) {
-      const int h = i / (4 * E), d = i % (4 * E), head = kvh * p.G + h0 + h;
-      float x = 0.f;
-      if (h < nh && d < p.D)
-        x = to_f32(static_cast<const T*>(p.q)[s * p.qs[0] + head * p.qs[1] + d]);
-      qsm[i] = x;
+    for (int i = threadIdx.x; i < HU * 4 * E; i += kThreads) {
+      const int h = i / (4 * E), d = i % (4 * E);
+      qsm[i] = h < nh && d < p.D ? to_f32(static_cast<const T*>(p.q)[w.s * p.qs[0] + (head0 + h) * p.qs[1] + d]) : 0.f;
     }
     float sc[HU];
 #pragma unroll
     for (int h = 0; h < HU; ++h)
-      sc[h] = h < nh ? (p.scale ? p.scale[p.scale_per_head ? kvh * p.G + h0 + h : 0] : p.scale_value) : 0.f;
+      sc[h] = h < nh ? (p.scale ? p.scale[p.scale_per_head ? head0 + h : 0] : p.scale_value) : 0.f;
     __syncthreads();
     float o[HU][E], z[HU];
 #pragma unroll
@@ -542,13 +621,16 @@ __global__ void __launch_bounds__(kWarps * 32) paged_born_general(const PagedPar
 #pragma unroll
       for (int e = 0; e < E; ++e) o[h][e] = 0.f;
     }
-    const int end = min(kk.hi, kk.base + tb * kTile);
-    for (int key0 = kk.base + ta * kTile + warp * 8; key0 < end; key0 += kWarps * 8) {
+    const int end = w.end_key(p);
+    for (int key0 = w.first_key(p) + warp * 8; key0 < end; key0 += kWarps * 8) {
       const int key = key0 + r;
-      int pg = 0, row = 0;
-      const bool counts = key >= kk.lo && key < end && find_page(p, table, key, pg, row);
-      const T* k = kbase + pg * p.ks[0] + row * p.ks[2];
-      const T* v = vbase + pg * p.vs[0] + row * p.vs[2];
+      int pg = -1, row = 0;
+      if (key >= w.k.lo && key < end) {
+        const int i = key / p.page;
+        pg = table[i];
+        row = key - i * p.page;
+      }
+      const bool counts = pg >= 0 && pg < p.pages;
       float kf[NI][VEC], vf[NI][VEC];
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
@@ -556,8 +638,8 @@ __global__ void __launch_bounds__(kWarps * 32) paged_born_general(const PagedPar
 #pragma unroll
         for (int e = 0; e < VEC; ++e) kf[i][e] = vf[i][e] = 0.f;
         if (counts && d < p.D) {
-          Piece<T, VEC>::load(k + d, kf[i]);
-          Piece<T, VEC>::load(v + d, vf[i]);
+          Piece<T, VEC>::load(kbase + pg * p.ks[0] + row * p.ks[2] + d, kf[i]);
+          Piece<T, VEC>::load(vbase + pg * p.vs[0] + row * p.vs[2] + d, vf[i]);
         }
       }
 #pragma unroll
@@ -570,12 +652,12 @@ __global__ void __launch_bounds__(kWarps * 32) paged_born_general(const PagedPar
         dot += __shfl_xor_sync(0xffffffffu, dot, 1);
         dot += __shfl_xor_sync(0xffffffffu, dot, 2);
         const float a = relu(dot * sc[h]);
-        const float w = counts ? a * a : 0.f;
-        z[h] += w;
+        const float wt = counts ? a * a : 0.f;
+        z[h] += wt;
 #pragma unroll
         for (int i = 0; i < NI; ++i)
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) o[h][i * VEC + e] = fmaf(w, vf[i][e], o[h][i * VEC + e]);
+          for (int e = 0; e < VEC; ++e) o[h][i * VEC + e] = fmaf(wt, vf[i][e], o[h][i * VEC + e]);
       }
     }
 #pragma unroll
@@ -588,55 +670,79 @@ __global__ void __launch_bounds__(kWarps * 32) paged_born_general(const PagedPar
 #pragma unroll
         for (int x = 4; x < 32; x <<= 1) o[h][e] += __shfl_xor_sync(0xffffffffu, o[h][e], x);
         const int d = (e / VEC * 4 + c) * VEC + e % VEC;
-        if (r == 0 && d < p.D) red[warp * red_warp + h * (p.D + 4) + d] = o[h][e];
+        if (r == 0 && d < p.D) red[(warp * HU + h) * ld + d] = o[h][e];
       }
     }
     __syncthreads();
-    finish_piece<T>(p, red, red_warp, rz, s, unit, whole, begins);
-    __syncthreads();
-  });
+    const int64_t slot = slot_of(blockIdx.x, w.a == 0);
+    for (int h = 0; h < nh; ++h) {
+      float zs = 0.f;
+#pragma unroll
+      for (int x = 0; x < kWarps; ++x) zs += rz[x * HU + h];
+      for (int d = threadIdx.x; d < p.D; d += kThreads) {
+        float os = 0.f;
+#pragma unroll
+        for (int x = 0; x < kWarps; ++x) os += red[(x * HU + h) * ld + d];
+        if (w.whole())
+          (static_cast<T*>(p.out) + w.s * p.os[0] + (head0 + h) * p.os[1])[d] =
+              from_f32<T>(zs == 0.f ? 0.f : os / (zs + p.eps));
+        else
+          p.part[(slot * HU + h) * p.D + d] = os;
+      }
+      if (!w.whole() && threadIdx.x == 0) slot_z(p)[slot * HU + h] = zs;
+    }
+    __syncthreads();  // the sums are read before the next piece writes them
+  } while (w.next(p));
 }
 
 // ------------------------------------------------------------------------------------------
-// The pieces of units that span several CTAs' shares, added in share order: one CTA per query head,
-// kJoinThreads / D' threads (D' = D rounded up to a power of two) on each dimension.
+// The pieces of units that span several shares, added in share order.  `ways` warps (a power of two) on
+// 32 dimensions of a query head, one on every ways-th piece; blocks of max(8, ways) warps.
 // ------------------------------------------------------------------------------------------
-template <typename T>
-__global__ void __launch_bounds__(kJoinThreads) paged_join(const PagedParams p) {
-  __shared__ int64_t sh[kJoinThreads / 32];
-  __shared__ float so[kJoinThreads], sz[kJoinThreads];
-  const int s = blockIdx.x / p.H, head = blockIdx.x % p.H;
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS) paged_join(const PagedParams p, int ways) {
+  __shared__ uint32_t pre[THREADS];
+  __shared__ float so[THREADS], sz[THREADS / 32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, slices = (p.D + 31) / 32;
+  const int per = tile_prefix<THREADS>(p, pre);
+  const int64_t item = (int64_t)blockIdx.x * (THREADS / 32 / ways) + warp / ways;
+  const bool work = item < (int64_t)p.S * p.H * slices;
+  const int way = warp % ways, d = (int)(item % slices) * 32 + lane;
+  const int s = work ? (int)(item / slices / p.H) : 0, head = work ? (int)(item / slices % p.H) : 0;
   const int kvh = head / p.G, chunk = head % p.G / p.HU, h = head % p.G % p.HU;
-  const int64_t total = tiles_before<kJoinThreads>(p, p.S, sh) * p.U;
-  const int64_t before = tiles_before<kJoinThreads>(p, s, sh) * p.U;
-  const int n = keys_of(p, s).tiles;
-  const int64_t t0 = before + (int64_t)(kvh * p.chunks + chunk) * n;
-  // CTA of tile t: the last one whose share starts at or before it
-  const int64_t C = min((int64_t)p.C, total);
-  const int c0 = (int)(((t0 + 1) * C - 1) / total), c1 = (int)(((t0 + n) * C - 1) / total);
+  // tiles before sequence s: those of the groups before its own, and of the sequences before it in that
+  const int g = s / per;
+  uint32_t before = 0;
+  for (int x = g * per + lane; x < s; x += 32) before += keys_of(p, x).tiles * p.U;
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) before += __shfl_xor_sync(0xffffffffu, before, x);
+  if (g > 0) before += pre[g - 1];
+  const uint32_t n = keys_of(p, s).tiles;
+  const uint32_t t0 = before + (uint32_t)(kvh * p.chunks + chunk) * n;
+  const Shares sh(pre[THREADS - 1], p.W);
+  const uint32_t w0 = sh.owner(t0), w1 = sh.owner(t0 + n - 1);
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (c0 == c1) return;  // finished by that CTA
-  int width = 1;
-  while (width < p.D) width <<= 1;
-  const int ways = kJoinThreads / width, way = threadIdx.x / width, d = threadIdx.x % width;
-  const float* zs = p.part + (int64_t)p.C * 2 * p.HU * p.D;
   float o = 0.f, z = 0.f;
-  if (d < p.D) {
-#pragma unroll 4
-    for (int c = c0 + way; c <= c1; c += ways) {
-      const int64_t slot = (int64_t)c * 2 + (c == c0 ? 1 : 0);
+  if (work && w0 != w1 && d < p.D) {
+    const float* zs = slot_z(p);
+#pragma unroll 8
+    for (uint32_t w = w0 + way; w <= w1; w += ways) {
+      const int64_t slot = slot_of(w, w == w0);
       o += p.part[(slot * p.HU + h) * p.D + d];
       z += zs[slot * p.HU + h];
     }
   }
-  so[threadIdx.x] = o;
-  sz[threadIdx.x] = z;
-  __syncthreads();
-  if (way == 0 && d < p.D) {
-    for (int w = 1; w < ways; ++w) {
-      o += so[w * width + d];
-      z += sz[w * width + d];
-    }
+  if (ways > 1) {
+    so[threadIdx.x] = o;
+    if (lane == 0) sz[warp] = z;
+    __syncthreads();
+    if (way == 0)
+      for (int x = 1; x < ways; ++x) {
+        o += so[threadIdx.x + 32 * x];
+        z += sz[warp + x];
+      }
+  }
+  if (work && w0 != w1 && d < p.D && way == 0) {
     T* out = static_cast<T*>(p.out) + s * p.os[0] + head * p.os[1];
     out[d] = from_f32<T>(z == 0.f ? 0.f : o / (z + p.eps));
   }
@@ -755,11 +861,13 @@ bool aligned16(const void* p, const int64_t* s, int n, int size) {
 
 // What a call launches, from sizes, types and alignment alone.
 struct PagedPlan {
-  bool tc;        // the tensor-core kernel
-  int vec;        // CUDA-core kernel: elements per load
-  int size_class; // ... and 0, 1, 2: D up to 64, 128, 256
+  bool tc;         // the tensor-core kernel
+  bool pack;       // ... with up to 8 heads per unit
+  int vec;         // CUDA-core kernel: elements per load
+  int size_class;  // ... and 0, 1, 2: D up to 64, 128, 256
   bool join;
-  int HU, chunks, C;
+  int HU, chunks, tile;
+  uint32_t W;
   size_t workspace;
 };
 
@@ -768,22 +876,27 @@ PagedPlan plan_paged(const fb_paged_args* a) {
   const int G = a->heads / a->kv_heads, size = a->dtype == FB_F32 ? 4 : 2;
   const bool rows16 = a->head_dim * size % 16 == 0 && aligned16(a->k, a->k_stride, 3, size) &&
                       aligned16(a->v, a->v_stride, 3, size);
-  pl.tc = size == 2 && (a->head_dim == 64 || a->head_dim == 128) && rows16 && aligned16(a->q, a->q_stride, 2, size);
+  pl.tc = size == 2 && (a->head_dim == 64 || a->head_dim == 128) && rows16 && aligned16(a->q, a->q_stride, 2, size) &&
+          aligned16(a->out, a->out_stride, 2, size);
+  pl.pack = G <= 8;
   pl.vec = rows16 ? 16 / size : 1;
   pl.size_class = a->head_dim <= 64 ? 0 : a->head_dim <= 128 ? 1 : 2;
-  const int hu = pl.tc ? 16 : 4 >> pl.size_class;
-  pl.HU = hu;
-  pl.chunks = (G + hu - 1) / hu;
-  // The most tiles that the lengths can give: the table's capacity, or the window and what it straddles
+  pl.HU = pl.tc ? (pl.pack ? 8 : 16) : 4 >> pl.size_class;
+  pl.chunks = (G + pl.HU - 1) / pl.HU;
+  // The most keys a unit can have: the table's capacity, or the window and what its start is rounded down by
   int64_t cap = (int64_t)a->page_size * a->max_pages;
   if (a->window_size > 0) cap = std::min<int64_t>(cap, (int64_t)a->window_size + kSub);
-  const int64_t per_unit = std::max<int64_t>((cap + kTile - 1) / kTile, 1);
   const int64_t units = (int64_t)a->seqs * a->kv_heads * pl.chunks;
-  const int per_sm = pl.tc ? (a->head_dim == 64 ? TcShape<64>::kCtasPerSm : TcShape<128>::kCtasPerSm) : 4;
-  // units of one tile cannot be cut: one CTA each, nothing to join
-  pl.join = per_unit > 1;
-  pl.C = (int)std::min<int64_t>(units * per_unit, pl.join ? (int64_t)per_sm * sm_count() : 0x7FFFFFFF);
-  pl.workspace = pl.join ? (size_t)pl.C * 2 * pl.HU * (a->head_dim + 1) * sizeof(float) : 0;
+  // Up to 64 keys take one worker less time than cutting them and a second kernel; longer units are cut
+  // finely, so that shares differ little (and coarsely enough that all tiles count in 31 bits).
+  pl.join = cap > 64;
+  int64_t tile = pl.join ? 2 * kSub : 64;
+  while (units * ((cap + tile - 1) / tile) > 0x7FFFFFFF) tile *= 2;
+  pl.tile = (int)std::min<int64_t>(tile, 1 << 30);
+  const int64_t tiles = units * std::max<int64_t>((cap + tile - 1) / tile, 1);
+  const int per_sm = pl.tc ? kWarps * (a->head_dim == 64 ? TcShape<64>::kCtasPerSm : TcShape<128>::kCtasPerSm) : 4;
+  pl.W = (uint32_t)std::min<int64_t>(tiles, pl.join ? (int64_t)per_sm * sm_count() : 0x7FFFFFFF);
+  pl.workspace = pl.join ? (size_t)pl.W * 2 * pl.HU * (a->head_dim + 1) * sizeof(float) : 0;
   return pl;
 }
 
@@ -791,7 +904,7 @@ int check_paged(const fb_paged_args* a) {
   if (a == nullptr) return FB_ERR_ARG;
   if (a->seqs < 0 || a->heads < 1 || a->kv_heads < 1 || a->heads % a->kv_heads != 0 || a->heads > 65535 ||
       a->head_dim < 1 || a->head_dim > 256 || a->page_size < 1 || a->num_pages < 0 || a->max_pages < 0 ||
-      (int64_t)a->page_size * a->max_pages > 0x7FFFFFFF - 2 * kTile || (int64_t)a->seqs * a->heads > 0x7FFFFFFF)
+      (int64_t)a->page_size * a->max_pages > 0x7FFFFFFF - 256 || (int64_t)a->seqs * a->heads > 0x0FFFFFFF)
     return FB_ERR_SHAPE;
   if (bad_dtype(a->dtype)) return FB_ERR_DTYPE;
   if (a->window_size < 0 || !(a->eps >= 0.f)) return FB_ERR_ARG;
@@ -809,8 +922,8 @@ int check_paged(const fb_paged_args* a) {
 template <typename T>
 cudaError_t launch_general(const PagedParams& p, const PagedPlan& pl, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T);
-  const int smem = (kWarps * p.HU * (p.D + 4) + p.HU * (256 >> (2 - pl.size_class))) * (int)sizeof(float);
-  const dim3 grid(p.C), block(kWarps * 32);
+  const int smem = (kWarps * p.HU * (p.D + 4) + p.HU * (64 << pl.size_class)) * (int)sizeof(float);
+  const dim3 grid(p.W), block(kThreads);
   if (pl.vec > 1) {
     if (pl.size_class == 0) paged_born_general<T, V, 16 / V, 4><<<grid, block, smem, st>>>(p);
     else if (pl.size_class == 1) paged_born_general<T, V, 32 / V, 2><<<grid, block, smem, st>>>(p);
@@ -823,38 +936,66 @@ cudaError_t launch_general(const PagedParams& p, const PagedPlan& pl, cudaStream
   return cudaGetLastError();
 }
 
-template <typename T, int D>
-cudaError_t launch_tc(const PagedParams& p, cudaStream_t st) {
-  const cudaError_t e = set_smem_limit_once(reinterpret_cast<const void*>(&paged_born_tc<T, D>), TcShape<D>::kSmem);
+// TMA maps of the pages, (B, H, T, D) = (page, kv head, row, dimension); false where TMA cannot take them:
+// a step's 16 keys must lie in one page, and every stride be positive.
+bool page_maps(const PagedParams& p, CUtensorMap* k, CUtensorMap* v) {
+  if (p.width == 0 || p.page % kSub != 0) return false;
+  const Tensor4 tk{p.k, {p.ks[0], p.ks[1], p.ks[2], 1}}, tv{p.v, {p.vs[0], p.vs[1], p.vs[2], 1}};
+  return tma_ok(tk) && tma_ok(tv) && encode_bhtd(k, tk, p.pages, p.Hkv, p.page, p.D, kSub, false) &&
+         encode_bhtd(v, tv, p.pages, p.Hkv, p.page, p.D, kSub, false);
+}
+
+template <typename T, int D, bool PACK, bool TMA>
+cudaError_t launch_tc(const PagedParams& p, const CUtensorMap& k, const CUtensorMap& v, cudaStream_t st) {
+  const auto kernel = &paged_born_tc<T, D, PACK, TMA>;
+  const cudaError_t e = set_smem_limit_once(reinterpret_cast<const void*>(kernel), TcShape<D>::kSmem);
   if (e != cudaSuccess) return e;
-  paged_born_tc<T, D><<<p.C, kWarps * 32, TcShape<D>::kSmem, st>>>(p);
+  kernel<<<(p.W + kWarps - 1) / kWarps, kThreads, TcShape<D>::kSmem, st>>>(p, k, v);
   return cudaGetLastError();
 }
 
-template <typename T>
-cudaError_t launch_paged(const PagedParams& p, const PagedPlan& pl, cudaStream_t st) {
-  cudaError_t e;
-  if constexpr (sizeof(T) == 2) {
-    e = !pl.tc ? launch_general<T>(p, pl, st) : p.D == 64 ? launch_tc<T, 64>(p, st) : launch_tc<T, 128>(p, st);
-  } else {
-    e = launch_general<T>(p, pl, st);
-  }
-  if (e != cudaSuccess || !pl.join) return e;
-  // the join's CTAs start while the last shares still run (their count is read meanwhile) and wait for them
+template <typename T, int D>
+cudaError_t launch_tc(const PagedParams& p, const PagedPlan& pl, cudaStream_t st) {
+  CUtensorMap k{}, v{};
+  const bool tma = page_maps(p, &k, &v);
+  if (pl.pack) return tma ? launch_tc<T, D, true, true>(p, k, v, st) : launch_tc<T, D, true, false>(p, k, v, st);
+  return tma ? launch_tc<T, D, false, true>(p, k, v, st) : launch_tc<T, D, false, false>(p, k, v, st);
+}
+
+template <typename T, int THREADS>
+cudaError_t launch_join(const PagedParams& p, int ways, cudaStream_t st) {
+  // its CTAs start while the last shares still run (what they need of the lengths is read meanwhile), and wait
+  const int64_t items = (int64_t)p.S * p.H * ((p.D + 31) / 32), each = THREADS / 32 / ways;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(p.S * p.H));
-  cfg.blockDim = dim3(kJoinThreads);
+  cfg.gridDim = dim3((unsigned)((items + each - 1) / each));
+  cfg.blockDim = dim3(THREADS);
   cfg.stream = st;
   cudaLaunchAttribute at{};
   at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, paged_join<T>, p);
+  return cudaLaunchKernelEx(&cfg, paged_join<T, THREADS>, p, ways);
+}
+
+template <typename T>
+cudaError_t launch_paged(const PagedParams& p, const PagedPlan& pl, cudaStream_t st) {
+  cudaError_t e;
+  if constexpr (sizeof(T) == 2) {
+    e = !pl.tc ? launch_general<T>(p, pl, st) : p.D == 64 ? launch_tc<T, 64>(p, pl, st) : launch_tc<T, 128>(p, pl, st);
+  } else {
+    e = launch_general<T>(p, pl, st);
+  }
+  if (e != cudaSuccess || !pl.join) return e;
+  // as many warps on an output as a unit has pieces, were the lengths alike
+  const uint32_t pieces = p.W / ((uint32_t)p.S * p.U) + 1;
+  int ways = 1;
+  while (ways < 32 && ways < (int)pieces) ways *= 2;
+  return ways <= 8 ? launch_join<T, 256>(p, ways, st) : launch_join<T, 1024>(p, ways, st);
 }
 
 int paged_fwd(const fb_paged_args* a, cudaStream_t st) {
-  const int rc = check_paged(a);
+  int rc = check_paged(a);
   if (rc != FB_OK) return rc;
   if (a->seqs == 0) {
     set_last_launch_count(0);
@@ -866,17 +1007,16 @@ int paged_fwd(const fb_paged_args* a, cudaStream_t st) {
   p.S = a->seqs; p.H = a->heads; p.Hkv = a->kv_heads; p.G = a->heads / a->kv_heads; p.D = a->head_dim;
   p.page = a->page_size; p.pages = a->num_pages;
   p.width = a->num_pages > 0 ? a->max_pages : 0;
-  p.page_shift = -1;
-  if ((p.page & (p.page - 1)) == 0)
-    for (p.page_shift = 0; (1 << p.page_shift) < p.page;) ++p.page_shift;
   p.window = a->window_size; p.eps = a->eps; p.scale_value = a->scale_value;
   p.scale = a->scale; p.scale_per_head = a->scale_numel > 1;
   p.q = a->q; p.k = a->k; p.v = a->v; p.out = a->out;
   for (int i = 0; i < 3; ++i) p.qs[i] = a->q_stride[i], p.os[i] = a->out_stride[i];
   for (int i = 0; i < 4; ++i) p.ks[i] = a->k_stride[i], p.vs[i] = a->v_stride[i];
   p.table = a->table; p.table_stride = a->table_stride; p.lens = a->lens;
-  p.HU = pl.HU; p.chunks = pl.chunks; p.U = p.Hkv * p.chunks; p.C = pl.C;
+  p.HU = pl.HU; p.chunks = pl.chunks; p.U = p.Hkv * p.chunks; p.tile = pl.tile; p.W = pl.W;
   p.part = static_cast<float*>(a->workspace);
+  p.status = device_status_word(&rc);
+  if (rc != FB_OK) return rc;
   cudaError_t e;
   if (a->dtype == FB_F32) e = launch_paged<float>(p, pl, st);
   else if (a->dtype == FB_F16) e = launch_paged<__half>(p, pl, st);
