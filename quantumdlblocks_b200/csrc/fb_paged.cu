@@ -207,8 +207,8 @@ template <int D> struct TcShape {
   static constexpr int kHalves = D / 64;                  // 128-byte rows per key
   static constexpr int kHalfBytes = kSub * 128;
   static constexpr int kStageBytes = 2 * kHalves * kHalfBytes;  // per warp: kSub keys, then their values
-  static constexpr int kStages = D == 64 ? 4 : 3;
-  static constexpr int kCtasPerSm = D == 64 ? 3 : 2;
+  static constexpr int kStages = 3;
+  static constexpr int kCtasPerSm = D == 64 ? 4 : 2;
   static constexpr int kSmem = kWarps * kStages * kStageBytes + 1024;  // + alignment of the swizzle
 };
 
@@ -705,10 +705,10 @@ __global__ void __launch_bounds__(THREADS) paged_join(const PagedParams p, int w
   __shared__ float so[THREADS], sz[THREADS / 32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, slices = (p.D + 31) / 32;
   const int per = tile_prefix<THREADS>(p, pre);
-  const int64_t item = (int64_t)blockIdx.x * (THREADS / 32 / ways) + warp / ways;
-  const bool work = item < (int64_t)p.S * p.H * slices;
-  const int way = warp % ways, d = (int)(item % slices) * 32 + lane;
-  const int s = work ? (int)(item / slices / p.H) : 0, head = work ? (int)(item / slices % p.H) : 0;
+  const uint32_t item = blockIdx.x * (THREADS / 32 / ways) + warp / ways, row = item / slices;
+  const bool work = row < (uint32_t)(p.S * p.H);
+  const int way = warp & (ways - 1), d = (int)(item - row * slices) * 32 + lane;
+  const int s = work ? (int)(row / p.H) : 0, head = work ? (int)(row % p.H) : 0;
   const int kvh = head / p.G, chunk = head % p.G / p.HU, h = head % p.G % p.HU;
   // tiles before sequence s: those of the groups before its own, and of the sequences before it in that
   const int g = s / per;
@@ -987,10 +987,11 @@ cudaError_t launch_paged(const PagedParams& p, const PagedPlan& pl, cudaStream_t
     e = launch_general<T>(p, pl, st);
   }
   if (e != cudaSuccess || !pl.join) return e;
-  // as many warps on an output as a unit has pieces, were the lengths alike
+  // A warp has eight pieces' loads under way at a time: a warp on an output for every eight of the pieces that a
+  // unit would have were the lengths alike (49 pieces of 192 units: 27 us with 32 warps each, 5 us with 8)
   const uint32_t pieces = p.W / ((uint32_t)p.S * p.U) + 1;
   int ways = 1;
-  while (ways < 32 && ways < (int)pieces) ways *= 2;
+  while (ways < 32 && ways * 8 < (int)pieces) ways *= 2;
   return ways <= 8 ? launch_join<T, 256>(p, ways, st) : launch_join<T, 1024>(p, ways, st);
 }
 
