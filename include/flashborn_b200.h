@@ -435,10 +435,11 @@ FB_API int fb_paged_qkv_write(const fb_paged_write_args* args, void* stream);
  *   lse = log sum_c exp(x_c);  logp = x_t - lse;  entropy = lse - sum_c p_c x_c
  *   top: the top_k largest x_c, equal ones by lowest index, NaN above everything: x_c - lse, c
  * -inf columns have no probability; a row with nothing but them, a +inf or a NaN is NaN, and so is
- * the logp of a target outside [0, vocab).  logp, entropy, lse, top_logp fp32; top_index int64.
+ * the logp of a target outside [0, vocab).  logp, entropy, top_logp fp32; top_index int64.
  *   backward   grad_c = g_logp ([c == t] - p_c) + sum_i g_top_i ([c == top_i] - p_c)
  *                       - g_entropy p_c (log p_c + entropy)
- * Any of g_logp, g_entropy, g_top may be NULL (zero).  top_k <= FB_MAX_TOP_K. */
+ * Any of g_logp, g_entropy, g_top may be NULL (zero); a row whose gradients all are 0 gets 0, whatever it
+ * holds.  top_k <= FB_MAX_TOP_K. */
 #define FB_MAX_TOP_K 64
 typedef struct fb_logprob_args {
   int64_t rows;
@@ -447,7 +448,7 @@ typedef struct fb_logprob_args {
   const int64_t* targets;
   float* logp;
   float* entropy;
-  float* lse;
+  float* stats;           /* (rows, 2): max x and log2 sum_c 2^((x_c - max) log2 e), for the backward */
   float* top_logp;        /* (rows, top_k) contiguous */
   int64_t* top_index;
   const float* g_logp;

@@ -162,7 +162,7 @@ class FbLogprobArgs(ctypes.Structure):
     _fields_ = [
         ("rows", ctypes.c_int64), ("vocab", ctypes.c_int32), ("dtype", ctypes.c_int32), ("top_k", ctypes.c_int32),
         ("logits", ctypes.c_void_p), ("ld", ctypes.c_int64), ("targets", ctypes.c_void_p),
-        ("logp", ctypes.c_void_p), ("entropy", ctypes.c_void_p), ("lse", ctypes.c_void_p),
+        ("logp", ctypes.c_void_p), ("entropy", ctypes.c_void_p), ("stats", ctypes.c_void_p),
         ("top_logp", ctypes.c_void_p), ("top_index", ctypes.c_void_p),
         ("g_logp", ctypes.c_void_p), ("g_entropy", ctypes.c_void_p), ("g_top", ctypes.c_void_p),
         ("grad", ctypes.c_void_p), ("grad_ld", ctypes.c_int64),

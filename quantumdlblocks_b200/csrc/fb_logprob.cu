@@ -2,16 +2,34 @@
 //
 //   forward   lse = log sum exp x, logp = x_t - lse, entropy = lse - sum p x, the top_k largest x
 //   backward  grad = g_logp ([c = t] - p) + sum_i g_top_i ([c = top_i] - p) - g_entropy p (log p + entropy)
+//
+// The forward reads the logits once, the backward reads them and writes the gradient: HBM bandwidth bounds
+// both for many rows, latency for few, where a cluster of CTAs shares a row and joins over distributed
+// shared memory.  A thread carries the running maximum m of its columns with s = sum 2^t and u = sum 2^t t,
+// t = (x - m) log2 e; then log2 sum = log2 s, entropy = ln 2 (log2 s - u / s).  All sums are fp32.
+//
+// The alternatives cost one extra look at a few columns: a thread also remembers where its maximum was.  The
+// K-th largest of the maxima of at least K groups of threads bounds the K-th largest logit from below, only
+// threads whose own maximum reaches it can hold one of the K, and their columns (a few hundred of 50,000) are
+// read again, from cache.
+#include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 
 #include "fb_common.cuh"
 
+namespace cg = cooperative_groups;
+
 namespace fb {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 512;
+constexpr int kWarps = kThreads / 32;
+constexpr int kCandidates = 1024;
+constexpr int kMaxCluster = 8;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct LogprobParams {
   int64_t rows;
@@ -21,7 +39,7 @@ struct LogprobParams {
   const int64_t* targets;
   float* logp;
   float* entropy;
-  float* lse;
+  float* stats;
   float* top_logp;
   int64_t* top_index;
   const float* g_logp;
@@ -31,110 +49,540 @@ struct LogprobParams {
   int64_t grad_ld;
 };
 
-__device__ __forceinline__ float block_max(float v, float* sh) {
-  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = sh[0];
-  for (int i = 1; i < kThreads / 32; ++i) v = fmaxf(v, sh[i]);
-  return v;
+__device__ __forceinline__ float ex2(float x) {  // 2^x, flushing to 0 below 2^-126; NaN stays
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
 }
 
-__device__ __forceinline__ float block_sum(float v, float* sh) {
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = sh[0];
-  for (int i = 1; i < kThreads / 32; ++i) v += sh[i];
-  return v;
+// ------------------------------------------------------------------------------------------
+// A row in 16-byte chunks: chunk j is columns [j N - shift, (j + 1) N - shift) of the row, aligned in memory
+// whatever the row's start; what falls outside the row reads as -inf.
+// ------------------------------------------------------------------------------------------
+template <typename T> struct Bits;
+template <> struct Bits<float> {
+  static constexpr uint32_t kNegInf = 0xFF800000u;
+};
+template <> struct Bits<__half> {
+  static constexpr uint32_t kNegInf = 0xFC00FC00u;
+};
+template <> struct Bits<__nv_bfloat16> {
+  static constexpr uint32_t kNegInf = 0xFF80FF80u;
+};
+
+template <typename T> struct Row {
+  static constexpr int N = 16 / sizeof(T);
+  const T* x;
+  int V, shift, chunks;
+  __device__ Row(const T* row, int vocab) : x(row), V(vocab) {
+    shift = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
+    chunks = (V + shift + N - 1) / N;
+  }
+  __device__ int column(int j) const { return j * N - shift; }
+  __device__ bool inside(int j) const { return column(j) >= 0 && column(j) + N <= V; }
+  __device__ uint4 load(int j) const {
+    const int c = column(j);
+    if (inside(j)) return __ldg(reinterpret_cast<const uint4*>(x + c));
+    uint4 w = make_uint4(Bits<T>::kNegInf, Bits<T>::kNegInf, Bits<T>::kNegInf, Bits<T>::kNegInf);
+    T* e = reinterpret_cast<T*>(&w);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (c + i >= 0 && c + i < V) e[i] = x[c + i];
+    return w;
+  }
+};
+
+__device__ __forceinline__ void unpack(const uint4& w, float (&f)[4], const float*) {
+  f[0] = __uint_as_float(w.x), f[1] = __uint_as_float(w.y), f[2] = __uint_as_float(w.z), f[3] = __uint_as_float(w.w);
+}
+__device__ __forceinline__ void unpack(const uint4& w, float (&f)[8], const __nv_bfloat16*) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[2 * i] = __uint_as_float((&w.x)[i] << 16);
+    f[2 * i + 1] = __uint_as_float((&w.x)[i] & 0xFFFF0000u);
+  }
+}
+__device__ __forceinline__ void unpack(const uint4& w, float (&f)[8], const __half*) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t b = (&w.x)[i];
+    const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&b));
+    f[2 * i] = v.x;
+    f[2 * i + 1] = v.y;
+  }
 }
 
-// 32 bits that order as the float does, NaN above everything, -0 and 0 alike
+// The lowest value that the sums use in place of anything lower (-inf too), and the lowest maximum for which
+// that changes nothing: the weight of what was replaced is 0.  A row below it takes the slow path.
+template <typename T> struct Floor {
+  static constexpr float kFloor = -8.5e37f, kLowestMax = -1e29f;  // kFloor log2 e is finite
+};
+template <> struct Floor<__half> {
+  static constexpr float kFloor = -65504.f, kLowestMax = -60000.f;
+};
+
+// Floor and maximum of a chunk, on packed pairs for the 16-bit types; a NaN stays in the values and is left
+// out of the maximum.
+__device__ __forceinline__ float prepare(uint4& w, float (&f)[4], const float* t) {
+  unpack(w, f, t);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f[i] = max_nan(f[i], Floor<float>::kFloor);
+  return fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3]));
+}
+template <typename P, typename T>
+__device__ __forceinline__ float prepare_pairs(uint4& w, float (&f)[8], const T* t, P low) {
+  P v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[i] = __hmax2_nan(*reinterpret_cast<P*>(&(&w.x)[i]), low);
+    (&w.x)[i] = *reinterpret_cast<uint32_t*>(&v[i]);
+  }
+  unpack(w, f, t);
+  const P m = __hmax2(__hmax2(v[0], v[1]), __hmax2(v[2], v[3]));
+  return fmaxf(to_f32(m.x), to_f32(m.y));
+}
+__device__ __forceinline__ float prepare(uint4& w, float (&f)[8], const __nv_bfloat16* t) {
+  return prepare_pairs<__nv_bfloat162>(w, f, t, __float2bfloat162_rn(Floor<__nv_bfloat16>::kFloor));
+}
+__device__ __forceinline__ float prepare(uint4& w, float (&f)[8], const __half* t) {
+  return prepare_pairs<__half2>(w, f, t, __float2half2_rn(Floor<__half>::kFloor));
+}
+
+// ------------------------------------------------------------------------------------------
+// Sums of columns: s = sum 2^t, u = sum 2^t t for t = (x - m) log2 e
+// ------------------------------------------------------------------------------------------
+struct Sums {
+  float m, s, u;
+};
+__device__ __forceinline__ void rescale(Sums& a, float m) {  // to a maximum m >= a.m, both finite
+  const float d = (a.m - m) * kLog2e, f = ex2(d);
+  a.u = f * fmaf(a.s, fmaxf(d, -1e30f), a.u);
+  a.s *= f;
+  a.m = m;
+}
+__device__ __forceinline__ Sums join(Sums a, Sums b) {
+  const float m = fmaxf(a.m, b.m);
+  rescale(a, m);
+  rescale(b, m);
+  return {m, a.s + b.s, a.u + b.u};
+}
+__device__ __forceinline__ Sums shuffle_join(Sums a, int o) {
+  return join(a, {__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o),
+                  __shfl_xor_sync(0xffffffffu, a.u, o)});
+}
+
+// 32 bits that order as the float does, NaN above everything, -0 and 0 alike; and back
 __device__ __forceinline__ uint32_t ordered(float x) {
   if (x != x) return 0xFFFFFFFFu;
   const uint32_t u = __float_as_uint(x + 0.f);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
+// (value, column) as one number: the greater value first, then the lower column
+__device__ __forceinline__ uint64_t order_key(float x, int c) { return (uint64_t)ordered(x) << 32 | (uint32_t)~c; }
+__device__ __forceinline__ int key_column(uint64_t k) { return (int)~(uint32_t)k; }
 
-// (value, column) as one number: greater value first, then the lower column
-__device__ __forceinline__ uint64_t order_key(float x, int c) {
-  return (uint64_t)ordered(x) << 32 | (uint32_t)~c;
+struct Shared {
+  Sums warp[kWarps];
+  Sums cta;                        // of the CTA's part of the row
+  uint64_t group[64];
+  uint64_t threshold;
+  uint32_t holders, candidates;
+  uint16_t holder[kThreads];
+  uint64_t candidate[kCandidates];
+  uint64_t top[64];                // the CTA's alternatives, in order
+  uint64_t merged[kMaxCluster * 64];
+  uint64_t best;
+};
+
+// ---- the row by itself, column by column: what the fast path cannot take (NaN, +inf, nothing above the
+// floor), and the alternatives where too many columns are equal
+template <typename T>
+__device__ Sums slow_sums(const Row<T>& row, Shared& sh) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  float m = -INFINITY;
+  for (int c = threadIdx.x; c < row.V; c += kThreads) m = max_nan(m, to_f32(row.x[c]));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+  __syncthreads();
+  if (lane == 0) sh.warp[warp].m = m;
+  __syncthreads();
+  for (int w = 0; w < kWarps; ++w) m = max_nan(m, sh.warp[w].m);
+  float s = 0.f, u = 0.f;
+  for (int c = threadIdx.x; c < row.V; c += kThreads) {
+    const float t = (to_f32(row.x[c]) - m) * kLog2e, e = ex2(t);  // NaN where m is not finite
+    s += e;
+    u += e * (t < -200.f ? -200.f : t);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    s += __shfl_xor_sync(0xffffffffu, s, o);
+    u += __shfl_xor_sync(0xffffffffu, u, o);
+  }
+  __syncthreads();
+  if (lane == 0) sh.warp[warp].s = s, sh.warp[warp].u = u;
+  __syncthreads();
+  s = u = 0.f;
+  for (int w = 0; w < kWarps; ++w) s += sh.warp[w].s, u += sh.warp[w].u;
+  __syncthreads();
+  return {m, s, u};
 }
 
+// the K largest of chunks [j0, j1) into sh.top, one at a time: the largest below the last one taken
 template <typename T>
-__global__ void __launch_bounds__(kThreads) logprob_fwd_simple(const LogprobParams p) {
-  __shared__ float sh[kThreads / 32];
-  __shared__ uint64_t best;
-  const int64_t row = blockIdx.x;
-  const T* x = static_cast<const T*>(p.x) + row * p.ld;
-  float m = -INFINITY;
-  for (int c = threadIdx.x; c < p.V; c += kThreads) m = fmaxf(m, to_f32(x[c]));
-  m = block_max(m, sh);
-  float s = 0.f, u = 0.f;
-  for (int c = threadIdx.x; c < p.V; c += kThreads) {
-    const float d = to_f32(x[c]) - m, e = expf(d);
-    s += e;
-    u += e * fmaxf(d, -1e30f);  // a column at -inf adds 0, not 0 * inf
-  }
-  s = block_sum(s, sh);
-  u = block_sum(u, sh);
-  const float lse = m + logf(s);
-  if (threadIdx.x == 0) {
-    const int64_t t = p.targets[row];
-    p.lse[row] = lse;
-    p.logp[row] = (t >= 0 && t < p.V) ? (to_f32(x[t]) - m) - logf(s) : NAN;
-    p.entropy[row] = logf(s) - u / s;
-  }
+__device__ void slow_top(const Row<T>& row, int j0, int j1, int K, Shared& sh) {
+  const int c0 = max(row.column(j0), 0), c1 = min(row.column(j1), row.V);
   uint64_t last = ~0ull;
-  for (int i = 0; i < p.K; ++i) {  // the largest below the last one taken
+  for (int i = 0; i < K; ++i) {
     uint64_t k = 0;
-    for (int c = threadIdx.x; c < p.V; c += kThreads) {
-      const uint64_t o = order_key(to_f32(x[c]), c);
+    for (int c = c0 + (int)threadIdx.x; c < c1; c += kThreads) {
+      const uint64_t o = order_key(to_f32(row.x[c]), c);
       if (o < last && o > k) k = o;
     }
-    if (threadIdx.x == 0) best = 0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) k = max(k, __shfl_xor_sync(0xffffffffu, k, o));
     __syncthreads();
-    atomicMax(reinterpret_cast<unsigned long long*>(&best), (unsigned long long)k);
+    if (threadIdx.x == 0) sh.best = 0;
     __syncthreads();
-    last = best;
-    if (threadIdx.x == 0) {
-      const int c = (int)~(uint32_t)last;
-      p.top_index[row * p.K + i] = c;
-      p.top_logp[row * p.K + i] = (to_f32(x[c]) - m) - logf(s);
-    }
+    if ((threadIdx.x & 31) == 0) atomicMax(reinterpret_cast<unsigned long long*>(&sh.best), (unsigned long long)k);
     __syncthreads();
+    last = sh.best;  // 0: fewer than K columns here
+    if (threadIdx.x == 0) sh.top[i] = last;
+  }
+  __syncthreads();
+}
+
+// The i-th largest of the n keys at `keys` (all different but for zeros) goes to out[i], i < K.
+__device__ void rank_keys(const uint64_t* keys, int n, int K, uint64_t* out) {
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    const uint64_t k = keys[i];
+    int rank = 0;
+    for (int j = 0; j < n; ++j) rank += keys[j] > k;
+    if (rank < K && k != 0) out[rank] = k;
   }
 }
 
+// The K largest of chunks [j0, j1) into sh.top; m, at: the thread's maximum and the chunk that it was first met in.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) logprob_bwd_simple(const LogprobParams p) {
-  const int64_t row = blockIdx.x;
-  const T* x = static_cast<const T*>(p.x) + row * p.ld;
-  T* dx = static_cast<T*>(p.grad) + row * p.grad_ld;
-  const float lse = p.lse[row], h = p.entropy[row];
-  const int64_t t = p.targets[row];
-  const float g = p.g_logp ? p.g_logp[row] : 0.f, gh = p.g_entropy ? p.g_entropy[row] : 0.f;
-  float a = (t >= 0 && t < p.V) || g == 0.f ? g : NAN;
-  if (p.g_top)
-    for (int i = 0; i < p.K; ++i) a += p.g_top[row * p.K + i];
-  for (int c = threadIdx.x; c < p.V; c += kThreads) {
-    float lp = to_f32(x[c]) - lse;
-    lp = lp < -200.f ? -200.f : lp;  // p is 0 there, and -inf must not meet it; a NaN stays
-    float d = -expf(lp) * (a + gh * (lp + h));
-    if (c == t) d += g;
-    if (p.g_top)
-      for (int i = 0; i < p.K; ++i)
-        if (p.top_index[row * p.K + i] == c) d += p.g_top[row * p.K + i];
-    dx[c] = from_f32<T>(d);
+__device__ void cta_top(const Row<T>& row, int j0, int j1, int K, float m, int at, Shared& sh) {
+  constexpr int N = Row<T>::N;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) sh.holders = sh.candidates = 0;
+  for (int i = threadIdx.x; i < K; i += kThreads) sh.top[i] = 0;
+  // by chunk: the columns of a chunk share a key.  A maximum at the floor may stand for -inf.
+  const uint64_t key = at >= 0 ? order_key(m <= Floor<T>::kFloor ? -INFINITY : m, at) : 0;
+  // at least K groups of neighbouring threads: 16 of 32, 32 of 16 or 64 of 8
+  const int width = K <= 16 ? 32 : K <= 32 ? 16 : 8, groups = kThreads / width;
+  uint64_t g = key;
+  for (int o = 1; o < width; o <<= 1) g = max(g, __shfl_xor_sync(0xffffffffu, g, o));
+  if (threadIdx.x % width == 0) sh.group[threadIdx.x / width] = g;
+  __syncthreads();
+  if (threadIdx.x < groups) {
+    const uint64_t k = sh.group[threadIdx.x];
+    int rank = 0;
+    for (int j = 0; j < groups; ++j) rank += sh.group[j] > k || (sh.group[j] == k && j < (int)threadIdx.x);
+    if (rank == K - 1) sh.threshold = k;
   }
+  __syncthreads();
+  const uint64_t least = sh.threshold;
+  if (key != 0 && key >= least) sh.holder[atomicAdd(&sh.holders, 1u)] = (uint16_t)threadIdx.x;
+  __syncthreads();
+  const int holders = (int)sh.holders;
+  for (int i = warp; i < holders; i += kWarps) {
+    for (int j = j0 + sh.holder[i] + lane * kThreads; j < j1; j += 32 * kThreads) {
+      const uint4 w = row.load(j);
+      float f[N];
+      unpack(w, f, static_cast<const T*>(nullptr));
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const int c = row.column(j) + e;
+        if (c >= 0 && c < row.V && order_key(f[e], j) >= least) {
+          const uint32_t n = atomicAdd(&sh.candidates, 1u);
+          if (n < kCandidates) sh.candidate[n] = order_key(f[e], c);
+        }
+      }
+    }
+  }
+  __syncthreads();
+  const int n = (int)sh.candidates;
+  if (n <= kCandidates) {
+    rank_keys(sh.candidate, n, K, sh.top);
+    __syncthreads();
+  } else {
+    slow_top(row, j0, j1, K, sh);
+  }
+}
+
+// One cluster of CTAs per row (clusters of 1 where there are many rows).
+template <typename T, bool CLUSTER>
+__global__ void __launch_bounds__(kThreads) logprob_fwd_kernel(const LogprobParams p) {
+  constexpr int N = Row<T>::N, kUnroll = 4;
+  __shared__ Shared sh;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int parts = 1, part = 0;
+  if constexpr (CLUSTER) {
+    parts = (int)cg::this_cluster().num_blocks();
+    part = (int)cg::this_cluster().block_rank();
+  }
+  const int64_t r = CLUSTER ? blockIdx.x / parts : blockIdx.x;
+  const Row<T> row(static_cast<const T*>(p.x) + r * p.ld, p.V);
+  const int j0 = (int)((int64_t)row.chunks * part / parts), j1 = (int)((int64_t)row.chunks * (part + 1) / parts);
+
+  Sums a{-1e30f, 0.f, 0.f};  // finite, and below every maximum that the fast path takes (kLowestMax)
+  float best = -INFINITY;    // the thread's maximum, for the alternatives
+  int at = -1;
+  for (int j = j0 + (int)threadIdx.x; j < j1; j += kUnroll * kThreads) {
+    uint4 w[kUnroll];
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) {
+      const int k = j + i * kThreads;
+      w[i] = k < j1 ? row.load(k)
+                    : make_uint4(Bits<T>::kNegInf, Bits<T>::kNegInf, Bits<T>::kNegInf, Bits<T>::kNegInf);
+    }
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) {
+      float f[N];
+      const float cm = prepare(w[i], f, static_cast<const T*>(nullptr));
+      if (cm > best) {
+        best = cm;
+        at = j + i * kThreads;
+        if (cm > a.m) rescale(a, cm);
+      }
+      const float ml = a.m * kLog2e;
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const float t = fmaf(f[e], kLog2e, -ml), x = ex2(t);
+        a.s += x;
+        a.u = fmaf(x, t, a.u);
+      }
+    }
+  }
+  if (at >= j1) at = -1;
+
+  Sums all = a;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) all = shuffle_join(all, o);
+  if (lane == 0) sh.warp[warp] = all;
+  __syncthreads();
+  all = sh.warp[lane % kWarps];
+#pragma unroll
+  for (int o = kWarps / 2; o > 0; o >>= 1) all = shuffle_join(all, o);
+  if (p.K > 0) cta_top(row, j0, j1, p.K, best, at, sh);
+
+  const uint64_t* top = sh.top;
+  if constexpr (CLUSTER) {
+    cg::cluster_group cluster = cg::this_cluster();
+    if (threadIdx.x == 0) sh.cta = all;
+    cluster.sync();
+    if (part == 0) {
+      all = *cluster.map_shared_rank(&sh.cta, 0);
+      for (int q = 1; q < parts; ++q) all = join(all, *cluster.map_shared_rank(&sh.cta, q));
+      for (int i = threadIdx.x; i < parts * p.K; i += kThreads)
+        sh.merged[i] = cluster.map_shared_rank(sh.top, i / p.K)[i % p.K];
+    }
+    cluster.sync();  // the others' shared memory has been read
+    if (part != 0) return;
+    __syncthreads();
+    rank_keys(sh.merged, parts * p.K, p.K, sh.candidate);
+    __syncthreads();
+    top = sh.candidate;
+  }
+  // the same for every thread of the CTA; a NaN among the columns, or +inf, has made s NaN
+  const bool plain = all.s == all.s && all.m > Floor<T>::kLowestMax && all.m < INFINITY;
+  if (!plain) {
+    all = slow_sums(row, sh);
+    if (p.K > 0) slow_top(row, 0, row.chunks, p.K, sh);
+    top = sh.top;
+  }
+  const float ls = log2f(all.s);
+  auto logp_of = [&](float x) { return (x - all.m) - kLn2 * ls; };
+  if (threadIdx.x == 0) {
+    const int64_t t = p.targets[r];
+    p.stats[2 * r] = all.m;
+    p.stats[2 * r + 1] = ls;
+    p.logp[r] = t >= 0 && t < p.V ? logp_of(to_f32(row.x[t])) : NAN;
+    p.entropy[r] = kLn2 * (ls - all.u / all.s);
+  }
+  for (int i = threadIdx.x; i < p.K; i += kThreads) {
+    const int c = key_column(top[i]);
+    p.top_index[r * p.K + i] = c;
+    p.top_logp[r * p.K + i] = logp_of(to_f32(row.x[c]));
+  }
+}
+
+// ------------------------------------------------------------------------------------------
+// Backward: a CTA on `span` chunks of a row (of the gradient's row, whose alignment the stores need; where the
+// logits' row is aligned otherwise they are read element by element)
+// ------------------------------------------------------------------------------------------
+__device__ __forceinline__ uint4 pack(const float (&f)[4], const float*) {
+  return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+}
+__device__ __forceinline__ uint4 pack(const float (&f)[8], const __nv_bfloat16*) {
+  uint4 w;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+    (&w.x)[i] = *reinterpret_cast<const uint32_t*>(&v);
+  }
+  return w;
+}
+__device__ __forceinline__ uint4 pack(const float (&f)[8], const __half*) {
+  uint4 w;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __half2 v = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+    (&w.x)[i] = *reinterpret_cast<const uint32_t*>(&v);
+  }
+  return w;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) logprob_bwd_kernel(const LogprobParams p, int spans) {
+  constexpr int N = Row<T>::N, kUnroll = 2;
+  const int64_t r = blockIdx.x / spans;
+  const int span = (int)(blockIdx.x % spans);
+  const Row<T> in(static_cast<const T*>(p.x) + r * p.ld, p.V);
+  T* grad = static_cast<T*>(p.grad) + r * p.grad_ld;
+  const Row<T> out(grad, p.V);
+  const bool same = in.shift == out.shift;
+  const int j0 = (int)((int64_t)out.chunks * span / spans), j1 = (int)((int64_t)out.chunks * (span + 1) / spans);
+  const float m = p.stats[2 * r], ls = p.stats[2 * r + 1];
+  const int64_t t = p.targets[r];
+  const float g = p.g_logp ? p.g_logp[r] : 0.f, gh = p.g_entropy ? p.g_entropy[r] : 0.f;
+  // the weight of -p: the gradients of all log probabilities taken (NaN where the target has none), and
+  // g_entropy (log p + entropy)
+  float c0 = t >= 0 && t < p.V ? g : g == 0.f ? 0.f : NAN;
+  bool none = g == 0.f && gh == 0.f;  // a row that nothing is asked of (a masked token) gets zeros, unread
+  if (p.g_top)
+    for (int i = 0; i < p.K; ++i) {
+      const float x = p.g_top[r * p.K + i];
+      none = none && x == 0.f;
+      c0 += x;
+    }
+  if (gh != 0.f) c0 = fmaf(gh, p.entropy[r], c0);
+  const float c1 = gh * kLn2;
+  auto value = [&](float x) {
+    // log2 p; below -200 p is 0 and -inf must not meet it.  A NaN stays.
+    const float l = max_nan(fmaf(x - m, kLog2e, -ls), -200.f);
+    return none ? 0.f : -ex2(l) * fmaf(c1, l, c0);
+  };
+  for (int j = j0 + (int)threadIdx.x; j < j1; j += kUnroll * kThreads) {
+    uint4 w[kUnroll];
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) {
+      const int k = j + i * kThreads;
+      if (k >= j1) continue;
+      if (none) {
+        w[i] = make_uint4(0, 0, 0, 0);
+      } else if (same) {
+        w[i] = in.load(k);
+      } else {
+        T* e = reinterpret_cast<T*>(&w[i]);
+#pragma unroll
+        for (int q = 0; q < N; ++q) {
+          const int c = out.column(k) + q;
+          e[q] = c >= 0 && c < p.V ? in.x[c] : from_f32<T>(0.f);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) {
+      const int k = j + i * kThreads;
+      if (k >= j1) continue;
+      float f[N];
+      unpack(w[i], f, static_cast<const T*>(nullptr));
+#pragma unroll
+      for (int e = 0; e < N; ++e) f[e] = value(f[e]);
+      const uint4 q = pack(f, static_cast<const T*>(nullptr));
+      if (out.inside(k)) {
+        *reinterpret_cast<uint4*>(grad + out.column(k)) = q;
+      } else {
+        const T* e = reinterpret_cast<const T*>(&q);
+#pragma unroll
+        for (int x = 0; x < N; ++x) {
+          const int c = out.column(k) + x;
+          if (c >= 0 && c < p.V) grad[c] = e[x];
+        }
+      }
+    }
+  }
+  // the columns that a log probability was taken of, once more, with what falls on them (at most K + 1)
+  __syncthreads();
+  const int K = p.g_top ? p.K : 0;
+  for (int i = threadIdx.x; i <= K; i += kThreads) {
+    const int64_t c = i < K ? p.top_index[r * p.K + i] : t;
+    if (c < 0 || c >= p.V) continue;
+    const int j = (int)(c + out.shift) / N;
+    if (j < j0 || j >= j1) continue;
+    if (i == K && p.g_logp == nullptr) continue;
+    // the alternatives differ from one another; one of them may be the target, which then leaves it to it
+    float d = value(to_f32(in.x[c]));
+    if (i < K) {
+      d += p.g_top[r * p.K + i];
+      if (c == t) d += g;
+    } else {
+      bool taken = false;
+      for (int q = 0; q < K; ++q) taken = taken || p.top_index[r * p.K + q] == c;
+      if (taken) continue;
+      d += g;
+    }
+    grad[c] = from_f32<T>(d);
+  }
+}
+
+int sm_count() {
+  static int count[64];  // per device; 0: not asked yet (two threads that ask write the same)
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  if (count[dev] == 0) {
+    int n = 0;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 1) return 148;
+    count[dev] = n;
+  }
+  return count[dev];
+}
+
+template <typename T>
+cudaError_t launch_fwd(const LogprobParams& p, cudaStream_t s) {
+  // few rows: several CTAs on each, of one chunk per thread at least, up to four CTAs per SM
+  const int chunks = p.V / (16 / (int)sizeof(T)) + 1;
+  int parts = 1;
+  while (parts < kMaxCluster && p.rows * parts * 2 <= 4 * sm_count() && chunks >= 2 * parts * kThreads) parts *= 2;
+  if (parts == 1) {
+    logprob_fwd_kernel<T, false><<<(unsigned)p.rows, kThreads, 0, s>>>(p);
+    return cudaGetLastError();
+  }
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(p.rows * parts));
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = s;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim.x = (unsigned)parts;
+  at.val.clusterDim.y = at.val.clusterDim.z = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, logprob_fwd_kernel<T, true>, p);
+}
+
+template <typename T>
+cudaError_t launch_bwd(const LogprobParams& p, cudaStream_t s) {
+  // few rows: several CTAs on each, of one chunk per thread at least
+  const int chunks = p.V / (16 / (int)sizeof(T)) + 1;
+  int spans = 1;
+  while (p.rows * spans * 2 <= 4 * sm_count() && chunks >= 2 * spans * kThreads) spans *= 2;
+  logprob_bwd_kernel<T><<<(unsigned)(p.rows * spans), kThreads, 0, s>>>(p, spans);
+  return cudaGetLastError();
 }
 
 int logprob(const fb_logprob_args* a, void* stream, bool backward) {
   if (a == nullptr) return FB_ERR_ARG;
-  if (a->rows < 0 || a->rows > 0x7FFFFFFF || a->vocab < 1 || a->ld < a->vocab || a->top_k < 0 ||
-      a->top_k > FB_MAX_TOP_K || a->top_k > a->vocab)
+  if (a->rows < 0 || a->rows > 0x7FFFFFFF || a->vocab < 1 || a->vocab > 0x7FFFFF00 || a->ld < a->vocab ||
+      a->top_k < 0 || a->top_k > FB_MAX_TOP_K || a->top_k > a->vocab)
     return FB_ERR_SHAPE;
   if (a->dtype != FB_F32 && a->dtype != FB_F16 && a->dtype != FB_BF16) return FB_ERR_DTYPE;
   if (backward && a->grad_ld < a->vocab) return FB_ERR_SHAPE;
@@ -142,25 +590,19 @@ int logprob(const fb_logprob_args* a, void* stream, bool backward) {
     set_last_launch_count(0);
     return FB_OK;
   }
-  if (a->logits == nullptr || a->targets == nullptr || a->lse == nullptr || a->entropy == nullptr) return FB_ERR_ARG;
+  if (a->logits == nullptr || a->targets == nullptr || a->stats == nullptr || a->entropy == nullptr) return FB_ERR_ARG;
   if (!backward && a->logp == nullptr) return FB_ERR_ARG;
   if (!backward && a->top_k > 0 && (a->top_logp == nullptr || a->top_index == nullptr)) return FB_ERR_ARG;
   if (backward && a->grad == nullptr) return FB_ERR_ARG;
   if (backward && a->top_k > 0 && a->g_top != nullptr && a->top_index == nullptr) return FB_ERR_ARG;
-  LogprobParams p{a->rows, a->vocab, a->top_k, a->logits, a->ld, a->targets, a->logp, a->entropy, a->lse, a->top_logp,
-                  a->top_index, a->g_logp, a->g_entropy, a->top_k > 0 ? a->g_top : nullptr, a->grad, a->grad_ld};
+  const LogprobParams p{a->rows, a->vocab, a->top_k, a->logits, a->ld, a->targets, a->logp, a->entropy, a->stats,
+                        a->top_logp, a->top_index, a->g_logp, a->g_entropy, a->top_k > 0 ? a->g_top : nullptr, a->grad,
+                        a->grad_ld};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const unsigned n = (unsigned)a->rows;
-  if (backward) {
-    if (a->dtype == FB_F32) logprob_bwd_simple<float><<<n, kThreads, 0, s>>>(p);
-    else if (a->dtype == FB_F16) logprob_bwd_simple<__half><<<n, kThreads, 0, s>>>(p);
-    else logprob_bwd_simple<__nv_bfloat16><<<n, kThreads, 0, s>>>(p);
-  } else {
-    if (a->dtype == FB_F32) logprob_fwd_simple<float><<<n, kThreads, 0, s>>>(p);
-    else if (a->dtype == FB_F16) logprob_fwd_simple<__half><<<n, kThreads, 0, s>>>(p);
-    else logprob_fwd_simple<__nv_bfloat16><<<n, kThreads, 0, s>>>(p);
-  }
-  const cudaError_t e = cudaGetLastError();
+  cudaError_t e;
+  if (a->dtype == FB_F32) e = backward ? launch_bwd<float>(p, s) : launch_fwd<float>(p, s);
+  else if (a->dtype == FB_F16) e = backward ? launch_bwd<__half>(p, s) : launch_fwd<__half>(p, s);
+  else e = backward ? launch_bwd<__nv_bfloat16>(p, s) : launch_fwd<__nv_bfloat16>(p, s);
   if (e != cudaSuccess) {
     record_cuda_error(e);
     return FB_ERR_LAUNCH;

@@ -36,22 +36,23 @@ def _args(logits: torch.Tensor, targets: torch.Tensor, top_k: int) -> _lib.FbLog
 
 def _forward(logits: torch.Tensor, targets: torch.Tensor, top_k: int) -> tuple[torch.Tensor, ...]:
     n, device = logits.shape[0], logits.device
-    logp, entropy, lse = torch.empty((3, n), dtype=torch.float32, device=device).unbind(0)
+    logp, entropy = torch.empty((2, n), dtype=torch.float32, device=device).unbind(0)
+    stats = torch.empty((n, 2), dtype=torch.float32, device=device)
     top_logp = torch.empty((n, top_k), dtype=torch.float32, device=device)
     top_index = torch.empty((n, top_k), dtype=torch.int64, device=device)
     a = _args(logits, targets, top_k)
-    a.logp, a.entropy, a.lse = logp.data_ptr(), entropy.data_ptr(), lse.data_ptr()
+    a.logp, a.entropy, a.stats = logp.data_ptr(), entropy.data_ptr(), stats.data_ptr()
     a.top_logp, a.top_index = top_logp.data_ptr(), top_index.data_ptr()
     with torch.cuda.device(device):
         _lib.check(_lib.load().fb_logprob_fwd(ctypes.byref(a), _stream_handle(device)), "token log probabilities")
-    return logp, entropy, lse, top_logp, top_index
+    return logp, entropy, stats, top_logp, top_index
 
 
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits: torch.Tensor, targets: torch.Tensor, top_k: int):
-        logp, entropy, lse, top_logp, top_index = _forward(logits, targets, top_k)
-        ctx.save_for_backward(logits, targets, entropy, lse, top_index)
+        logp, entropy, stats, top_logp, top_index = _forward(logits, targets, top_k)
+        ctx.save_for_backward(logits, targets, entropy, stats, top_index)
         ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(top_index)
         return logp, entropy, top_logp, top_index
@@ -59,11 +60,11 @@ class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def backward(ctx, g_logp: Optional[torch.Tensor], g_entropy: Optional[torch.Tensor],
                  g_top: Optional[torch.Tensor], _g_index):
-        logits, targets, entropy, lse, top_index = ctx.saved_tensors
+        logits, targets, entropy, stats, top_index = ctx.saved_tensors
         grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         top_k = top_index.shape[1]
         a = _args(logits, targets, top_k)
-        a.entropy, a.lse, a.top_index = entropy.data_ptr(), lse.data_ptr(), top_index.data_ptr()
+        a.entropy, a.stats, a.top_index = entropy.data_ptr(), stats.data_ptr(), top_index.data_ptr()
         given = [g if g is None else g.to(torch.float32).contiguous() for g in (g_logp, g_entropy, g_top)]
         a.g_logp, a.g_entropy, a.g_top = (None if g is None else g.data_ptr() for g in given)
         a.grad, a.grad_ld = grad.data_ptr(), max(grad.stride(0), grad.shape[1])
@@ -81,7 +82,8 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0) 
     ``top_k`` (at most 64, and V) largest logits in falling order, equal ones by lowest index, a NaN above
     everything; ``-inf`` columns have no probability.  A target outside ``[0, V)`` gives a NaN logp, and a row
     of nothing but ``-inf``, or with a NaN or ``+inf``, is NaN.  ``logp``, ``entropy`` and ``top_logp`` are
-    differentiable in the logits (the gradient has their dtype).
+    differentiable in the logits (the gradient has their dtype; a row whose incoming gradients are all 0 gets 0,
+    whatever it holds).
     """
     if not (logits.is_cuda and targets.is_cuda):
         raise RuntimeError("token_logprobs (B200): CUDA tensors required; there is no CPU path")

@@ -105,7 +105,7 @@ def test_paged_write_validation(kw, code):
 def test_logprob_validation(kw, code):
     a = _lib.FbLogprobArgs()
     a.rows, a.vocab, a.dtype, a.top_k, a.ld, a.grad_ld = 3, 100, _lib.FB_F32, 4, 100, 100
-    for n in ("logits", "targets", "logp", "entropy", "lse", "top_logp", "top_index"):
+    for n in ("logits", "targets", "logp", "entropy", "stats", "top_logp", "top_index"):
         setattr(a, n, FAKE)
     for k, v in kw.items():
         setattr(a, k, v)
