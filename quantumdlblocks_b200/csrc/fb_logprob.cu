@@ -78,13 +78,21 @@ template <> struct Bits<__nv_bfloat16> {
 template <typename T> struct Row {
   static constexpr int N = 16 / sizeof(T);
   const T* x;
-  int V, shift, chunks;
+  int V, shift, chunks, full0, fulls;  // chunks [full0, full0 + fulls) lie inside the row
   __device__ Row(const T* row, int vocab) : x(row), V(vocab) {
     shift = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
     chunks = (V + shift + N - 1) / N;
+    full0 = shift > 0;
+    fulls = max((V + shift) / N - full0, 0);
   }
   __device__ int column(int j) const { return j * N - shift; }
-  __device__ bool inside(int j) const { return column(j) >= 0 && column(j) + N <= V; }
+  __device__ bool inside(int j) const { return (uint32_t)(j - full0) < (uint32_t)fulls; }
+  // the part-th of `parts` even parts: chunks [j0, j1)
+  __device__ void part_of(int part, int parts, int& j0, int& j1) const {
+    const int each = (chunks + parts - 1) / parts;
+    j0 = min(part * each, chunks);
+    j1 = min(j0 + each, chunks);
+  }
   __device__ uint4 load(int j) const {
     const int c = column(j);
     if (inside(j)) return __ldg(reinterpret_cast<const uint4*>(x + c));
@@ -319,7 +327,7 @@ __device__ void cta_top(const Row<T>& row, int j0, int j1, int K, float m, int a
 
 // One cluster of CTAs per row (clusters of 1 where there are many rows).
 template <typename T, bool CLUSTER>
-__global__ void __launch_bounds__(kThreads) logprob_fwd_kernel(const LogprobParams p) {
+__global__ void __launch_bounds__(kThreads, 3) logprob_fwd_kernel(const LogprobParams p) {
   constexpr int N = Row<T>::N, kUnroll = 4;
   __shared__ Shared sh;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -330,7 +338,8 @@ __global__ void __launch_bounds__(kThreads) logprob_fwd_kernel(const LogprobPara
   }
   const int64_t r = CLUSTER ? blockIdx.x / parts : blockIdx.x;
   const Row<T> row(static_cast<const T*>(p.x) + r * p.ld, p.V);
-  const int j0 = (int)((int64_t)row.chunks * part / parts), j1 = (int)((int64_t)row.chunks * (part + 1) / parts);
+  int j0, j1;
+  row.part_of(part, parts, j0, j1);
 
   Sums a{-1e30f, 0.f, 0.f};  // finite, and below every maximum that the fast path takes (kLowestMax)
   float best = -INFINITY;    // the thread's maximum, for the alternatives
@@ -340,18 +349,20 @@ __global__ void __launch_bounds__(kThreads) logprob_fwd_kernel(const LogprobPara
 #pragma unroll
     for (int i = 0; i < kUnroll; ++i) {
       const int k = j + i * kThreads;
-      w[i] = k < j1 ? row.load(k)
-                    : make_uint4(Bits<T>::kNegInf, Bits<T>::kNegInf, Bits<T>::kNegInf, Bits<T>::kNegInf);
+      if (k < j1) w[i] = row.load(k);
     }
 #pragma unroll
     for (int i = 0; i < kUnroll; ++i) {
+      if (j + i * kThreads >= j1) break;
       float f[N];
       const float cm = prepare(w[i], f, static_cast<const T*>(nullptr));
       if (cm > best) {
         best = cm;
         at = j + i * kThreads;
-        if (cm > a.m) rescale(a, cm);
       }
+      // sums to an older maximum are as good while 2^t stays small: a warp in which some lane has a new maximum,
+      // which is most of the time, does not stop for it
+      if (cm > a.m + 10.f) rescale(a, cm);
       const float ml = a.m * kLog2e;
 #pragma unroll
       for (int e = 0; e < N; ++e) {
@@ -361,7 +372,7 @@ __global__ void __launch_bounds__(kThreads) logprob_fwd_kernel(const LogprobPara
       }
     }
   }
-  if (at >= j1) at = -1;
+  if (best > a.m) rescale(a, best);
 
   Sums all = a;
 #pragma unroll
@@ -441,16 +452,16 @@ __device__ __forceinline__ uint4 pack(const float (&f)[8], const __half*) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) logprob_bwd_kernel(const LogprobParams p, int spans) {
-  constexpr int N = Row<T>::N, kUnroll = 2;
-  const int64_t r = blockIdx.x / spans;
-  const int span = (int)(blockIdx.x % spans);
+__global__ void __launch_bounds__(kThreads, 3) logprob_bwd_kernel(const LogprobParams p) {
+  constexpr int N = Row<T>::N, kUnroll = 4;
+  const int64_t r = blockIdx.x;
   const Row<T> in(static_cast<const T*>(p.x) + r * p.ld, p.V);
   T* grad = static_cast<T*>(p.grad) + r * p.grad_ld;
   const Row<T> out(grad, p.V);
   const bool same = in.shift == out.shift;
-  const int j0 = (int)((int64_t)out.chunks * span / spans), j1 = (int)((int64_t)out.chunks * (span + 1) / spans);
-  const float m = p.stats[2 * r], ls = p.stats[2 * r + 1];
+  int j0, j1;
+  out.part_of(blockIdx.y, gridDim.y, j0, j1);
+  float m = p.stats[2 * r], ls = p.stats[2 * r + 1];
   const int64_t t = p.targets[r];
   const float g = p.g_logp ? p.g_logp[r] : 0.f, gh = p.g_entropy ? p.g_entropy[r] : 0.f;
   // the weight of -p: the gradients of all log probabilities taken (NaN where the target has none), and
@@ -464,11 +475,12 @@ __global__ void __launch_bounds__(kThreads) logprob_bwd_kernel(const LogprobPara
       c0 += x;
     }
   if (gh != 0.f) c0 = fmaf(gh, p.entropy[r], c0);
+  if (none) m = ls = 0.f;  // which may be NaN
   const float c1 = gh * kLn2;
   auto value = [&](float x) {
     // log2 p; below -200 p is 0 and -inf must not meet it.  A NaN stays.
     const float l = max_nan(fmaf(x - m, kLog2e, -ls), -200.f);
-    return none ? 0.f : -ex2(l) * fmaf(c1, l, c0);
+    return -ex2(l) * fmaf(c1, l, c0);
   };
   for (int j = j0 + (int)threadIdx.x; j < j1; j += kUnroll * kThreads) {
     uint4 w[kUnroll];
@@ -492,7 +504,7 @@ __global__ void __launch_bounds__(kThreads) logprob_bwd_kernel(const LogprobPara
 #pragma unroll
     for (int i = 0; i < kUnroll; ++i) {
       const int k = j + i * kThreads;
-      if (k >= j1) continue;
+      if (k >= j1) break;
       float f[N];
       unpack(w[i], f, static_cast<const T*>(nullptr));
 #pragma unroll
@@ -511,6 +523,7 @@ __global__ void __launch_bounds__(kThreads) logprob_bwd_kernel(const LogprobPara
     }
   }
   // the columns that a log probability was taken of, once more, with what falls on them (at most K + 1)
+  if (none) return;
   __syncthreads();
   const int K = p.g_top ? p.K : 0;
   for (int i = threadIdx.x; i <= K; i += kThreads) {
@@ -575,7 +588,7 @@ cudaError_t launch_bwd(const LogprobParams& p, cudaStream_t s) {
   const int chunks = p.V / (16 / (int)sizeof(T)) + 1;
   int spans = 1;
   while (p.rows * spans * 2 <= 4 * sm_count() && chunks >= 2 * spans * kThreads) spans *= 2;
-  logprob_bwd_kernel<T><<<(unsigned)(p.rows * spans), kThreads, 0, s>>>(p, spans);
+  logprob_bwd_kernel<T><<<dim3((unsigned)p.rows, spans), kThreads, 0, s>>>(p);
   return cudaGetLastError();
 }
 
