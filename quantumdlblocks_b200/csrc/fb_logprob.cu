@@ -19,14 +19,18 @@
 #include <cmath>
 
 #include "fb_common.cuh"
+#include "fb_sm100.cuh"
 
 namespace cg = cooperative_groups;
 
 namespace fb {
 namespace {
 
-constexpr int kThreads = 512;
-constexpr int kWarps = kThreads / 32;
+using namespace sm100;  // packed fp32 pairs
+
+// Threads of a CTA: kMany where there are rows enough to fill the GPU with CTAs that small (the fixed work of
+// a thread is then spread over twice the columns), else kFew.
+constexpr int kFew = 512, kMany = 256;
 constexpr int kCandidates = 1024;
 constexpr int kMaxCluster = 8;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
@@ -94,8 +98,8 @@ template <typename T> struct Row {
     j1 = min(j0 + each, chunks);
   }
   __device__ uint4 load(int j) const {
+    if (inside(j)) return __ldg(reinterpret_cast<const uint4*>(x - shift) + j);
     const int c = column(j);
-    if (inside(j)) return __ldg(reinterpret_cast<const uint4*>(x + c));
     uint4 w = make_uint4(Bits<T>::kNegInf, Bits<T>::kNegInf, Bits<T>::kNegInf, Bits<T>::kNegInf);
     T* e = reinterpret_cast<T*>(&w);
 #pragma unroll
@@ -179,9 +183,19 @@ __device__ __forceinline__ Sums join(Sums a, Sums b) {
   rescale(b, m);
   return {m, a.s + b.s, a.u + b.u};
 }
-__device__ __forceinline__ Sums shuffle_join(Sums a, int o) {
-  return join(a, {__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o),
-                  __shfl_xor_sync(0xffffffffu, a.u, o)});
+// over the lanes whose numbers differ in the bits below WIDTH
+template <int WIDTH>
+__device__ __forceinline__ Sums join_lanes(Sums a) {
+  float m = a.m;
+#pragma unroll
+  for (int o = 1; o < WIDTH; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  rescale(a, m);
+#pragma unroll
+  for (int o = 1; o < WIDTH; o <<= 1) {
+    a.s += __shfl_xor_sync(0xffffffffu, a.s, o);
+    a.u += __shfl_xor_sync(0xffffffffu, a.u, o);
+  }
+  return a;
 }
 
 // 32 bits that order as the float does, NaN above everything, -0 and 0 alike; and back
@@ -194,13 +208,13 @@ __device__ __forceinline__ uint32_t ordered(float x) {
 __device__ __forceinline__ uint64_t order_key(float x, int c) { return (uint64_t)ordered(x) << 32 | (uint32_t)~c; }
 __device__ __forceinline__ int key_column(uint64_t k) { return (int)~(uint32_t)k; }
 
-struct Shared {
-  Sums warp[kWarps];
+template <int THREADS> struct Shared {
+  Sums warp[THREADS / 32];
   Sums cta;                        // of the CTA's part of the row
-  uint64_t group[64];
+  uint64_t group[THREADS < 64 ? THREADS : 64];
   uint64_t threshold;
   uint32_t holders, candidates;
-  uint16_t holder[kThreads];
+  uint16_t holder[THREADS];
   uint64_t candidate[kCandidates];
   uint64_t top[64];                // the CTA's alternatives, in order
   uint64_t merged[kMaxCluster * 64];
@@ -209,11 +223,12 @@ struct Shared {
 
 // ---- the row by itself, column by column: what the fast path cannot take (NaN, +inf, nothing above the
 // floor), and the alternatives where too many columns are equal
-template <typename T>
-__device__ Sums slow_sums(const Row<T>& row, Shared& sh) {
+template <typename T, int THREADS>
+__device__ Sums slow_sums(const Row<T>& row, Shared<THREADS>& sh) {
+  constexpr int kWarps = THREADS / 32;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   float m = -INFINITY;
-  for (int c = threadIdx.x; c < row.V; c += kThreads) m = max_nan(m, to_f32(row.x[c]));
+  for (int c = threadIdx.x; c < row.V; c += THREADS) m = max_nan(m, to_f32(row.x[c]));
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
   __syncthreads();
@@ -221,7 +236,7 @@ __device__ Sums slow_sums(const Row<T>& row, Shared& sh) {
   __syncthreads();
   for (int w = 0; w < kWarps; ++w) m = max_nan(m, sh.warp[w].m);
   float s = 0.f, u = 0.f;
-  for (int c = threadIdx.x; c < row.V; c += kThreads) {
+  for (int c = threadIdx.x; c < row.V; c += THREADS) {
     const float t = (to_f32(row.x[c]) - m) * kLog2e, e = ex2(t);  // NaN where m is not finite
     s += e;
     u += e * (t < -200.f ? -200.f : t);
@@ -241,13 +256,13 @@ __device__ Sums slow_sums(const Row<T>& row, Shared& sh) {
 }
 
 // the K largest of chunks [j0, j1) into sh.top, one at a time: the largest below the last one taken
-template <typename T>
-__device__ void slow_top(const Row<T>& row, int j0, int j1, int K, Shared& sh) {
+template <typename T, int THREADS>
+__device__ void slow_top(const Row<T>& row, int j0, int j1, int K, Shared<THREADS>& sh) {
   const int c0 = max(row.column(j0), 0), c1 = min(row.column(j1), row.V);
   uint64_t last = ~0ull;
   for (int i = 0; i < K; ++i) {
     uint64_t k = 0;
-    for (int c = c0 + (int)threadIdx.x; c < c1; c += kThreads) {
+    for (int c = c0 + (int)threadIdx.x; c < c1; c += THREADS) {
       const uint64_t o = order_key(to_f32(row.x[c]), c);
       if (o < last && o > k) k = o;
     }
@@ -265,8 +280,9 @@ __device__ void slow_top(const Row<T>& row, int j0, int j1, int K, Shared& sh) {
 }
 
 // The i-th largest of the n keys at `keys` (all different but for zeros) goes to out[i], i < K.
+template <int THREADS>
 __device__ void rank_keys(const uint64_t* keys, int n, int K, uint64_t* out) {
-  for (int i = threadIdx.x; i < n; i += kThreads) {
+  for (int i = threadIdx.x; i < n; i += THREADS) {
     const uint64_t k = keys[i];
     int rank = 0;
     for (int j = 0; j < n; ++j) rank += keys[j] > k;
@@ -275,16 +291,18 @@ __device__ void rank_keys(const uint64_t* keys, int n, int K, uint64_t* out) {
 }
 
 // The K largest of chunks [j0, j1) into sh.top; m, at: the thread's maximum and the chunk that it was first met in.
-template <typename T>
-__device__ void cta_top(const Row<T>& row, int j0, int j1, int K, float m, int at, Shared& sh) {
-  constexpr int N = Row<T>::N;
+template <typename T, int THREADS>
+__device__ void cta_top(const Row<T>& row, int j0, int j1, int K, float m, int at, Shared<THREADS>& sh) {
+  constexpr int N = Row<T>::N, kWarps = THREADS / 32;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) sh.holders = sh.candidates = 0;
-  for (int i = threadIdx.x; i < K; i += kThreads) sh.top[i] = 0;
+  for (int i = threadIdx.x; i < K; i += THREADS) sh.top[i] = 0;
   // by chunk: the columns of a chunk share a key.  A maximum at the floor may stand for -inf.
   const uint64_t key = at >= 0 ? order_key(m <= Floor<T>::kFloor ? -INFINITY : m, at) : 0;
-  // at least K groups of neighbouring threads: 16 of 32, 32 of 16 or 64 of 8
-  const int width = K <= 16 ? 32 : K <= 32 ? 16 : 8, groups = kThreads / width;
+  // at least K groups of neighbouring threads: a warp each or less
+  int width = 32;
+  while (THREADS / width < K) width /= 2;
+  const int groups = THREADS / width;
   uint64_t g = key;
   for (int o = 1; o < width; o <<= 1) g = max(g, __shfl_xor_sync(0xffffffffu, g, o));
   if (threadIdx.x % width == 0) sh.group[threadIdx.x / width] = g;
@@ -301,7 +319,7 @@ __device__ void cta_top(const Row<T>& row, int j0, int j1, int K, float m, int a
   __syncthreads();
   const int holders = (int)sh.holders;
   for (int i = warp; i < holders; i += kWarps) {
-    for (int j = j0 + sh.holder[i] + lane * kThreads; j < j1; j += 32 * kThreads) {
+    for (int j = j0 + sh.holder[i] + lane * THREADS; j < j1; j += 32 * THREADS) {
       const uint4 w = row.load(j);
       float f[N];
       unpack(w, f, static_cast<const T*>(nullptr));
@@ -318,7 +336,7 @@ __device__ void cta_top(const Row<T>& row, int j0, int j1, int K, float m, int a
   __syncthreads();
   const int n = (int)sh.candidates;
   if (n <= kCandidates) {
-    rank_keys(sh.candidate, n, K, sh.top);
+    rank_keys<THREADS>(sh.candidate, n, K, sh.top);
     __syncthreads();
   } else {
     slow_top(row, j0, j1, K, sh);
@@ -326,10 +344,10 @@ __device__ void cta_top(const Row<T>& row, int j0, int j1, int K, float m, int a
 }
 
 // One cluster of CTAs per row (clusters of 1 where there are many rows).
-template <typename T, bool CLUSTER>
-__global__ void __launch_bounds__(kThreads, 3) logprob_fwd_kernel(const LogprobParams p) {
-  constexpr int N = Row<T>::N, kUnroll = 4;
-  __shared__ Shared sh;
+template <typename T, int THREADS, bool CLUSTER>
+__global__ void __launch_bounds__(THREADS, 1280 / THREADS) logprob_fwd_kernel(const LogprobParams p) {
+  constexpr int N = Row<T>::N, kUnroll = 4, kWarps = THREADS / 32;
+  __shared__ Shared<THREADS> sh;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int parts = 1, part = 0;
   if constexpr (CLUSTER) {
@@ -342,46 +360,52 @@ __global__ void __launch_bounds__(kThreads, 3) logprob_fwd_kernel(const LogprobP
   row.part_of(part, parts, j0, j1);
 
   Sums a{-1e30f, 0.f, 0.f};  // finite, and below every maximum that the fast path takes (kLowestMax)
+  f32x2 s2 = f2_make(0.f, 0.f), u2 = s2;  // its sums, of even and of odd columns
   float best = -INFINITY;    // the thread's maximum, for the alternatives
   int at = -1;
-  for (int j = j0 + (int)threadIdx.x; j < j1; j += kUnroll * kThreads) {
+  for (int j = j0 + (int)threadIdx.x; j < j1; j += kUnroll * THREADS) {
     uint4 w[kUnroll];
 #pragma unroll
     for (int i = 0; i < kUnroll; ++i) {
-      const int k = j + i * kThreads;
+      const int k = j + i * THREADS;
       if (k < j1) w[i] = row.load(k);
     }
 #pragma unroll
     for (int i = 0; i < kUnroll; ++i) {
-      if (j + i * kThreads >= j1) break;
+      if (j + i * THREADS >= j1) break;
       float f[N];
       const float cm = prepare(w[i], f, static_cast<const T*>(nullptr));
       if (cm > best) {
         best = cm;
-        at = j + i * kThreads;
+        at = j + i * THREADS;
       }
       // sums to an older maximum are as good while 2^t stays small: a warp in which some lane has a new maximum,
       // which is most of the time, does not stop for it
-      if (cm > a.m + 10.f) rescale(a, cm);
+      if (cm > a.m + 10.f) {
+        Sums b{a.m, f2_hi(s2), f2_hi(u2)};
+        a.s = f2_lo(s2), a.u = f2_lo(u2);
+        rescale(a, cm);
+        rescale(b, cm);
+        s2 = f2_make(a.s, b.s), u2 = f2_make(a.u, b.u);
+      }
       const float ml = a.m * kLog2e;
 #pragma unroll
-      for (int e = 0; e < N; ++e) {
-        const float t = fmaf(f[e], kLog2e, -ml), x = ex2(t);
-        a.s += x;
-        a.u = fmaf(x, t, a.u);
+      for (int e = 0; e < N; e += 2) {
+        const f32x2 t = f2_fma(f2_make(f[e], f[e + 1]), f2_make(kLog2e, kLog2e), f2_make(-ml, -ml));
+        const f32x2 x = f2_make(ex2(f2_lo(t)), ex2(f2_hi(t)));
+        s2 = f2_add(s2, x);
+        u2 = f2_fma(x, t, u2);
       }
     }
   }
+  a.s = f2_lo(s2) + f2_hi(s2);
+  a.u = f2_lo(u2) + f2_hi(u2);
   if (best > a.m) rescale(a, best);
 
-  Sums all = a;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) all = shuffle_join(all, o);
+  Sums all = join_lanes<32>(a);
   if (lane == 0) sh.warp[warp] = all;
   __syncthreads();
-  all = sh.warp[lane % kWarps];
-#pragma unroll
-  for (int o = kWarps / 2; o > 0; o >>= 1) all = shuffle_join(all, o);
+  all = join_lanes<kWarps>(sh.warp[lane % kWarps]);
   if (p.K > 0) cta_top(row, j0, j1, p.K, best, at, sh);
 
   const uint64_t* top = sh.top;
@@ -392,13 +416,13 @@ __global__ void __launch_bounds__(kThreads, 3) logprob_fwd_kernel(const LogprobP
     if (part == 0) {
       all = *cluster.map_shared_rank(&sh.cta, 0);
       for (int q = 1; q < parts; ++q) all = join(all, *cluster.map_shared_rank(&sh.cta, q));
-      for (int i = threadIdx.x; i < parts * p.K; i += kThreads)
+      for (int i = threadIdx.x; i < parts * p.K; i += THREADS)
         sh.merged[i] = cluster.map_shared_rank(sh.top, i / p.K)[i % p.K];
     }
     cluster.sync();  // the others' shared memory has been read
     if (part != 0) return;
     __syncthreads();
-    rank_keys(sh.merged, parts * p.K, p.K, sh.candidate);
+    rank_keys<THREADS>(sh.merged, parts * p.K, p.K, sh.candidate);
     __syncthreads();
     top = sh.candidate;
   }
@@ -409,6 +433,7 @@ __global__ void __launch_bounds__(kThreads, 3) logprob_fwd_kernel(const LogprobP
     if (p.K > 0) slow_top(row, 0, row.chunks, p.K, sh);
     top = sh.top;
   }
+  if (threadIdx.x > p.K) return;
   const float ls = log2f(all.s);
   auto logp_of = [&](float x) { return (x - all.m) - kLn2 * ls; };
   if (threadIdx.x == 0) {
@@ -418,7 +443,7 @@ __global__ void __launch_bounds__(kThreads, 3) logprob_fwd_kernel(const LogprobP
     p.logp[r] = t >= 0 && t < p.V ? logp_of(to_f32(row.x[t])) : NAN;
     p.entropy[r] = kLn2 * (ls - all.u / all.s);
   }
-  for (int i = threadIdx.x; i < p.K; i += kThreads) {
+  for (int i = threadIdx.x; i < p.K; i += THREADS) {
     const int c = key_column(top[i]);
     p.top_index[r * p.K + i] = c;
     p.top_logp[r * p.K + i] = logp_of(to_f32(row.x[c]));
@@ -451,8 +476,8 @@ __device__ __forceinline__ uint4 pack(const float (&f)[8], const __half*) {
   return w;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads, 3) logprob_bwd_kernel(const LogprobParams p) {
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1280 / THREADS) logprob_bwd_kernel(const LogprobParams p) {
   constexpr int N = Row<T>::N, kUnroll = 4;
   const int64_t r = blockIdx.x;
   const Row<T> in(static_cast<const T*>(p.x) + r * p.ld, p.V);
@@ -482,11 +507,11 @@ __global__ void __launch_bounds__(kThreads, 3) logprob_bwd_kernel(const LogprobP
     const float l = max_nan(fmaf(x - m, kLog2e, -ls), -200.f);
     return -ex2(l) * fmaf(c1, l, c0);
   };
-  for (int j = j0 + (int)threadIdx.x; j < j1; j += kUnroll * kThreads) {
+  for (int j = j0 + (int)threadIdx.x; j < j1; j += kUnroll * THREADS) {
     uint4 w[kUnroll];
 #pragma unroll
     for (int i = 0; i < kUnroll; ++i) {
-      const int k = j + i * kThreads;
+      const int k = j + i * THREADS;
       if (k >= j1) continue;
       if (none) {
         w[i] = make_uint4(0, 0, 0, 0);
@@ -503,12 +528,19 @@ __global__ void __launch_bounds__(kThreads, 3) logprob_bwd_kernel(const LogprobP
     }
 #pragma unroll
     for (int i = 0; i < kUnroll; ++i) {
-      const int k = j + i * kThreads;
+      const int k = j + i * THREADS;
       if (k >= j1) break;
       float f[N];
       unpack(w[i], f, static_cast<const T*>(nullptr));
 #pragma unroll
-      for (int e = 0; e < N; ++e) f[e] = value(f[e]);
+      for (int e = 0; e < N; e += 2) {
+        const f32x2 d = f2_add(f2_make(f[e], f[e + 1]), f2_make(-m, -m));
+        const f32x2 l = f2_fma(d, f2_make(kLog2e, kLog2e), f2_make(-ls, -ls));
+        const float l0 = max_nan(f2_lo(l), -200.f), l1 = max_nan(f2_hi(l), -200.f);
+        const f32x2 g2 = f2_fma(f2_make(-c1, -c1), f2_make(l0, l1), f2_make(-c0, -c0));
+        const f32x2 q = f2_mul(f2_make(ex2(l0), ex2(l1)), g2);
+        f[e] = f2_lo(q), f[e + 1] = f2_hi(q);
+      }
       const uint4 q = pack(f, static_cast<const T*>(nullptr));
       if (out.inside(k)) {
         *reinterpret_cast<uint4*>(grad + out.column(k)) = q;
@@ -526,7 +558,7 @@ __global__ void __launch_bounds__(kThreads, 3) logprob_bwd_kernel(const LogprobP
   if (none) return;
   __syncthreads();
   const int K = p.g_top ? p.K : 0;
-  for (int i = threadIdx.x; i <= K; i += kThreads) {
+  for (int i = threadIdx.x; i <= K; i += THREADS) {
     const int64_t c = i < K ? p.top_index[r * p.K + i] : t;
     if (c < 0 || c >= p.V) continue;
     const int j = (int)(c + out.shift) / N;
@@ -559,19 +591,29 @@ int sm_count() {
   return count[dev];
 }
 
+// A row on one CTA while there are CTAs for every SM several times over; few rows on several CTAs each, of
+// one chunk per thread at least.
+int parts_of(const LogprobParams& p, int chunk, int most) {
+  int parts = 1;
+  const int64_t chunks = p.V / chunk + 1;
+  while (parts < most && p.rows * parts * 2 <= 4 * sm_count() && chunks >= 2 * parts * kFew) parts *= 2;
+  return parts;
+}
+
+bool many(const LogprobParams& p) { return p.rows >= 8 * sm_count(); }
+
 template <typename T>
 cudaError_t launch_fwd(const LogprobParams& p, cudaStream_t s) {
-  // few rows: several CTAs on each, of one chunk per thread at least, up to four CTAs per SM
-  const int chunks = p.V / (16 / (int)sizeof(T)) + 1;
-  int parts = 1;
-  while (parts < kMaxCluster && p.rows * parts * 2 <= 4 * sm_count() && chunks >= 2 * parts * kThreads) parts *= 2;
+  const unsigned n = (unsigned)p.rows;
+  const int parts = parts_of(p, 16 / sizeof(T), kMaxCluster);
   if (parts == 1) {
-    logprob_fwd_kernel<T, false><<<(unsigned)p.rows, kThreads, 0, s>>>(p);
+    if (many(p)) logprob_fwd_kernel<T, kMany, false><<<n, kMany, 0, s>>>(p);
+    else logprob_fwd_kernel<T, kFew, false><<<n, kFew, 0, s>>>(p);
     return cudaGetLastError();
   }
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(p.rows * parts));
-  cfg.blockDim = dim3(kThreads);
+  cfg.gridDim = dim3(n * parts);
+  cfg.blockDim = dim3(kFew);
   cfg.stream = s;
   cudaLaunchAttribute at{};
   at.id = cudaLaunchAttributeClusterDimension;
@@ -579,16 +621,14 @@ cudaError_t launch_fwd(const LogprobParams& p, cudaStream_t s) {
   at.val.clusterDim.y = at.val.clusterDim.z = 1;
   cfg.attrs = &at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, logprob_fwd_kernel<T, true>, p);
+  return cudaLaunchKernelEx(&cfg, logprob_fwd_kernel<T, kFew, true>, p);
 }
 
 template <typename T>
 cudaError_t launch_bwd(const LogprobParams& p, cudaStream_t s) {
-  // few rows: several CTAs on each, of one chunk per thread at least
-  const int chunks = p.V / (16 / (int)sizeof(T)) + 1;
-  int spans = 1;
-  while (p.rows * spans * 2 <= 4 * sm_count() && chunks >= 2 * spans * kThreads) spans *= 2;
-  logprob_bwd_kernel<T><<<dim3((unsigned)p.rows, spans), kThreads, 0, s>>>(p);
+  const dim3 grid((unsigned)p.rows, parts_of(p, 16 / sizeof(T), 1024));
+  if (many(p)) logprob_bwd_kernel<T, kMany><<<grid, kMany, 0, s>>>(p);
+  else logprob_bwd_kernel<T, kFew><<<grid, kFew, 0, s>>>(p);
   return cudaGetLastError();
 }
 
