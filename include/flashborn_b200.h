@@ -464,9 +464,9 @@ FB_API int fb_logprob_bwd(const fb_logprob_args* args, void* stream);
  *   norm = sqrt(sum over all tensors of g^2);  c = min(1, max_norm / (norm + eps));  out = c g
  * The arrays of `count` entries are host memory, read during the call.  grads[i] and out[i] are
  * dense tensors of numel[i] elements of type dtype[i] and out_dtype[i] (the same, or FB_F32).
- * out[i] == grads[i] scales in place, and then nothing is written when c is 1.  out NULL: the norm
- * alone.  A NaN gradient gives a NaN norm and NaN outputs; squares are summed in fp32 per thread and
- * in fp64 across threads.  norm: device fp32 scalar. */
+ * out[i] == grads[i] scales in place; where all do, nothing is written when c is 1.  out NULL: the norm
+ * alone.  A NaN gradient gives a NaN norm and NaN outputs; a thread's few squares of a chunk are summed in
+ * fp32, everything beyond in fp64.  At most 2^36 elements a tensor.  norm: device fp32 scalar. */
 typedef struct fb_clip_args {
   int32_t count;
   const void* const* grads;

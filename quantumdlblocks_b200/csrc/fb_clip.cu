@@ -1,6 +1,18 @@
 // fb_clip.cu -- the global norm of many gradient tensors, and clipping.
 //
 //   norm = sqrt(sum g^2),  c = min(1, max_norm / (norm + eps)),  out = c g
+//
+// Two kernels, whatever the tensors' number and types.  All tensors' elements are cut into chunks of
+// kChunkBytes, the table of tensors travels in the kernel's parameters (kTensors to a launch; more take
+// more launches), and CTA b of a launch takes chunks b, b + grid, ...:
+//
+//   clip_sum    each CTA's sum of squares: fp32 for the 16 or 32 squares of a thread and chunk, fp64 beyond
+//   clip_scale  each CTA adds all CTAs' sums, in order, to the norm (the same bits everywhere and every time),
+//               and scales its chunks; in place with c = 1 there is nothing to do.  It takes the chunks from the
+//               last to the first: what clip_sum read last is still in L2.
+//
+// Both are bound by HBM bandwidth for many elements; for few by the two launches, the second of which is
+// under way while the first runs.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -12,97 +24,339 @@ namespace fb {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kBlocks = 64;  // per tensor
+constexpr int kUnroll = 4;                                // 16-byte loads a thread has under way
+constexpr int kChunkBytes = kThreads * kUnroll * 16;      // 16 KB
+constexpr int kTensors = 96;                              // per launch: the table stays under 4 KB
+constexpr int kCtasPerSm = 6;
+
+struct Tensor {
+  const void* g;
+  void* out;
+  int64_t n;
+  uint32_t chunk0;    // its first chunk in the launch
+  uint8_t dtype, out_dtype;
+};
+
+struct ClipParams {
+  Tensor t[kTensors];
+  int count;
+  uint32_t chunks;    // of the launch
+  double* part;       // clip_sum: this launch's sums; clip_scale: all launches'
+  int parts;          // clip_scale
+  float max_norm, eps;
+  float* norm;        // clip_scale: where its first launch writes the norm
+  bool in_place;      // all of them
+};
+static_assert(sizeof(ClipParams) <= 4096, "kernel parameters");
+
+template <typename T> struct Vec {
+  static constexpr int N = 16 / sizeof(T);
+};
+__device__ __forceinline__ void unpack(const uint4& w, float (&f)[4], const float*) {
+  f[0] = __uint_as_float(w.x), f[1] = __uint_as_float(w.y), f[2] = __uint_as_float(w.z), f[3] = __uint_as_float(w.w);
+}
+__device__ __forceinline__ void unpack(const uint4& w, float (&f)[8], const __nv_bfloat16*) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[2 * i] = __uint_as_float((&w.x)[i] << 16);
+    f[2 * i + 1] = __uint_as_float((&w.x)[i] & 0xFFFF0000u);
+  }
+}
+__device__ __forceinline__ void unpack(const uint4& w, float (&f)[8], const __half*) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t b = (&w.x)[i];
+    const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&b));
+    f[2 * i] = v.x;
+    f[2 * i + 1] = v.y;
+  }
+}
+
+// Elements of a chunk: 16-byte vectors of memory from the first that the tensor touches, so that every load is
+// aligned; the tensor's first and last vector may be partly its own.
+template <typename T> struct Span {
+  static constexpr int N = Vec<T>::N;
+  const T* base;   // 16-byte boundary at or before the tensor
+  int64_t lo, hi;  // the tensor's elements from there
+  int64_t v0;      // the chunk's first vector
+  __device__ Span(const Tensor& t, uint32_t chunk) {
+    const int shift = (int)((reinterpret_cast<uintptr_t>(t.g) & 15) / sizeof(T));
+    base = static_cast<const T*>(t.g) - shift;
+    lo = shift;
+    hi = shift + t.n;
+    v0 = (int64_t)(chunk - t.chunk0) * (kChunkBytes / 16);
+  }
+  // 0: outside, 1: wholly inside, 2: partly
+  __device__ int kind(int64_t v) const {
+    if (v * N >= lo && (v + 1) * N <= hi) return 1;
+    return v * N < hi && (v + 1) * N > lo ? 2 : 0;
+  }
+  __device__ uint4 load(int64_t v, int k) const {
+    if (k == 1) return *(reinterpret_cast<const uint4*>(base) + v);
+    uint4 w = make_uint4(0, 0, 0, 0);
+    if (k == 2) {
+      T* e = reinterpret_cast<T*>(&w);
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (v * N + i >= lo && v * N + i < hi) e[i] = base[v * N + i];
+    }
+    return w;
+  }
+};
+
+// The tensor that holds a chunk (the last that starts at or before it: tensors without elements have none)
+__device__ __forceinline__ int tensor_of(const ClipParams& p, uint32_t chunk) {
+  int a = 0, b = p.count;  // t[a].chunk0 <= chunk, t[b].chunk0 > chunk
+  while (b - a > 1) {
+    const int m = (a + b) / 2;
+    if (p.t[m].chunk0 <= chunk) a = m;
+    else b = m;
+  }
+  return a;
+}
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) clip_sum_simple(const T* g, int64_t n, double* part) {
-  float s = 0.f;
-  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < n; i += (int64_t)kBlocks * kThreads) {
-    const float x = to_f32(g[i]);
-    s += x * x;
+__device__ __forceinline__ float squares(const Tensor& t, uint32_t chunk) {
+  const Span<T> s(t, chunk);
+  uint4 w[kUnroll];
+#pragma unroll
+  for (int i = 0; i < kUnroll; ++i) {
+    const int64_t v = s.v0 + i * kThreads + threadIdx.x;
+    w[i] = s.load(v, s.kind(v));
   }
-  double d = s;
-  for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < kUnroll; ++i) {
+    float f[Vec<T>::N];
+    unpack(w[i], f, static_cast<const T*>(nullptr));
+#pragma unroll
+    for (int e = 0; e < Vec<T>::N; ++e) sum = fmaf(f[e], f[e], sum);
+  }
+  return sum;
+}
+
+// The sum over the block, in every thread
+__device__ __forceinline__ double block_sum(double d) {
   __shared__ double sh[kThreads / 32];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
   if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = d;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    d = 0.0;
-    for (int i = 0; i < kThreads / 32; ++i) d += sh[i];
-    part[blockIdx.x] = d;
+  d = 0.0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) d += sh[w];
+  return d;
+}
+
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) clip_sum(const __grid_constant__ ClipParams p) {
+  asm volatile("griddepcontrol.launch_dependents;");
+  double sum = 0.0;
+  for (uint32_t chunk = blockIdx.x; chunk < p.chunks; chunk += gridDim.x) {
+    const Tensor& t = p.t[tensor_of(p, chunk)];
+    if (t.dtype == FB_F32) sum += squares<float>(t, chunk);
+    else if (t.dtype == FB_BF16) sum += squares<__nv_bfloat16>(t, chunk);
+    else sum += squares<__half>(t, chunk);
+  }
+  const double d = block_sum(sum);
+  if (threadIdx.x == 0) p.part[blockIdx.x] = d;
+}
+
+__device__ __forceinline__ uint4 pack(const float (&f)[4], const float*) {
+  return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+}
+__device__ __forceinline__ uint4 pack(const float (&f)[8], const __nv_bfloat16*) {
+  uint4 w;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+    (&w.x)[i] = *reinterpret_cast<const uint32_t*>(&v);
+  }
+  return w;
+}
+__device__ __forceinline__ uint4 pack(const float (&f)[8], const __half*) {
+  uint4 w;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __half2 v = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+    (&w.x)[i] = *reinterpret_cast<const uint32_t*>(&v);
+  }
+  return w;
+}
+__device__ __forceinline__ void store(__nv_bfloat16* to, const float (&f)[8]) {
+  *reinterpret_cast<uint4*>(to) = pack(f, static_cast<const __nv_bfloat16*>(nullptr));
+}
+__device__ __forceinline__ void store(__half* to, const float (&f)[8]) {
+  *reinterpret_cast<uint4*>(to) = pack(f, static_cast<const __half*>(nullptr));
+}
+__device__ __forceinline__ void store(float* to, const float (&f)[4]) {
+  *reinterpret_cast<uint4*>(to) = pack(f, static_cast<const float*>(nullptr));
+}
+__device__ __forceinline__ void store(float* to, const float (&f)[8]) {
+  reinterpret_cast<float4*>(to)[0] = make_float4(f[0], f[1], f[2], f[3]);
+  reinterpret_cast<float4*>(to)[1] = make_float4(f[4], f[5], f[6], f[7]);
+}
+
+template <typename T, typename U>
+__device__ __forceinline__ void scale(const Tensor& t, uint32_t chunk, float c) {
+  constexpr int N = Vec<T>::N;
+  const Span<T> s(t, chunk);
+  U* out = static_cast<U*>(t.out) - s.lo;  // element i of the span goes to out[i]
+  const bool aligned = (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+  uint4 w[kUnroll];
+#pragma unroll
+  for (int i = 0; i < kUnroll; ++i) {
+    const int64_t v = s.v0 + i * kThreads + threadIdx.x;
+    w[i] = s.load(v, s.kind(v));
+  }
+#pragma unroll
+  for (int i = 0; i < kUnroll; ++i) {
+    const int64_t v = s.v0 + i * kThreads + threadIdx.x;
+    const int k = s.kind(v);
+    float f[N];
+    unpack(w[i], f, static_cast<const T*>(nullptr));
+#pragma unroll
+    for (int e = 0; e < N; ++e) f[e] *= c;
+    if (k == 1 && aligned) {
+      store(out + v * N, f);
+    } else if (k != 0) {
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (v * N + e >= s.lo && v * N + e < s.hi) out[v * N + e] = from_f32<U>(f[e]);
+    }
   }
 }
 
-__global__ void clip_norm_simple(const double* part, int n, float* norm) {
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) clip_scale(const __grid_constant__ ClipParams p) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;");
   double d = 0.0;
-  for (int i = 0; i < n; ++i) d += part[i];
-  *norm = (float)sqrt(d);
+  for (int i = threadIdx.x; i < p.parts; i += kThreads) d += p.part[i];
+  const float norm = (float)sqrt(block_sum(d));
+  if (p.norm != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *p.norm = norm;
+  float c = p.max_norm / (norm + p.eps);
+  if (c >= 1.f) c = 1.f;  // a NaN norm stays NaN
+  if (c == 1.f && p.in_place) return;
+  for (uint32_t i = blockIdx.x; i < p.chunks; i += gridDim.x) {
+    const uint32_t chunk = p.chunks - 1 - i;
+    const Tensor& t = p.t[tensor_of(p, chunk)];
+    if (t.dtype == FB_F32) scale<float, float>(t, chunk, c);
+    else if (t.dtype == FB_BF16 && t.out_dtype == FB_BF16) scale<__nv_bfloat16, __nv_bfloat16>(t, chunk, c);
+    else if (t.dtype == FB_BF16) scale<__nv_bfloat16, float>(t, chunk, c);
+    else if (t.out_dtype == FB_F16) scale<__half, __half>(t, chunk, c);
+    else scale<__half, float>(t, chunk, c);
+  }
 }
 
-__device__ __forceinline__ float clip_factor(float norm, float max_norm, float eps) {
-  const float c = max_norm / (norm + eps);
-  return c >= 1.f ? 1.f : c;  // a NaN norm stays NaN
-}
-
-template <typename T, typename U>
-__global__ void __launch_bounds__(kThreads) clip_scale_simple(const T* g, U* out, int64_t n, const float* norm,
-                                                              float max_norm, float eps) {
-  const float c = clip_factor(*norm, max_norm, eps);
-  if (c == 1.f && static_cast<const void*>(g) == static_cast<const void*>(out)) return;
-  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < n; i += (int64_t)kBlocks * kThreads)
-    out[i] = from_f32<U>(to_f32(g[i]) * c);
-}
-
-template <typename T, typename U>
-void scale_one(const fb_clip_args* a, int i, cudaStream_t s) {
-  clip_scale_simple<T, U><<<kBlocks, kThreads, 0, s>>>(static_cast<const T*>(a->grads[i]), static_cast<U*>(a->out[i]),
-                                                       a->numel[i], a->norm, a->max_norm, a->eps);
+int sm_count() {
+  static int count[64];  // per device; 0: not asked yet (two threads that ask write the same)
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  if (count[dev] == 0) {
+    int n = 0;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 1) return 148;
+    count[dev] = n;
+  }
+  return count[dev];
 }
 
 bool bad_dtype(int d) { return d != FB_F32 && d != FB_F16 && d != FB_BF16; }
+int size_of(int dtype) { return dtype == FB_F32 ? 4 : 2; }
 
-size_t workspace_size(const fb_clip_args* a) { return (size_t)std::max(a->count, 1) * kBlocks * sizeof(double); }
+uint64_t chunks_of(const void* g, int64_t n, int dtype) {
+  if (n == 0) return 0;
+  const uint64_t bytes = (uint64_t)n * size_of(dtype) + (reinterpret_cast<uintptr_t>(g) & 15);
+  return (bytes + kChunkBytes - 1) / kChunkBytes;
+}
 
-int clip(const fb_clip_args* a, cudaStream_t s) {
+// Every launch leaves at most kCtasPerSm sums per SM
+size_t workspace_size(const fb_clip_args* a) {
+  const size_t launches = (size_t)std::max(1, (a->count + kTensors - 1) / kTensors);
+  return launches * kCtasPerSm * sm_count() * sizeof(double);
+}
+
+int check(const fb_clip_args* a) {
   if (a == nullptr || a->norm == nullptr) return FB_ERR_ARG;
   if (a->count < 0) return FB_ERR_SHAPE;
   if (a->count > 0 && (a->grads == nullptr || a->numel == nullptr || a->dtype == nullptr)) return FB_ERR_ARG;
   if (a->out != nullptr && (!(a->max_norm >= 0.f) || !(a->eps >= 0.f))) return FB_ERR_ARG;
   for (int i = 0; i < a->count; ++i) {
-    if (a->numel[i] < 0) return FB_ERR_SHAPE;
+    if (a->numel[i] < 0 || a->numel[i] > (1ll << 36)) return FB_ERR_SHAPE;  // a launch's chunks count in 32 bits
     if (bad_dtype(a->dtype[i])) return FB_ERR_DTYPE;
     if (a->out != nullptr && a->out_dtype != nullptr && a->out_dtype[i] != a->dtype[i] && a->out_dtype[i] != FB_F32)
       return FB_ERR_DTYPE;
-    if (a->numel[i] > 0 && (a->grads[i] == nullptr || (a->out != nullptr && a->out[i] == nullptr))) return FB_ERR_ARG;
+    if (a->numel[i] == 0) continue;
+    if (a->grads[i] == nullptr || (a->out != nullptr && a->out[i] == nullptr)) return FB_ERR_ARG;
+    const int out_size = a->out_dtype != nullptr ? size_of(a->out_dtype[i]) : size_of(a->dtype[i]);
+    if (reinterpret_cast<uintptr_t>(a->grads[i]) % size_of(a->dtype[i]) != 0 ||
+        (a->out != nullptr && reinterpret_cast<uintptr_t>(a->out[i]) % out_size != 0))
+      return FB_ERR_ALIGN;
   }
   if (a->workspace == nullptr || a->workspace_bytes < workspace_size(a)) return FB_ERR_WORKSPACE;
-  double* part = static_cast<double*>(a->workspace);
-  int launches = 1;
-  for (int i = 0; i < a->count; ++i, ++launches) {
-    double* to = part + (size_t)i * kBlocks;
-    if (a->dtype[i] == FB_F32)
-      clip_sum_simple<float><<<kBlocks, kThreads, 0, s>>>(static_cast<const float*>(a->grads[i]), a->numel[i], to);
-    else if (a->dtype[i] == FB_F16)
-      clip_sum_simple<__half><<<kBlocks, kThreads, 0, s>>>(static_cast<const __half*>(a->grads[i]), a->numel[i], to);
-    else
-      clip_sum_simple<__nv_bfloat16>
-          <<<kBlocks, kThreads, 0, s>>>(static_cast<const __nv_bfloat16*>(a->grads[i]), a->numel[i], to);
+  return FB_OK;
+}
+
+// The launch's table: tensors [i0, i1)
+void fill(ClipParams* p, const fb_clip_args* a, int i0, int i1) {
+  p->count = 0;
+  p->chunks = 0;
+  p->in_place = true;
+  for (int i = i0; i < i1; ++i) {
+    const uint64_t n = chunks_of(a->grads[i], a->numel[i], a->dtype[i]);
+    if (n == 0) continue;
+    Tensor& t = p->t[p->count++];
+    t.g = a->grads[i];
+    t.out = a->out != nullptr ? a->out[i] : nullptr;
+    p->in_place = p->in_place && t.out == t.g;
+    t.n = a->numel[i];
+    t.chunk0 = p->chunks;
+    t.dtype = (uint8_t)a->dtype[i];
+    t.out_dtype = (uint8_t)(a->out_dtype != nullptr ? a->out_dtype[i] : a->dtype[i]);
+    p->chunks += (uint32_t)n;
   }
-  clip_norm_simple<<<1, 1, 0, s>>>(part, a->count * kBlocks, a->norm);
-  for (int i = 0; a->out != nullptr && i < a->count; ++i, ++launches) {
-    const int in = a->dtype[i], to = a->out_dtype != nullptr ? a->out_dtype[i] : in;
-    if (in == FB_F32) scale_one<float, float>(a, i, s);
-    else if (in == FB_F16 && to == FB_F16) scale_one<__half, __half>(a, i, s);
-    else if (in == FB_F16) scale_one<__half, float>(a, i, s);
-    else if (to == FB_BF16) scale_one<__nv_bfloat16, __nv_bfloat16>(a, i, s);
-    else scale_one<__nv_bfloat16, float>(a, i, s);
+}
+
+int clip(const fb_clip_args* a, cudaStream_t s) {
+  const int rc = check(a);
+  if (rc != FB_OK) return rc;
+  const int most = kCtasPerSm * sm_count(), launches = std::max(1, (a->count + kTensors - 1) / kTensors);
+  ClipParams p{};
+  p.max_norm = a->max_norm;
+  p.eps = a->eps;
+  double* sums = static_cast<double*>(a->workspace);
+  int parts = 0;
+  cudaError_t e = cudaSuccess;
+  for (int l = 0; l < launches && e == cudaSuccess; ++l) {
+    fill(&p, a, l * kTensors, std::min(a->count, (l + 1) * kTensors));
+    const int grid = (int)std::max<uint32_t>(1, std::min<uint32_t>(p.chunks, most));
+    p.part = sums + parts;
+    parts += grid;
+    clip_sum<<<grid, kThreads, 0, s>>>(p);
+    e = cudaGetLastError();
   }
-  const cudaError_t e = cudaGetLastError();
+  // one launch: its table still is in p
+  p.part = sums;
+  p.parts = parts;
+  int n = launches;
+  for (int l = 0; l < (a->out != nullptr ? launches : 1) && e == cudaSuccess; ++l, ++n) {
+    if (launches > 1) fill(&p, a, l * kTensors, std::min(a->count, (l + 1) * kTensors));
+    p.norm = l == 0 ? a->norm : nullptr;
+    if (a->out == nullptr) p.chunks = 0;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(std::max<uint32_t>(1, std::min<uint32_t>(p.chunks, most)));
+    cfg.blockDim = dim3(kThreads);
+    cfg.stream = s;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, clip_scale, p);
+  }
   if (e != cudaSuccess) {
     record_cuda_error(e);
     return FB_ERR_LAUNCH;
   }
-  set_last_launch_count(launches);
+  set_last_launch_count(n);
   return FB_OK;
 }
 
