@@ -767,26 +767,139 @@ struct WriteParams {
   void* v_out;
 };
 
-// One warp per (token, head).
+// The page and row of token n's slot; false where it has none.
+__device__ __forceinline__ bool slot_of_token(const WriteParams& p, int64_t n, int& pg, int& row) {
+  const int64_t slot = p.slots[n], all = (int64_t)p.pages * p.page;
+  const bool stored = slot >= 0 && slot < all;
+  const uint64_t s = stored ? (uint64_t)slot : 0;
+  pg = all <= 0xFFFFFFFFll ? (int)((uint32_t)s / (uint32_t)p.page) : (int)(s / (uint32_t)p.page);
+  row = (int)(s - (uint64_t)pg * p.page);
+  return stored;
+}
+
+// Where head h's row of token n goes: its place in the cache (or q), and its copy.
+template <typename T> struct Targets {
+  T *to, *copy;
+  bool put;
+  __device__ Targets(const WriteParams& p, int64_t n, int h, int pg, int row, bool stored) {
+    copy = nullptr;
+    put = stored;
+    if (h < p.H) {
+      to = static_cast<T*>(p.q) + (n * p.H + h) * p.D;
+      put = true;
+    } else {
+      const bool is_v = h >= p.H + p.Hkv;
+      const int kvh = h - p.H - (is_v ? p.Hkv : 0);
+      to = is_v ? static_cast<T*>(p.v) + pg * p.vs[0] + kvh * p.vs[1] + row * p.vs[2]
+                : static_cast<T*>(p.k) + pg * p.ks[0] + kvh * p.ks[1] + row * p.ks[2];
+      void* c = is_v ? p.v_out : p.k_out;
+      if (c) copy = static_cast<T*>(c) + (n * p.Hkv + kvh) * p.D;
+    }
+  }
+};
+
+__device__ __forceinline__ void unpack16(const uint4& w, float (&f)[4], const float*) {
+  f[0] = __uint_as_float(w.x), f[1] = __uint_as_float(w.y), f[2] = __uint_as_float(w.z), f[3] = __uint_as_float(w.w);
+}
+__device__ __forceinline__ void unpack16(const uint4& w, float (&f)[8], const __nv_bfloat16*) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[2 * i] = __uint_as_float((&w.x)[i] << 16);
+    f[2 * i + 1] = __uint_as_float((&w.x)[i] & 0xFFFF0000u);
+  }
+}
+__device__ __forceinline__ void unpack16(const uint4& w, float (&f)[8], const __half*) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f[2 * i] = half_lo((&w.x)[i]), f[2 * i + 1] = half_hi((&w.x)[i]);
+}
+
+// Rows of 8, 16 or 32 16-byte pieces on 16-byte boundaries: LPH lanes a head, 32 / LPH heads an access, ACC
+// accesses a warp, all of one token.  The turn's other half of a piece is LPH / 2 lanes away (one exchange of
+// the raw words), the norm a sum over the head's lanes.  Reads and writes every element once: HBM bandwidth
+// bounds it, latency for a batch's new tokens (ACC = 1 spreads them over more warps).
+template <typename T, int LPH, int ACC>
+__global__ void __launch_bounds__(256) paged_write_vec(const WriteParams p, int per_token) {
+  constexpr int N = 16 / sizeof(T), HPA = 32 / LPH;
+  const int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int64_t n = item / per_token;
+  if (n >= p.N) return;
+  const int lane = threadIdx.x & 31, sub = lane % LPH, heads = p.H + 2 * p.Hkv;
+  const int h0 = (int)(item - n * per_token) * (HPA * ACC) + lane / LPH;
+  const T* x = static_cast<const T*>(p.qkv) + n * p.ld + sub * N;
+  uint4 w[ACC];
+#pragma unroll
+  for (int i = 0; i < ACC; ++i) {
+    const int h = h0 + i * HPA;
+    w[i] = make_uint4(0, 0, 0, 0);
+    if (h < heads) w[i] = *reinterpret_cast<const uint4*>(x + (int64_t)h * p.D);
+  }
+  int pg, row;
+  const bool stored = slot_of_token(p, n, pg, row);
+  const int64_t pos = p.positions[n];
+  const bool known = pos >= 0 && pos < p.rope_rows;
+  float c[N], s[N];
+  {
+    const int64_t at = (known ? pos : 0) * (p.D / 2) + (sub % (LPH / 2)) * N;
+#pragma unroll
+    for (int e = 0; e < N; e += 4) {
+      const float4 a = known ? *reinterpret_cast<const float4*>(p.cos + at + e) : make_float4(NAN, NAN, NAN, NAN);
+      const float4 b = known ? *reinterpret_cast<const float4*>(p.sin + at + e) : make_float4(NAN, NAN, NAN, NAN);
+      c[e] = a.x, c[e + 1] = a.y, c[e + 2] = a.z, c[e + 3] = a.w;
+      s[e] = b.x, s[e + 1] = b.y, s[e + 2] = b.z, s[e + 3] = b.w;
+    }
+    if (sub < LPH / 2) {  // first half: a cos - b sin; second: b cos + a sin
+#pragma unroll
+      for (int e = 0; e < N; ++e) s[e] = -s[e];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < ACC; ++i) {
+    const int h = h0 + i * HPA;
+    uint4 o;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) (&o.x)[e] = __shfl_xor_sync(0xffffffffu, (&w[i].x)[e], LPH / 2);
+    float f[N], g[N], ss = 0.f;
+    unpack16(w[i], f, static_cast<const T*>(nullptr));
+    unpack16(o, g, static_cast<const T*>(nullptr));
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      f[e] = f[e] * c[e] + g[e] * s[e];
+      ss = fmaf(f[e], f[e], ss);
+    }
+#pragma unroll
+    for (int d = LPH / 2; d > 0; d >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
+    if (h >= heads) continue;
+    uint4 out = w[i];
+    if (h < p.H + p.Hkv) {
+      const float r = rsqrtf(ss + p.eps);
+      T t[N];
+#pragma unroll
+      for (int e = 0; e < N; ++e) t[e] = from_f32<T>(f[e] * r);
+      memcpy(&out, t, 16);
+    }
+    const Targets<T> to(p, n, h, pg, row, stored);
+    if (to.put) *reinterpret_cast<uint4*>(to.to + sub * N) = out;
+    if (to.copy) *reinterpret_cast<uint4*>(to.copy + sub * N) = out;
+  }
+}
+
+// Every other head dimension and alignment: one warp per (token, head), element by element.
 template <typename T>
-__global__ void __launch_bounds__(256) paged_write_simple(const WriteParams p) {
+__global__ void __launch_bounds__(256) paged_write_general(const WriteParams p) {
   const int heads = p.H + 2 * p.Hkv;
   const int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (item >= p.N * heads) return;
   const int64_t n = item / heads;
-  const int h = (int)(item % heads), lane = threadIdx.x & 31, half = p.D / 2;
+  if (n >= p.N) return;
+  const int h = (int)(item - n * heads), lane = threadIdx.x & 31, half = p.D / 2;
   const T* x = static_cast<const T*>(p.qkv) + n * p.ld + (int64_t)h * p.D;
-  const int64_t slot = p.slots[n], pos = p.positions[n];
-  const bool stored = slot >= 0 && slot < (int64_t)p.pages * p.page;
-  const int64_t pg = stored ? slot / p.page : 0;
-  const int row = stored ? (int)(slot % p.page) : 0;
-  if (h >= p.H + p.Hkv) {  // V
-    const int kvh = h - p.H - p.Hkv;
-    T* to = static_cast<T*>(p.v) + pg * p.vs[0] + kvh * p.vs[1] + row * p.vs[2];
-    T* copy = p.v_out ? static_cast<T*>(p.v_out) + (n * p.Hkv + kvh) * p.D : nullptr;
+  int pg, row;
+  const bool stored = slot_of_token(p, n, pg, row);
+  const int64_t pos = p.positions[n];
+  const Targets<T> to(p, n, h, pg, row, stored);
+  if (h >= p.H + p.Hkv) {
     for (int d = lane; d < p.D; d += 32) {
-      if (stored) to[d] = x[d];
-      if (copy) copy[d] = x[d];
+      if (to.put) to.to[d] = x[d];
+      if (to.copy) to.copy[d] = x[d];
     }
     return;
   }
@@ -796,30 +909,20 @@ __global__ void __launch_bounds__(256) paged_write_simple(const WriteParams p) {
   for (int i = 0; i < 4; ++i) {
     const int d = lane + 32 * i;
     if (d >= half) continue;
-    const float c = known ? p.cos[pos * half + d] : NAN, sn = known ? p.sin[pos * half + d] : NAN;
+    const float c = known ? p.cos[pos * half + d] : NAN, s = known ? p.sin[pos * half + d] : NAN;
     const float x1 = to_f32(x[d]), x2 = to_f32(x[d + half]);
-    a[i] = x1 * c - x2 * sn;
-    b[i] = x1 * sn + x2 * c;
+    a[i] = x1 * c - x2 * s;
+    b[i] = x1 * s + x2 * c;
     ss += a[i] * a[i] + b[i] * b[i];
   }
   const float r = rsqrtf(warp_sum(ss) + p.eps);
-  T *to, *copy = nullptr;
-  bool put = true;
-  if (h < p.H) {
-    to = static_cast<T*>(p.q) + (n * p.H + h) * p.D;
-  } else {
-    const int kvh = h - p.H;
-    to = static_cast<T*>(p.k) + pg * p.ks[0] + kvh * p.ks[1] + row * p.ks[2];
-    put = stored;
-    if (p.k_out) copy = static_cast<T*>(p.k_out) + (n * p.Hkv + kvh) * p.D;
-  }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int d = lane + 32 * i;
     if (d >= half) continue;
     const T lo = from_f32<T>(a[i] * r), hi = from_f32<T>(b[i] * r);
-    if (put) to[d] = lo, to[d + half] = hi;
-    if (copy) copy[d] = lo, copy[d + half] = hi;
+    if (to.put) to.to[d] = lo, to.to[d + half] = hi;
+    if (to.copy) to.copy[d] = lo, to.copy[d + half] = hi;
   }
 }
 
@@ -1030,6 +1133,18 @@ int paged_fwd(const fb_paged_args* a, cudaStream_t st) {
   return FB_OK;
 }
 
+template <typename T, int LPH>
+void launch_write(const WriteParams& p, bool spread, int per_token, unsigned blocks, cudaStream_t st) {
+  if (spread) paged_write_vec<T, LPH, 1><<<blocks, 256, 0, st>>>(p, per_token);
+  else paged_write_vec<T, LPH, 4><<<blocks, 256, 0, st>>>(p, per_token);
+}
+template <typename T>
+void launch_write(const WriteParams& p, int lanes, bool spread, int per_token, unsigned blocks, cudaStream_t st) {
+  if (lanes == 8) launch_write<T, 8>(p, spread, per_token, blocks, st);
+  else if (lanes == 16) launch_write<T, 16>(p, spread, per_token, blocks, st);
+  else launch_write<T, 32>(p, spread, per_token, blocks, st);
+}
+
 int paged_write(const fb_paged_write_args* a, cudaStream_t st) {
   if (a == nullptr) return FB_ERR_ARG;
   if (a->tokens < 0 || a->heads < 1 || a->kv_heads < 1 || a->heads % a->kv_heads != 0 || a->heads > 65535 ||
@@ -1053,11 +1168,27 @@ int paged_write(const fb_paged_write_args* a, cudaStream_t st) {
   p.positions = a->positions; p.slots = a->slots; p.k = a->k; p.v = a->v; p.q = a->q;
   p.k_out = a->k_out; p.v_out = a->v_out;
   for (int i = 0; i < 4; ++i) p.ks[i] = a->k_stride[i], p.vs[i] = a->v_stride[i];
-  const int64_t blocks = (p.N * (p.H + 2 * p.Hkv) + 7) / 8;
+  const int size = a->dtype == FB_F32 ? 4 : 2, lanes = p.D * size / 16;
+  auto at16 = [](const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0; };
+  const bool vec = p.D * size % 16 == 0 && (lanes == 8 || lanes == 16 || lanes == 32) && aligned16(p.k, p.ks, 3, size) &&
+                   aligned16(p.v, p.vs, 3, size) && aligned16(p.qkv, &p.ld, 1, size) && at16(p.q) && at16(p.cos) &&
+                   at16(p.sin) && at16(p.k_out) && at16(p.v_out);
+  if (!vec) {
+    const int64_t blocks = (p.N * (p.H + 2 * p.Hkv) + 7) / 8;
+    if (blocks > 0x7FFFFFFF) return FB_ERR_SHAPE;
+    if (a->dtype == FB_F32) paged_write_general<float><<<(unsigned)blocks, 256, 0, st>>>(p);
+    else if (a->dtype == FB_F16) paged_write_general<__half><<<(unsigned)blocks, 256, 0, st>>>(p);
+    else paged_write_general<__nv_bfloat16><<<(unsigned)blocks, 256, 0, st>>>(p);
+    return launched(1);
+  }
+  const int accesses = (p.H + 2 * p.Hkv + 32 / lanes - 1) / (32 / lanes);
+  const bool spread = p.N * accesses < 4 * 64 * (int64_t)sm_count();  // fewer warps than the SMs hold, at four accesses each
+  const int per_token = spread ? accesses : (accesses + 3) / 4;
+  const int64_t blocks = (p.N * per_token + 7) / 8;
   if (blocks > 0x7FFFFFFF) return FB_ERR_SHAPE;
-  if (a->dtype == FB_F32) paged_write_simple<float><<<(unsigned)blocks, 256, 0, st>>>(p);
-  else if (a->dtype == FB_F16) paged_write_simple<__half><<<(unsigned)blocks, 256, 0, st>>>(p);
-  else paged_write_simple<__nv_bfloat16><<<(unsigned)blocks, 256, 0, st>>>(p);
+  if (a->dtype == FB_F32) launch_write<float>(p, lanes, spread, per_token, (unsigned)blocks, st);
+  else if (a->dtype == FB_F16) launch_write<__half>(p, lanes, spread, per_token, (unsigned)blocks, st);
+  else launch_write<__nv_bfloat16>(p, lanes, spread, per_token, (unsigned)blocks, st);
   return launched(1);
 }
 

@@ -6,46 +6,56 @@ their number, sizes and types.  CUDA only, like every op here.
 """
 from __future__ import annotations
 
-import ctypes
+import array
 from typing import Iterable, Optional, Sequence
 
 import torch
 
 from .. import _lib
-from .flash_born import _DTYPE_CODE, _stream_handle
+from ._host import launch, packer
+from .flash_born import _DTYPE_CODE
 
 __all__ = ["clip_grad_norm_", "grad_norm"]
+
+
+_clip_args = packer(_lib.FbClipArgs)
+
+
+def _codes(what: str, tensors: Sequence[torch.Tensor], index: int) -> array.array:
+    """The tensors' dtype codes; raises where one is not a float tensor on device `index`."""
+    if any(t.get_device() != index for t in tensors):
+        if all(t.is_cuda for t in tensors):
+            raise RuntimeError(f"{what}: all tensors must be on one device; got {sorted({str(t.device) for t in tensors})}")
+        raise RuntimeError(f"{what} (B200): CUDA tensors required; there is no CPU path")
+    try:
+        return array.array("i", [_DTYPE_CODE[t.dtype] for t in tensors])
+    except KeyError:
+        raise ValueError(f"{what}: gradients are dense float32 / float16 / bfloat16; got "
+                         f"{sorted({str(t.dtype) for t in tensors})}") from None
 
 
 def _run(grads: Sequence[torch.Tensor], out: Optional[Sequence[torch.Tensor]], max_norm: float, eps: float,
          what: str) -> torch.Tensor:
     if not grads:
         raise ValueError(f"{what}: no gradients given (their device is the result's)")
-    device = grads[0].device
-    tensors = list(grads) if out is None or out is grads else list(grads) + list(out)
-    for t in tensors:
-        if not t.is_cuda:
-            raise RuntimeError(f"{what} (B200): CUDA tensors required; there is no CPU path")
-        if t.device != device:
-            raise RuntimeError(f"{what}: all tensors must be on {device}; got one on {t.device}")
-        if t.dtype not in _DTYPE_CODE:
-            raise ValueError(f"{what}: gradients are dense float32 / float16 / bfloat16; got {t.dtype}")
-    n = len(grads)
-    a = _lib.FbClipArgs()
-    a.count, a.max_norm, a.eps = n, max_norm, eps
-    keep = [(ctypes.c_void_p * n)(*[g.data_ptr() for g in grads]), (ctypes.c_int64 * n)(*[g.numel() for g in grads]),
-            (ctypes.c_int32 * n)(*[_DTYPE_CODE[g.dtype] for g in grads])]
-    a.grads, a.numel, a.dtype = (ctypes.cast(x, ctypes.c_void_p) for x in keep)
-    if out is not None:
-        keep += [(ctypes.c_void_p * n)(*[o.data_ptr() for o in out]), (ctypes.c_int32 * n)(*[_DTYPE_CODE[o.dtype] for o in out])]
-        a.out, a.out_dtype = (ctypes.cast(x, ctypes.c_void_p) for x in keep[3:])
-    norm = torch.empty((), dtype=torch.float32, device=device)
+    first = grads[0]
+    index = max(first.get_device(), 0)
+    codes = _codes(what, grads, index)
+    ptrs = array.array("Q", [g.data_ptr() for g in grads])
+    numel = array.array("q", [g.numel() for g in grads])
+    out_ptrs, out_codes = ptrs, codes  # in place
+    if out is not None and out is not grads:
+        out_codes = _codes(what, out, index)
+        out_ptrs = array.array("Q", [o.data_ptr() for o in out])
+    norm = torch.empty((), dtype=torch.float32, device=first.device)
+    a = _clip_args(len(grads), ptrs.buffer_info()[0], out_ptrs.buffer_info()[0] if out is not None else 0,
+                   numel.buffer_info()[0], codes.buffer_info()[0], out_codes.buffer_info()[0], max_norm, eps,
+                   norm.data_ptr(), 0, 0)
     lib = _lib.load()
-    need = lib.fb_clip_workspace_size(ctypes.byref(a))
-    ws = torch.empty(need, dtype=torch.uint8, device=device)
-    a.norm, a.workspace, a.workspace_bytes = norm.data_ptr(), ws.data_ptr(), need
-    with torch.cuda.device(device):
-        _lib.check(lib.fb_clip_grad_norm(ctypes.byref(a), _stream_handle(device)), what)
+    need = lib.fb_clip_workspace_size(a)
+    ws = torch.empty(need, dtype=torch.uint8, device=first.device)
+    a.workspace, a.workspace_bytes = ws.data_ptr(), need
+    launch(lib.fb_clip_grad_norm, a, index, what)
     return norm
 
 
@@ -93,13 +103,17 @@ def clip_grad_norm_(
     to = gs if out is None else list(out)
     if len(to) != len(gs):
         raise ValueError(f"clip_grad_norm_: {len(gs)} gradients, but out has {len(to)} tensors")
-    for g in gs:
-        if not _dense(g):
-            raise ValueError(f"clip_grad_norm_: gradients must be dense; got strides {g.stride()} for {tuple(g.shape)}")
+    plain = all([g.is_contiguous() for g in gs])
+    if not plain:
+        for g in gs:
+            if not _dense(g):
+                raise ValueError(f"clip_grad_norm_: gradients must be dense; got strides {g.stride()} for {tuple(g.shape)}")
     if to is not gs:
-        for g, o in zip(gs, to):
-            if o.shape != g.shape or o.stride() != g.stride() or o.dtype not in (g.dtype, torch.float32):
-                raise ValueError(f"clip_grad_norm_: out must match its gradient's shape and strides, and its dtype or "
-                                 f"float32; got {tuple(o.shape)} {o.stride()} {o.dtype} for {tuple(g.shape)} "
-                                 f"{g.stride()} {g.dtype}")
+        alike = [g.shape for g in gs] == [o.shape for o in to]
+        alike = alike and (all([o.is_contiguous() for o in to]) if plain else [g.stride() for g in gs] == [o.stride() for o in to])
+        if not alike or any([o.dtype is not torch.float32 and o.dtype is not g.dtype for g, o in zip(gs, to)]):
+            raise ValueError("clip_grad_norm_: each of out must match its gradient's shape and memory order, and have its "
+                             "dtype or float32; got "
+                             f"{[(tuple(o.shape), o.stride(), o.dtype) for o in to]} for "
+                             f"{[(tuple(g.shape), g.stride(), g.dtype) for g in gs]}")
     return _run(gs, to, float(max_norm), float(eps), "clip_grad_norm_")

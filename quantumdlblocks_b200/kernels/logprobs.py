@@ -8,13 +8,13 @@ rows of ``-logp`` alone, bf16, aligned vocabularies.)  CUDA only, like every op 
 """
 from __future__ import annotations
 
-import ctypes
 from typing import NamedTuple, Optional
 
 import torch
 
 from .. import _lib
-from .flash_born import _DTYPE_CODE, _stream_handle
+from ._host import launch, packer, same_device
+from .flash_born import _DTYPE_CODE
 
 __all__ = ["TokenLogprobs", "token_logprobs"]
 
@@ -26,35 +26,43 @@ class TokenLogprobs(NamedTuple):
     top_index: torch.Tensor  # (N, top_k) int64
 
 
-def _args(logits: torch.Tensor, targets: torch.Tensor, top_k: int) -> _lib.FbLogprobArgs:
-    a = _lib.FbLogprobArgs()
-    a.rows, a.vocab, a.ld = logits.shape[0], logits.shape[1], max(logits.stride(0), logits.shape[1])
-    a.dtype, a.top_k = _DTYPE_CODE[logits.dtype], top_k
-    a.logits, a.targets = logits.data_ptr(), targets.data_ptr()
-    return a
+_pack = packer(_lib.FbLogprobArgs)
 
 
-def _forward(logits: torch.Tensor, targets: torch.Tensor, top_k: int) -> tuple[torch.Tensor, ...]:
-    n, device = logits.shape[0], logits.device
-    logp, entropy = torch.empty((2, n), dtype=torch.float32, device=device).unbind(0)
-    stats = torch.empty((n, 2), dtype=torch.float32, device=device)
-    top_logp = torch.empty((n, top_k), dtype=torch.float32, device=device)
-    top_index = torch.empty((n, top_k), dtype=torch.int64, device=device)
-    a = _args(logits, targets, top_k)
-    a.logp, a.entropy, a.stats = logp.data_ptr(), entropy.data_ptr(), stats.data_ptr()
-    a.top_logp, a.top_index = top_logp.data_ptr(), top_index.data_ptr()
-    with torch.cuda.device(device):
-        _lib.check(_lib.load().fb_logprob_fwd(ctypes.byref(a), _stream_handle(device)), "token log probabilities")
-    return logp, entropy, stats, top_logp, top_index
+def _args(logits: torch.Tensor, targets: torch.Tensor, top_k: int, logp: int = 0, entropy: int = 0, stats: int = 0,
+          top_logp: int = 0, top_index: int = 0, g_logp: int = 0, g_entropy: int = 0, g_top: int = 0, grad: int = 0):
+    n, v = logits.shape
+    return _pack(n, v, _DTYPE_CODE[logits.dtype], top_k, logits.data_ptr(), max(logits.stride(0), v), targets.data_ptr(),
+                 logp, entropy, stats, top_logp, top_index, g_logp, g_entropy, g_top, grad, v)
+
+
+def _forward(logits: torch.Tensor, targets: torch.Tensor, top_k: int, index: int) -> tuple[torch.Tensor, ...]:
+    n = logits.shape[0]
+    # one allocation where nothing needs the results as tensors of their own
+    logp, entropy, top_logp, stats = torch.empty(n * (4 + top_k), dtype=torch.float32, device=logits.device).split_with_sizes(
+        (n, n, n * top_k, 2 * n))
+    top_index = torch.empty((n, top_k), dtype=torch.int64, device=logits.device)
+    a = _args(logits, targets, top_k, logp.data_ptr(), entropy.data_ptr(), stats.data_ptr(), top_logp.data_ptr(),
+              top_index.data_ptr())
+    launch(_lib.load().fb_logprob_fwd, a, index, "token log probabilities")
+    return logp, entropy, top_logp.view(n, top_k), top_index, stats
 
 
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits: torch.Tensor, targets: torch.Tensor, top_k: int):
-        logp, entropy, stats, top_logp, top_index = _forward(logits, targets, top_k)
+    def forward(ctx, logits: torch.Tensor, targets: torch.Tensor, top_k: int, index: int):
+        # tensors of their own: a caller may change a result in place
+        n, opts = logits.shape[0], dict(dtype=torch.float32, device=logits.device)
+        logp, entropy, top_logp = torch.empty(n, **opts), torch.empty(n, **opts), torch.empty((n, top_k), **opts)
+        stats = torch.empty((n, 2), **opts)
+        top_index = torch.empty((n, top_k), dtype=torch.int64, device=logits.device)
+        a = _args(logits, targets, top_k, logp.data_ptr(), entropy.data_ptr(), stats.data_ptr(),
+                  top_logp.data_ptr(), top_index.data_ptr())
+        launch(_lib.load().fb_logprob_fwd, a, index, "token log probabilities")
         ctx.save_for_backward(logits, targets, entropy, stats, top_index)
         ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(top_index)
+        ctx.index = index
         return logp, entropy, top_logp, top_index
 
     @staticmethod
@@ -62,16 +70,12 @@ class _TokenLogprobs(torch.autograd.Function):
                  g_top: Optional[torch.Tensor], _g_index):
         logits, targets, entropy, stats, top_index = ctx.saved_tensors
         grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        top_k = top_index.shape[1]
-        a = _args(logits, targets, top_k)
-        a.entropy, a.stats, a.top_index = entropy.data_ptr(), stats.data_ptr(), top_index.data_ptr()
         given = [g if g is None else g.to(torch.float32).contiguous() for g in (g_logp, g_entropy, g_top)]
-        a.g_logp, a.g_entropy, a.g_top = (None if g is None else g.data_ptr() for g in given)
-        a.grad, a.grad_ld = grad.data_ptr(), max(grad.stride(0), grad.shape[1])
-        with torch.cuda.device(logits.device):
-            _lib.check(_lib.load().fb_logprob_bwd(ctypes.byref(a), _stream_handle(logits.device)),
-                       "token log probabilities backward")
-        return grad, None, None
+        ptrs = [0 if g is None else g.data_ptr() for g in given]
+        a = _args(logits, targets, top_index.shape[1], 0, entropy.data_ptr(), stats.data_ptr(), 0, top_index.data_ptr(),
+                  *ptrs, grad.data_ptr())
+        launch(_lib.load().fb_logprob_bwd, a, ctx.index, "token log probabilities backward")
+        return grad, None, None, None
 
 
 def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0) -> TokenLogprobs:
@@ -85,8 +89,7 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0) 
     differentiable in the logits (the gradient has their dtype; a row whose incoming gradients are all 0 gets 0,
     whatever it holds).
     """
-    if not (logits.is_cuda and targets.is_cuda):
-        raise RuntimeError("token_logprobs (B200): CUDA tensors required; there is no CPU path")
+    index = same_device("token_logprobs", logits, targets)
     if logits.dim() != 2 or logits.shape[1] < 1 or logits.dtype not in _DTYPE_CODE:
         raise ValueError(f"token_logprobs takes (N, V) float32 / float16 / bfloat16 logits; got {tuple(logits.shape)} "
                          f"{logits.dtype}")
@@ -95,12 +98,10 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0) 
         raise ValueError(f"targets must be ({N},) integers; got {tuple(targets.shape)} {targets.dtype}")
     if not 0 <= top_k <= min(V, _lib.FB_MAX_TOP_K):
         raise ValueError(f"top_k must be in [0, {min(V, _lib.FB_MAX_TOP_K)}]; got {top_k}")
-    if targets.device != logits.device:
-        raise RuntimeError(f"token_logprobs: targets must be on {logits.device}; got {targets.device}")
     # rows closer than V elements (an expanded tensor's) are copied as well: the kernels need ld >= V
     x = logits if (V == 1 or logits.stride(1) == 1) and (N <= 1 or logits.stride(0) >= V) else logits.contiguous()
-    t = targets.to(torch.int64).contiguous()
+    t = targets if targets.dtype is torch.int64 else targets.to(torch.int64)
+    t = t if t.is_contiguous() else t.contiguous()
     if torch.is_grad_enabled() and logits.requires_grad:
-        return TokenLogprobs(*_TokenLogprobs.apply(x, t, int(top_k)))
-    logp, entropy, _, top_logp, top_index = _forward(x, t, int(top_k))
-    return TokenLogprobs(logp, entropy, top_logp, top_index)
+        return TokenLogprobs(*_TokenLogprobs.apply(x, t, int(top_k), index))
+    return TokenLogprobs(*_forward(x, t, int(top_k), index)[:4])

@@ -19,16 +19,16 @@ import ctypes
 import torch
 
 from .. import _lib
-from .flash_born import _DTYPE_CODE, _stream_handle
+from ._host import launch, packer, same_device
+from .flash_born import _DTYPE_CODE
 
 __all__ = ["paged_born_attention", "paged_qkv_write"]
 
-_I64x3, _I64x4 = _lib._I64x3, _lib._I64x4
+_paged_args = packer(_lib.FbPagedArgs)
+_write_args = packer(_lib.FbPagedWriteArgs)
 
 
 def _check_pages(what: str, x: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor) -> None:
-    if not (x.is_cuda and k_pages.is_cuda and v_pages.is_cuda):
-        raise RuntimeError(f"{what} (B200): CUDA tensors required; there is no CPU path")
     if k_pages.dim() != 4 or k_pages.shape != v_pages.shape:
         raise ValueError(f"{what}: pages must be two (num_pages, kv_heads, page_size, head_dim) tensors of one shape; "
                          f"got {tuple(k_pages.shape)}, {tuple(v_pages.shape)}")
@@ -39,17 +39,6 @@ def _check_pages(what: str, x: torch.Tensor, k_pages: torch.Tensor, v_pages: tor
         raise ValueError(f"{what}: pages must have a unit inner stride (they are not copied)")
     if torch.is_grad_enabled() and (x.requires_grad or k_pages.requires_grad or v_pages.requires_grad):
         raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad()")
-
-
-def _check_devices(what: str, device: torch.device, *tensors: torch.Tensor) -> None:
-    for t in tensors:
-        if t.device != device:
-            raise RuntimeError(f"{what}: all tensors must be on {device}; got one on {t.device}")
-
-
-def _page_strides(t: torch.Tensor):
-    s = t.stride()
-    return _I64x4(s[0], s[1], s[2], 1)
 
 
 def paged_born_attention(
@@ -72,6 +61,7 @@ def paged_born_attention(
     keys all have zero weight) gives zeros.  Lengths past ``max_pages * page_size`` are cut to it, and a table
     entry outside the pages holds no keys.  What pages hold past a sequence's length is never used.
     """
+    index = same_device("paged_born_attention", q, k_pages, v_pages, block_table, seq_lens)
     _check_pages("paged_born_attention", q, k_pages, v_pages)
     if q.dim() != 3:
         raise ValueError(f"paged_born_attention: q must be (S, H, D); got {tuple(q.shape)}")
@@ -88,37 +78,34 @@ def paged_born_attention(
                          f"{seq_lens.dtype}")
     if not eps >= 0.0 or window_size < 0:
         raise ValueError(f"paged_born_attention: eps and window_size must not be negative; got {eps}, {window_size}")
-    device = q.device
-    _check_devices("paged_born_attention", device, k_pages, v_pages, block_table, seq_lens)
-    a = _lib.FbPagedArgs()
+    value, numel, scale_ptr = 0.0, 0, 0
     if isinstance(scale, torch.Tensor):
-        sc = scale.detach().reshape(-1).to(device=device, dtype=torch.float32).contiguous()
-        if sc.numel() not in (1, H):
-            raise ValueError(f"scale must have 1 or H={H} elements, got {sc.numel()}")
-        a.scale, a.scale_numel = sc.data_ptr(), sc.numel()
+        numel = scale.numel()
+        if numel != 1 and numel != H:
+            raise ValueError(f"scale must have 1 or H={H} elements, got {numel}")
+        if scale.dtype is not torch.float32 or scale.get_device() != index or not scale.is_contiguous():
+            scale = scale.detach().reshape(-1).to(device=q.device, dtype=torch.float32).contiguous()
+        scale_ptr = scale.data_ptr()
     else:
-        a.scale_value = float(scale)
-    qc = q if D == 1 or q.stride(2) == 1 else q.contiguous()
-    table = block_table if block_table.shape[1] <= 1 or block_table.stride(1) == 1 else block_table.contiguous()
-    lens = seq_lens.contiguous()
-    out = torch.empty((S, H, D), dtype=q.dtype, device=device)
-    a.seqs, a.heads, a.kv_heads, a.head_dim = S, H, Hkv, D
-    a.dtype = _DTYPE_CODE[q.dtype]
-    a.page_size, a.num_pages, a.max_pages = page, P, table.shape[1]
-    a.window_size, a.eps = int(window_size), float(eps)
-    s = qc.stride()
-    a.q, a.q_stride = qc.data_ptr(), _I64x3(s[0], s[1], 1)
-    a.k, a.k_stride = k_pages.data_ptr(), _page_strides(k_pages)
-    a.v, a.v_stride = v_pages.data_ptr(), _page_strides(v_pages)
-    a.out, a.out_stride = out.data_ptr(), _I64x3(H * D, D, 1)
-    a.table, a.table_stride, a.lens = table.data_ptr(), table.stride(0), lens.data_ptr()
+        value = float(scale)
+    if D > 1 and q.stride(2) != 1:
+        q = q.contiguous()
+    if block_table.shape[1] > 1 and block_table.stride(1) != 1:
+        block_table = block_table.contiguous()
+    if not seq_lens.is_contiguous():
+        seq_lens = seq_lens.contiguous()
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    qs, ks, vs = q.stride(), k_pages.stride(), v_pages.stride()
+    a = _paged_args(
+        S, H, Hkv, D, _DTYPE_CODE[q.dtype], page, P, block_table.shape[1], int(window_size), eps, value, numel, scale_ptr,
+        q.data_ptr(), qs[0], qs[1], 1, k_pages.data_ptr(), ks[0], ks[1], ks[2], 1, v_pages.data_ptr(), vs[0], vs[1], vs[2], 1,
+        out.data_ptr(), H * D, D, 1, block_table.data_ptr(), block_table.stride(0), seq_lens.data_ptr(), 0, 0)
     lib = _lib.load()
     need = lib.fb_paged_workspace_size(ctypes.byref(a))
     if need:
-        ws = torch.empty(need, dtype=torch.uint8, device=device)
+        ws = q.new_empty(need // q.element_size())
         a.workspace, a.workspace_bytes = ws.data_ptr(), need
-    with torch.cuda.device(device):
-        _lib.check(lib.fb_paged_born_fwd(ctypes.byref(a), _stream_handle(device)), "paged Born attention")
+    launch(lib.fb_paged_born_fwd, a, index, "paged Born attention")
     return out
 
 
@@ -143,6 +130,7 @@ def paged_qkv_write(
     gives NaN Q and K; two tokens must not share a slot.  ``return_kv=True`` also returns K and V
     ``(N, Hkv, D)``, for the prompt's own attention.  head_dim is even, up to 256.
     """
+    index = same_device("paged_qkv_write", qkv, k_pages, v_pages, cos, sin, positions, slots)
     _check_pages("paged_qkv_write", qkv, k_pages, v_pages)
     P, Hkv, page, D = k_pages.shape
     if qkv.dim() != 2 or D < 2 or D > 256 or D % 2 or Hkv < 1 or page < 1 or heads < 1 or heads % Hkv != 0 \
@@ -159,24 +147,25 @@ def paged_qkv_write(
                          f"{cos.dtype}, {tuple(sin.shape)} {sin.dtype}")
     if not eps >= 0.0:
         raise ValueError(f"paged_qkv_write: eps must not be negative; got {eps}")
-    device = qkv.device
-    _check_devices("paged_qkv_write", device, k_pages, v_pages, cos, sin, positions, slots)
-    x = qkv if qkv.stride(1) == 1 else qkv.contiguous()
-    cos, sin = cos.contiguous(), sin.contiguous()
-    positions, slots = positions.to(torch.int64).contiguous(), slots.to(torch.int64).contiguous()
-    q = torch.empty((N, heads, D), dtype=qkv.dtype, device=device)
-    a = _lib.FbPagedWriteArgs()
-    a.tokens, a.heads, a.kv_heads, a.head_dim = N, heads, Hkv, D
-    a.dtype = _DTYPE_CODE[qkv.dtype]
-    a.page_size, a.num_pages, a.rope_rows, a.eps = page, P, cos.shape[0], float(eps)
-    a.qkv, a.qkv_stride = x.data_ptr(), x.stride(0)
-    a.cos, a.sin, a.positions, a.slots = cos.data_ptr(), sin.data_ptr(), positions.data_ptr(), slots.data_ptr()
-    a.k, a.k_stride = k_pages.data_ptr(), _page_strides(k_pages)
-    a.v, a.v_stride = v_pages.data_ptr(), _page_strides(v_pages)
-    a.q = q.data_ptr()
+    if qkv.stride(1) != 1:
+        qkv = qkv.contiguous()
+    if not (cos.is_contiguous() and sin.is_contiguous()):
+        cos, sin = cos.contiguous(), sin.contiguous()
+    positions, slots = _int64(positions), _int64(slots)
+    q = qkv.new_empty((N, heads, D))
+    k = v = None
     if return_kv:
-        k, v = (torch.empty((N, Hkv, D), dtype=qkv.dtype, device=device) for _ in range(2))
-        a.k_out, a.v_out = k.data_ptr(), v.data_ptr()
-    with torch.cuda.device(device):
-        _lib.check(_lib.load().fb_paged_qkv_write(ctypes.byref(a), _stream_handle(device)), "paged QKV write")
+        k, v = qkv.new_empty((N, Hkv, D)), qkv.new_empty((N, Hkv, D))
+    ks, vs = k_pages.stride(), v_pages.stride()
+    a = _write_args(
+        N, heads, Hkv, D, _DTYPE_CODE[qkv.dtype], page, P, cos.shape[0], eps, qkv.data_ptr(), qkv.stride(0), cos.data_ptr(),
+        sin.data_ptr(), positions.data_ptr(), slots.data_ptr(), k_pages.data_ptr(), ks[0], ks[1], ks[2], 1, v_pages.data_ptr(),
+        vs[0], vs[1], vs[2], 1, q.data_ptr(), k.data_ptr() if return_kv else 0, v.data_ptr() if return_kv else 0)
+    launch(_lib.load().fb_paged_qkv_write, a, index, "paged QKV write")
     return (q, k, v) if return_kv else q
+
+
+def _int64(x: torch.Tensor) -> torch.Tensor:
+    if x.dtype is not torch.int64:
+        x = x.to(torch.int64)
+    return x if x.is_contiguous() else x.contiguous()
