@@ -207,6 +207,10 @@ __device__ __forceinline__ uint32_t ordered(float x) {
 // (value, column) as one number: the greater value first, then the lower column
 __device__ __forceinline__ uint64_t order_key(float x, int c) { return (uint64_t)ordered(x) << 32 | (uint32_t)~c; }
 __device__ __forceinline__ int key_column(uint64_t k) { return (int)~(uint32_t)k; }
+__device__ __forceinline__ float key_value(uint64_t k) {
+  const uint32_t u = (uint32_t)(k >> 32);
+  return __uint_as_float(u & 0x80000000u ? u & 0x7FFFFFFFu : ~u);
+}
 
 template <int THREADS> struct Shared {
   Sums warp[THREADS / 32];
@@ -299,9 +303,10 @@ __device__ void cta_top(const Row<T>& row, int j0, int j1, int K, float m, int a
   for (int i = threadIdx.x; i < K; i += THREADS) sh.top[i] = 0;
   // by chunk: the columns of a chunk share a key.  A maximum at the floor may stand for -inf.
   const uint64_t key = at >= 0 ? order_key(m <= Floor<T>::kFloor ? -INFINITY : m, at) : 0;
-  // at least K groups of neighbouring threads: a warp each or less
+  // four groups of neighbouring threads for each of the K, but at most 64 (and at least K): the more there are, the
+  // closer the K-th of their maxima comes to the K-th of all
   int width = 32;
-  while (THREADS / width < K) width /= 2;
+  while (THREADS / width < 64 && THREADS / width < 4 * K) width /= 2;
   const int groups = THREADS / width;
   uint64_t g = key;
   for (int o = 1; o < width; o <<= 1) g = max(g, __shfl_xor_sync(0xffffffffu, g, o));
@@ -358,6 +363,11 @@ __global__ void __launch_bounds__(THREADS, 1280 / THREADS) logprob_fwd_kernel(co
   const Row<T> row(static_cast<const T*>(p.x) + r * p.ld, p.V);
   int j0, j1;
   row.part_of(part, parts, j0, j1);
+  float target = NAN;  // thread 0 of the first part: the target's logit, asked for before all else
+  if (part == 0 && threadIdx.x == 0) {
+    const int64_t t = p.targets[r];
+    if (t >= 0 && t < p.V) target = to_f32(row.x[t]);
+  }
 
   Sums a{-1e30f, 0.f, 0.f};  // finite, and below every maximum that the fast path takes (kLowestMax)
   f32x2 s2 = f2_make(0.f, 0.f), u2 = s2;  // its sums, of even and of odd columns
@@ -419,8 +429,12 @@ __global__ void __launch_bounds__(THREADS, 1280 / THREADS) logprob_fwd_kernel(co
       for (int i = threadIdx.x; i < parts * p.K; i += THREADS)
         sh.merged[i] = cluster.map_shared_rank(sh.top, i / p.K)[i % p.K];
     }
-    cluster.sync();  // the others' shared memory has been read
-    if (part != 0) return;
+    // none leaves before the first has read its shared memory
+    asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");
+    if (part != 0) {
+      asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+      return;
+    }
     __syncthreads();
     rank_keys<THREADS>(sh.merged, parts * p.K, p.K, sh.candidate);
     __syncthreads();
@@ -433,20 +447,23 @@ __global__ void __launch_bounds__(THREADS, 1280 / THREADS) logprob_fwd_kernel(co
     if (p.K > 0) slow_top(row, 0, row.chunks, p.K, sh);
     top = sh.top;
   }
-  if (threadIdx.x > p.K) return;
-  const float ls = log2f(all.s);
-  auto logp_of = [&](float x) { return (x - all.m) - kLn2 * ls; };
-  if (threadIdx.x == 0) {
-    const int64_t t = p.targets[r];
-    p.stats[2 * r] = all.m;
-    p.stats[2 * r + 1] = ls;
-    p.logp[r] = t >= 0 && t < p.V ? logp_of(to_f32(row.x[t])) : NAN;
-    p.entropy[r] = kLn2 * (ls - all.u / all.s);
+  if (threadIdx.x <= p.K) {
+    const float ls = log2f(all.s);
+    auto logp_of = [&](float x) { return (x - all.m) - kLn2 * ls; };
+    if (threadIdx.x == 0) {
+      p.stats[2 * r] = all.m;
+      p.stats[2 * r + 1] = ls;
+      p.logp[r] = logp_of(target);
+      p.entropy[r] = kLn2 * (ls - all.u / all.s);
+    }
+    for (int i = threadIdx.x; i < p.K; i += THREADS) {
+      p.top_index[r * p.K + i] = key_column(top[i]);
+      p.top_logp[r * p.K + i] = logp_of(key_value(top[i]));
+    }
   }
-  for (int i = threadIdx.x; i < p.K; i += THREADS) {
-    const int c = key_column(top[i]);
-    p.top_index[r * p.K + i] = c;
-    p.top_logp[r * p.K + i] = logp_of(to_f32(row.x[c]));
+  if constexpr (CLUSTER) {
+    __syncthreads();
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
   }
 }
 
@@ -596,7 +613,7 @@ int sm_count() {
 int parts_of(const LogprobParams& p, int chunk, int most) {
   int parts = 1;
   const int64_t chunks = p.V / chunk + 1;
-  while (parts < most && p.rows * parts * 2 <= 4 * sm_count() && chunks >= 2 * parts * kFew) parts *= 2;
+  while (parts < most && p.rows * parts * 2 <= 2 * sm_count() && chunks >= 2 * parts * kFew) parts *= 2;
   return parts;
 }
 
