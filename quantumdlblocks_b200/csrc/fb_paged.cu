@@ -820,8 +820,8 @@ __device__ __forceinline__ void unpack16(const uint4& w, float (&f)[8], const __
 template <typename T, int LPH, int ACC>
 __global__ void __launch_bounds__(256) paged_write_vec(const WriteParams p, int per_token) {
   constexpr int N = 16 / sizeof(T), HPA = 32 / LPH;
-  const int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int64_t n = item / per_token;
+  const uint32_t item = blockIdx.x * 8 + (threadIdx.x >> 5);
+  const uint32_t n = item / (uint32_t)per_token;
   if (n >= p.N) return;
   const int lane = threadIdx.x & 31, sub = lane % LPH, heads = p.H + 2 * p.Hkv;
   const int h0 = (int)(item - n * per_token) * (HPA * ACC) + lane / LPH;
@@ -1185,7 +1185,7 @@ int paged_write(const fb_paged_write_args* a, cudaStream_t st) {
   const bool spread = p.N * accesses < 4 * 64 * (int64_t)sm_count();  // fewer warps than the SMs hold, at four accesses each
   const int per_token = spread ? accesses : (accesses + 3) / 4;
   const int64_t blocks = (p.N * per_token + 7) / 8;
-  if (blocks > 0x7FFFFFFF) return FB_ERR_SHAPE;
+  if (blocks > 0x1FFFFFFF) return FB_ERR_SHAPE;  // warps count in 32 bits
   if (a->dtype == FB_F32) launch_write<float>(p, lanes, spread, per_token, (unsigned)blocks, st);
   else if (a->dtype == FB_F16) launch_write<__half>(p, lanes, spread, per_token, (unsigned)blocks, st);
   else launch_write<__nv_bfloat16>(p, lanes, spread, per_token, (unsigned)blocks, st);
