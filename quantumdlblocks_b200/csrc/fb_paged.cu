@@ -777,109 +777,116 @@ __device__ __forceinline__ bool slot_of_token(const WriteParams& p, int64_t n, i
   return stored;
 }
 
-// Where head h's row of token n goes: its place in the cache (or q), and its copy.
-template <typename T> struct Targets {
-  T *to, *copy;
-  bool put;
-  __device__ Targets(const WriteParams& p, int64_t n, int h, int pg, int row, bool stored) {
-    copy = nullptr;
-    put = stored;
-    if (h < p.H) {
-      to = static_cast<T*>(p.q) + (n * p.H + h) * p.D;
-      put = true;
-    } else {
-      const bool is_v = h >= p.H + p.Hkv;
-      const int kvh = h - p.H - (is_v ? p.Hkv : 0);
-      to = is_v ? static_cast<T*>(p.v) + pg * p.vs[0] + kvh * p.vs[1] + row * p.vs[2]
-                : static_cast<T*>(p.k) + pg * p.ks[0] + kvh * p.ks[1] + row * p.ks[2];
-      void* c = is_v ? p.v_out : p.k_out;
-      if (c) copy = static_cast<T*>(c) + (n * p.Hkv + kvh) * p.D;
-    }
-  }
-};
-
-__device__ __forceinline__ void unpack16(const uint4& w, float (&f)[4], const float*) {
-  f[0] = __uint_as_float(w.x), f[1] = __uint_as_float(w.y), f[2] = __uint_as_float(w.z), f[3] = __uint_as_float(w.w);
+// A 16-byte piece as fp32 pairs, and back rounded
+__device__ __forceinline__ void unpack_pairs(const uint4& w, sm100::f32x2 (&f)[2], const float*) {
+  f[0] = sm100::f2_make(__uint_as_float(w.x), __uint_as_float(w.y));
+  f[1] = sm100::f2_make(__uint_as_float(w.z), __uint_as_float(w.w));
 }
-__device__ __forceinline__ void unpack16(const uint4& w, float (&f)[8], const __nv_bfloat16*) {
+__device__ __forceinline__ void unpack_pairs(const uint4& w, sm100::f32x2 (&f)[4], const __nv_bfloat16*) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f[i] = sm100::f2_make(sm100::bf16_lo((&w.x)[i]), sm100::bf16_hi((&w.x)[i]));
+}
+__device__ __forceinline__ void unpack_pairs(const uint4& w, sm100::f32x2 (&f)[4], const __half*) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f[i] = sm100::f2_make(half_lo((&w.x)[i]), half_hi((&w.x)[i]));
+}
+__device__ __forceinline__ uint4 pack_pairs(const sm100::f32x2 (&f)[2], const float*) {
+  return make_uint4(__float_as_uint(sm100::f2_lo(f[0])), __float_as_uint(sm100::f2_hi(f[0])),
+                    __float_as_uint(sm100::f2_lo(f[1])), __float_as_uint(sm100::f2_hi(f[1])));
+}
+__device__ __forceinline__ uint4 pack_pairs(const sm100::f32x2 (&f)[4], const __nv_bfloat16*) {
+  return make_uint4(sm100::f2_bf16(f[0]), sm100::f2_bf16(f[1]), sm100::f2_bf16(f[2]), sm100::f2_bf16(f[3]));
+}
+__device__ __forceinline__ uint4 pack_pairs(const sm100::f32x2 (&f)[4], const __half*) {
+  uint4 w;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    f[2 * i] = __uint_as_float((&w.x)[i] << 16);
-    f[2 * i + 1] = __uint_as_float((&w.x)[i] & 0xFFFF0000u);
+    const __half2 v = __floats2half2_rn(sm100::f2_lo(f[i]), sm100::f2_hi(f[i]));
+    (&w.x)[i] = *reinterpret_cast<const uint32_t*>(&v);
   }
-}
-__device__ __forceinline__ void unpack16(const uint4& w, float (&f)[8], const __half*) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) f[2 * i] = half_lo((&w.x)[i]), f[2 * i + 1] = half_hi((&w.x)[i]);
+  return w;
 }
 
-// Rows of 8, 16 or 32 16-byte pieces on 16-byte boundaries: LPH lanes a head, 32 / LPH heads an access, ACC
-// accesses a warp, all of one token.  The turn's other half of a piece is LPH / 2 lanes away (one exchange of
-// the raw words), the norm a sum over the head's lanes.  Reads and writes every element once: HBM bandwidth
-// bounds it, latency for a batch's new tokens (ACC = 1 spreads them over more warps).
+// Rows of 8, 16 or 32 16-byte pieces on 16-byte boundaries: LPH lanes a head, 32 / LPH heads an access; a warp
+// makes `accesses` of them, all of one token, ACC at a time.  The turn's other half of a piece is LPH / 2 lanes
+// away (one exchange of the raw words), the norm a sum over the head's lanes.  Reads and writes every element
+// once: HBM bandwidth bounds it, and for a batch's new tokens latency (one access a warp spreads them over more).
 template <typename T, int LPH, int ACC>
-__global__ void __launch_bounds__(256) paged_write_vec(const WriteParams p, int per_token) {
+__global__ void __launch_bounds__(256) paged_write_vec(const WriteParams p, int warps_per_token, int accesses) {
+  using namespace sm100;
   constexpr int N = 16 / sizeof(T), HPA = 32 / LPH;
   const uint32_t item = blockIdx.x * 8 + (threadIdx.x >> 5);
-  const uint32_t n = item / (uint32_t)per_token;
+  const uint32_t n = item / (uint32_t)warps_per_token;
   if (n >= p.N) return;
   const int lane = threadIdx.x & 31, sub = lane % LPH, heads = p.H + 2 * p.Hkv;
-  const int h0 = (int)(item - n * per_token) * (HPA * ACC) + lane / LPH;
+  const int first = (int)(item - n * warps_per_token) * accesses * HPA, last = min(first + accesses * HPA, heads);
   const T* x = static_cast<const T*>(p.qkv) + n * p.ld + sub * N;
   uint4 w[ACC];
+  auto load = [&](int at) {  // heads at + lane / LPH, ...
 #pragma unroll
-  for (int i = 0; i < ACC; ++i) {
-    const int h = h0 + i * HPA;
-    w[i] = make_uint4(0, 0, 0, 0);
-    if (h < heads) w[i] = *reinterpret_cast<const uint4*>(x + (int64_t)h * p.D);
-  }
+    for (int i = 0; i < ACC; ++i) {
+      const int h = at + i * HPA + lane / LPH;
+      w[i] = make_uint4(0, 0, 0, 0);
+      if (h < last) w[i] = *reinterpret_cast<const uint4*>(x + (int64_t)h * p.D);
+    }
+  };
+  load(first);
   int pg, row;
   const bool stored = slot_of_token(p, n, pg, row);
   const int64_t pos = p.positions[n];
   const bool known = pos >= 0 && pos < p.rope_rows;
-  float c[N], s[N];
+  f32x2 c[N / 2], s[N / 2];
   {
     const int64_t at = (known ? pos : 0) * (p.D / 2) + (sub % (LPH / 2)) * N;
+    const float sign = sub < LPH / 2 ? -1.f : 1.f;  // first half: a cos - b sin; second: b cos + a sin
 #pragma unroll
     for (int e = 0; e < N; e += 4) {
       const float4 a = known ? *reinterpret_cast<const float4*>(p.cos + at + e) : make_float4(NAN, NAN, NAN, NAN);
       const float4 b = known ? *reinterpret_cast<const float4*>(p.sin + at + e) : make_float4(NAN, NAN, NAN, NAN);
-      c[e] = a.x, c[e + 1] = a.y, c[e + 2] = a.z, c[e + 3] = a.w;
-      s[e] = b.x, s[e + 1] = b.y, s[e + 2] = b.z, s[e + 3] = b.w;
-    }
-    if (sub < LPH / 2) {  // first half: a cos - b sin; second: b cos + a sin
-#pragma unroll
-      for (int e = 0; e < N; ++e) s[e] = -s[e];
+      c[e / 2] = f2_make(a.x, a.y), c[e / 2 + 1] = f2_make(a.z, a.w);
+      s[e / 2] = f2_make(sign * b.x, sign * b.y), s[e / 2 + 1] = f2_make(sign * b.z, sign * b.w);
     }
   }
+  T* q = static_cast<T*>(p.q) + (int64_t)n * p.H * p.D + sub * N;
+  T* kp = static_cast<T*>(p.k) + pg * p.ks[0] + row * p.ks[2] + sub * N;
+  T* vp = static_cast<T*>(p.v) + pg * p.vs[0] + row * p.vs[2] + sub * N;
+  const int64_t copy = (int64_t)n * p.Hkv * p.D + sub * N;
+  for (int at = first; at < last; at += ACC * HPA) {
+    if (at != first) load(at);
 #pragma unroll
-  for (int i = 0; i < ACC; ++i) {
-    const int h = h0 + i * HPA;
-    uint4 o;
+    for (int i = 0; i < ACC; ++i) {
+      const int h = at + i * HPA + lane / LPH;
+      uint4 out = w[i];
+      if (at + i * HPA < p.H + p.Hkv) {  // the same for the whole warp: some of its heads are Q or K
+        uint4 o;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) (&o.x)[e] = __shfl_xor_sync(0xffffffffu, (&w[i].x)[e], LPH / 2);
-    float f[N], g[N], ss = 0.f;
-    unpack16(w[i], f, static_cast<const T*>(nullptr));
-    unpack16(o, g, static_cast<const T*>(nullptr));
+        for (int e = 0; e < 4; ++e) (&o.x)[e] = __shfl_xor_sync(0xffffffffu, (&out.x)[e], LPH / 2);
+        f32x2 f[N / 2], g[N / 2], ss = f2_make(0.f, 0.f);
+        unpack_pairs(out, f, static_cast<const T*>(nullptr));
+        unpack_pairs(o, g, static_cast<const T*>(nullptr));
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-      f[e] = f[e] * c[e] + g[e] * s[e];
-      ss = fmaf(f[e], f[e], ss);
+        for (int e = 0; e < N / 2; ++e) {
+          f[e] = f2_fma(f[e], c[e], f2_mul(g[e], s[e]));
+          ss = f2_fma(f[e], f[e], ss);
+        }
+        float sum = f2_lo(ss) + f2_hi(ss);
+#pragma unroll
+        for (int d = LPH / 2; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        const float r = rsqrtf(sum + p.eps);
+#pragma unroll
+        for (int e = 0; e < N / 2; ++e) f[e] = f2_mul(f[e], f2_make(r, r));
+        if (h < p.H + p.Hkv) out = pack_pairs(f, static_cast<const T*>(nullptr));
+      }
+      if (h < p.H) {
+        if (h < last) *reinterpret_cast<uint4*>(q + (int64_t)h * p.D) = out;
+      } else if (h < last) {
+        const bool is_v = h >= p.H + p.Hkv;
+        const int kvh = h - p.H - (is_v ? p.Hkv : 0);
+        if (stored) *reinterpret_cast<uint4*>(is_v ? vp + kvh * p.vs[1] : kp + kvh * p.ks[1]) = out;
+        if (p.k_out)
+          *reinterpret_cast<uint4*>(static_cast<T*>(is_v ? p.v_out : p.k_out) + copy + (int64_t)kvh * p.D) = out;
+      }
     }
-#pragma unroll
-    for (int d = LPH / 2; d > 0; d >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
-    if (h >= heads) continue;
-    uint4 out = w[i];
-    if (h < p.H + p.Hkv) {
-      const float r = rsqrtf(ss + p.eps);
-      T t[N];
-#pragma unroll
-      for (int e = 0; e < N; ++e) t[e] = from_f32<T>(f[e] * r);
-      memcpy(&out, t, 16);
-    }
-    const Targets<T> to(p, n, h, pg, row, stored);
-    if (to.put) *reinterpret_cast<uint4*>(to.to + sub * N) = out;
-    if (to.copy) *reinterpret_cast<uint4*>(to.copy + sub * N) = out;
   }
 }
 
@@ -895,11 +902,19 @@ __global__ void __launch_bounds__(256) paged_write_general(const WriteParams p) 
   int pg, row;
   const bool stored = slot_of_token(p, n, pg, row);
   const int64_t pos = p.positions[n];
-  const Targets<T> to(p, n, h, pg, row, stored);
-  if (h >= p.H + p.Hkv) {
+  // where the head's row goes: q or its place in the cache, and its copy
+  const bool is_v = h >= p.H + p.Hkv;
+  const int kvh = h - p.H - (is_v ? p.Hkv : 0);
+  T *to = static_cast<T*>(p.q) + (n * p.H + h) * p.D, *copy = nullptr;
+  if (h >= p.H) {
+    const int64_t* st = is_v ? p.vs : p.ks;
+    to = stored ? static_cast<T*>(is_v ? p.v : p.k) + pg * st[0] + kvh * st[1] + row * st[2] : nullptr;
+    if (p.k_out) copy = static_cast<T*>(is_v ? p.v_out : p.k_out) + (n * p.Hkv + kvh) * p.D;
+  }
+  if (is_v) {
     for (int d = lane; d < p.D; d += 32) {
-      if (to.put) to.to[d] = x[d];
-      if (to.copy) to.copy[d] = x[d];
+      if (to) to[d] = x[d];
+      if (copy) copy[d] = x[d];
     }
     return;
   }
@@ -921,8 +936,8 @@ __global__ void __launch_bounds__(256) paged_write_general(const WriteParams p) 
     const int d = lane + 32 * i;
     if (d >= half) continue;
     const T lo = from_f32<T>(a[i] * r), hi = from_f32<T>(b[i] * r);
-    if (to.put) to.to[d] = lo, to.to[d + half] = hi;
-    if (to.copy) to.copy[d] = lo, to.copy[d + half] = hi;
+    if (to) to[d] = lo, to[d + half] = hi;
+    if (copy) copy[d] = lo, copy[d + half] = hi;
   }
 }
 
@@ -1134,15 +1149,15 @@ int paged_fwd(const fb_paged_args* a, cudaStream_t st) {
 }
 
 template <typename T, int LPH>
-void launch_write(const WriteParams& p, bool spread, int per_token, unsigned blocks, cudaStream_t st) {
-  if (spread) paged_write_vec<T, LPH, 1><<<blocks, 256, 0, st>>>(p, per_token);
-  else paged_write_vec<T, LPH, 4><<<blocks, 256, 0, st>>>(p, per_token);
+void launch_write(const WriteParams& p, int warps, int each, unsigned blocks, cudaStream_t st) {
+  if (each == 1) paged_write_vec<T, LPH, 1><<<blocks, 256, 0, st>>>(p, warps, each);
+  else paged_write_vec<T, LPH, 4><<<blocks, 256, 0, st>>>(p, warps, each);
 }
 template <typename T>
-void launch_write(const WriteParams& p, int lanes, bool spread, int per_token, unsigned blocks, cudaStream_t st) {
-  if (lanes == 8) launch_write<T, 8>(p, spread, per_token, blocks, st);
-  else if (lanes == 16) launch_write<T, 16>(p, spread, per_token, blocks, st);
-  else launch_write<T, 32>(p, spread, per_token, blocks, st);
+void launch_write(const WriteParams& p, int lanes, int warps, int each, unsigned blocks, cudaStream_t st) {
+  if (lanes == 8) launch_write<T, 8>(p, warps, each, blocks, st);
+  else if (lanes == 16) launch_write<T, 16>(p, warps, each, blocks, st);
+  else launch_write<T, 32>(p, warps, each, blocks, st);
 }
 
 int paged_write(const fb_paged_write_args* a, cudaStream_t st) {
@@ -1182,13 +1197,14 @@ int paged_write(const fb_paged_write_args* a, cudaStream_t st) {
     return launched(1);
   }
   const int accesses = (p.H + 2 * p.Hkv + 32 / lanes - 1) / (32 / lanes);
-  const bool spread = p.N * accesses < 4 * 64 * (int64_t)sm_count();  // fewer warps than the SMs hold, at four accesses each
-  const int per_token = spread ? accesses : (accesses + 3) / 4;
-  const int64_t blocks = (p.N * per_token + 7) / 8;
+  // a warp to each access while those are fewer than four per warp that the SMs hold, else to each token
+  const bool spread = p.N * accesses < 4 * 64 * (int64_t)sm_count();
+  const int warps = spread ? accesses : 1, each = spread ? 1 : accesses;
+  const int64_t blocks = (p.N * warps + 7) / 8;
   if (blocks > 0x1FFFFFFF) return FB_ERR_SHAPE;  // warps count in 32 bits
-  if (a->dtype == FB_F32) launch_write<float>(p, lanes, spread, per_token, (unsigned)blocks, st);
-  else if (a->dtype == FB_F16) launch_write<__half>(p, lanes, spread, per_token, (unsigned)blocks, st);
-  else launch_write<__nv_bfloat16>(p, lanes, spread, per_token, (unsigned)blocks, st);
+  if (a->dtype == FB_F32) launch_write<float>(p, lanes, warps, each, (unsigned)blocks, st);
+  else if (a->dtype == FB_F16) launch_write<__half>(p, lanes, warps, each, (unsigned)blocks, st);
+  else launch_write<__nv_bfloat16>(p, lanes, warps, each, (unsigned)blocks, st);
   return launched(1);
 }
 
