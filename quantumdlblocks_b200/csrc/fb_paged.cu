@@ -812,7 +812,7 @@ __device__ __forceinline__ uint4 pack_pairs(const sm100::f32x2 (&f)[4], const __
 // away (one exchange of the raw words), the norm a sum over the head's lanes.  Reads and writes every element
 // once: HBM bandwidth bounds it, and for a batch's new tokens latency (one access a warp spreads them over more).
 template <typename T, int LPH, int ACC>
-__global__ void __launch_bounds__(256) paged_write_vec(const WriteParams p, int warps_per_token, int accesses) {
+__global__ void __launch_bounds__(256, 4) paged_write_vec(const WriteParams p, int warps_per_token, int accesses) {
   using namespace sm100;
   constexpr int N = 16 / sizeof(T), HPA = 32 / LPH;
   const uint32_t item = blockIdx.x * 8 + (threadIdx.x >> 5);
