@@ -580,20 +580,40 @@ template <> struct Piece<__half, 8> {
   }
 };
 
-// Lane (r, c) takes key r of 8 and the pieces c, c + 4, ... of its row (VEC elements each, E = NI VEC of
-// them, E at least D / 4): a dot product is finished by two shuffles among four lanes, the four have the
-// weight, and each adds it times its own part of the value row.  The eight keys' sums meet at the end of the
-// piece, the CTA's warps' too.  HU query heads share a read of the row; a kv head with more is several units.
-template <typename T, int VEC, int NI, int HU>
-__global__ void __launch_bounds__(kThreads) paged_born_general(const PagedParams p) {
-  constexpr int E = NI * VEC;
+// Shapes of the CUDA-core kernel: 16 elements of a row per lane (NI pieces of VEC), LANES lanes per row, so up
+// to 64, 128 or 256 dimensions; for pieces of 16 bytes a ring of copies, kStages steps of kKeys keys per warp.
+template <typename T, int VEC, int LANES> struct GenShape {
+  static constexpr int E = 16, NI = E / VEC;
+  static constexpr int kKeys = 32 / LANES;
+  static constexpr bool kRing = VEC * sizeof(T) == 16;
+  static constexpr int kStages = 3;
+  static constexpr int kStageBytes = kRing ? 2 * NI * 512 : 0;
+  static constexpr int kRingBytes = kWarps * kStages * kStageBytes;
+  static constexpr int kCtasPerSm = kRing ? 4 : 3;
+};
+
+// Lane (r, c) takes key r of kKeys and the pieces c, c + LANES, ... of its row: a dot product is finished by
+// shuffles among LANES lanes, which all have the weight then, and each adds it times its own part of the value
+// row.  The keys' sums meet at the end of the piece, the CTA's warps' too.  HU query heads share a read of the
+// row; a kv head with more is several units.  Every lane reads back only what it copied: no barrier in the loop.
+template <typename T, int VEC, int LANES, int HU>
+__global__ void __launch_bounds__(kThreads, (GenShape<T, VEC, LANES>::kCtasPerSm))
+    paged_born_general(const PagedParams p) {
+  using Sh = GenShape<T, VEC, LANES>;
+  using namespace sm100;
+  constexpr int E = Sh::E, NI = Sh::NI, kStep = kWarps * Sh::kKeys, kDims = E * LANES, kGroup = VEC == 1 ? 4 : VEC;
   extern __shared__ __align__(16) uint8_t smem_raw[];
   __shared__ uint32_t pre[kThreads];
   __shared__ float rz[kWarps * HU];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane / LANES, c = lane % LANES;
   const int ld = p.D + 4;
-  float* red = reinterpret_cast<float*>(smem_raw);  // [kWarps][HU][ld]
-  float* qsm = red + kWarps * HU * ld;              // [HU][4 E] queries, piece i of lane c at (i * 4 + c) VEC
+  uint8_t* ring = smem_raw + warp * Sh::kStages * Sh::kStageBytes + lane * 16;
+  const uint32_t ring_s = sm100::smem_u32(ring);
+  // a warp's sums at the end of a piece, [HU][ld], lie over its ring
+  float* red = reinterpret_cast<float*>(smem_raw);
+  const int red_warp = Sh::kRing ? Sh::kStages * Sh::kStageBytes / 4 : HU * ld;
+  static_assert(!Sh::kRing || HU * (kDims + 4) * 4 <= Sh::kStages * Sh::kStageBytes, "they fit");
+  float* qsm = red + kWarps * red_warp;  // [HU][kDims] queries
 
   asm volatile("griddepcontrol.launch_dependents;");
   const int per = tile_prefix<kThreads>(p, pre);
@@ -605,8 +625,47 @@ __global__ void __launch_bounds__(kThreads) paged_born_general(const PagedParams
     const int32_t* table = p.table + w.s * p.table_stride;
     const T* kbase = static_cast<const T*>(p.k) + kvh * p.ks[1];
     const T* vbase = static_cast<const T*>(p.v) + kvh * p.vs[1];
-    for (int i = threadIdx.x; i < HU * 4 * E; i += kThreads) {
-      const int h = i / (4 * E), d = i % (4 * E);
+    const int end = w.end_key(p), first = w.first_key(p) + warp * Sh::kKeys;
+    const int n = end > first ? (end - first + kStep - 1) / kStep : 0;  // this warp's steps
+    // page and row of the lane's key in step i; false where it has none
+    auto find = [&](int i, int& pg, int& row) {
+      const int key = first + i * kStep + r;
+      pg = -1, row = 0;
+      if (i < n && key >= w.k.lo && key < end) {
+        const int x = key / p.page;
+        pg = table[x];
+        row = key - x * p.page;
+        if (pg >= p.pages) pg = -1;
+      }
+    };
+    auto issue = [&](int i, int pg, int row) {
+      if (i < n) {
+        const uint32_t to = ring_s + (i % Sh::kStages) * Sh::kStageBytes;
+        const T* k = pg >= 0 ? kbase + pg * p.ks[0] + row * p.ks[2] : kbase;
+        const T* v = pg >= 0 ? vbase + pg * p.vs[0] + row * p.vs[2] : vbase;
+#pragma unroll
+        for (int x = 0; x < NI; ++x) {
+          const int d = (x * LANES + c) * VEC;
+          const bool ok = pg >= 0 && d < p.D;
+          copy16(to + x * 512, k + (ok ? d : 0), ok);
+          copy16(to + (NI + x) * 512, v + (ok ? d : 0), ok);
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    int pg, row;          // of the next step to be asked for (of the current one, without a ring)
+    uint32_t counts = 0;  // bit i % 32: the lane's key of step i counts
+    if constexpr (Sh::kRing) {
+#pragma unroll
+      for (int i = 0; i < Sh::kStages - 1; ++i) {
+        find(i, pg, row);
+        counts |= (pg >= 0 ? 1u : 0u) << i;
+        issue(i, pg, row);
+      }
+      find(Sh::kStages - 1, pg, row);
+    }
+    for (int i = threadIdx.x; i < HU * kDims; i += kThreads) {
+      const int h = i / kDims, d = i % kDims;
       qsm[i] = h < nh && d < p.D ? to_f32(static_cast<const T*>(p.q)[w.s * p.qs[0] + (head0 + h) * p.qs[1] + d]) : 0.f;
     }
     float sc[HU];
@@ -614,63 +673,116 @@ __global__ void __launch_bounds__(kThreads) paged_born_general(const PagedParams
     for (int h = 0; h < HU; ++h)
       sc[h] = h < nh ? (p.scale ? p.scale[p.scale_per_head ? head0 + h : 0] : p.scale_value) : 0.f;
     __syncthreads();
-    float o[HU][E], z[HU];
+    f32x2 o[HU][E / 2];
+    float z[HU];
 #pragma unroll
     for (int h = 0; h < HU; ++h) {
       z[h] = 0.f;
 #pragma unroll
-      for (int e = 0; e < E; ++e) o[h][e] = 0.f;
+      for (int e = 0; e < E / 2; ++e) o[h][e] = f2_make(0.f, 0.f);
     }
-    const int end = w.end_key(p);
-    for (int key0 = w.first_key(p) + warp * 8; key0 < end; key0 += kWarps * 8) {
-      const int key = key0 + r;
-      int pg = -1, row = 0;
-      if (key >= w.k.lo && key < end) {
-        const int i = key / p.page;
-        pg = table[i];
-        row = key - i * p.page;
+    for (int i = 0; i < n; ++i) {
+      const uint8_t* stage = ring + (i % Sh::kStages) * Sh::kStageBytes;
+      const T *k = kbase, *v = vbase;
+      bool here;
+      if constexpr (Sh::kRing) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(Sh::kStages - 2) : "memory");
+        here = counts >> (i & 31) & 1;
+      } else {
+        find(i, pg, row);
+        here = pg >= 0;
+        if (here) k += pg * p.ks[0] + row * p.ks[2], v += pg * p.vs[0] + row * p.vs[2];
       }
-      const bool counts = pg >= 0 && pg < p.pages;
-      float kf[NI][VEC], vf[NI][VEC];
-#pragma unroll
-      for (int i = 0; i < NI; ++i) {
-        const int d = (i * 4 + c) * VEC;
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) kf[i][e] = vf[i][e] = 0.f;
-        if (counts && d < p.D) {
-          Piece<T, VEC>::load(kbase + pg * p.ks[0] + row * p.ks[2] + d, kf[i]);
-          Piece<T, VEC>::load(vbase + pg * p.vs[0] + row * p.vs[2] + d, vf[i]);
+      // the lane's piece x of its key (at = 0) or value (at = 1)
+      auto piece = [&](int at, int x, float (&f)[VEC]) {
+        if constexpr (Sh::kRing) {
+          Piece<T, VEC>::load(reinterpret_cast<const T*>(stage + (at * NI + x) * 512), f);
+        } else {
+          const int d = (x * LANES + c) * VEC;
+          f[0] = 0.f;
+          if (here && d < p.D) Piece<T, VEC>::load((at ? v : k) + d, f);
         }
+      };
+      // kGroup of them at a time
+      auto group = [&](int at, int x, float (&f)[kGroup]) {
+        if constexpr (VEC == kGroup) {
+          piece(at, x, f);
+        } else {
+#pragma unroll
+          for (int e = 0; e < kGroup; ++e) {
+            float one[VEC];
+            piece(at, x * kGroup + e, one);
+            f[e] = one[0];
+          }
+        }
+      };
+      auto dim = [&](int e) { return (e / VEC * LANES + c) * VEC + e % VEC; };  // of the lane's element e
+      // sums of pairs of dimensions, two at a time for each head: one would wait for itself
+      f32x2 dot[HU][2];
+      float wt[HU];
+#pragma unroll
+      for (int h = 0; h < HU; ++h) dot[h][0] = dot[h][1] = f2_make(0.f, 0.f);
+#pragma unroll
+      for (int x = 0; x < E / kGroup; ++x) {
+        float f[kGroup];
+        group(0, x, f);
+#pragma unroll
+        for (int h = 0; h < HU; ++h)
+#pragma unroll
+          for (int e = 0; e < kGroup; e += 4) {
+            const float* at = qsm + h * kDims + dim(x * kGroup + e);
+            float4 q;
+            if constexpr (VEC > 1) q = *reinterpret_cast<const float4*>(at);
+            else q = make_float4(at[0], at[LANES], at[2 * LANES], at[3 * LANES]);
+            dot[h][0] = f2_fma(f2_make(q.x, q.y), f2_make(f[e], f[e + 1]), dot[h][0]);
+            dot[h][1] = f2_fma(f2_make(q.z, q.w), f2_make(f[e + 2], f[e + 3]), dot[h][1]);
+          }
       }
 #pragma unroll
       for (int h = 0; h < HU; ++h) {
-        float dot = 0.f;
+        const f32x2 both = f2_add(dot[h][0], dot[h][1]);
+        wt[h] = f2_lo(both) + f2_hi(both);
 #pragma unroll
-        for (int i = 0; i < NI; ++i)
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) dot = fmaf(qsm[h * 4 * E + (i * 4 + c) * VEC + e], kf[i][e], dot);
-        dot += __shfl_xor_sync(0xffffffffu, dot, 1);
-        dot += __shfl_xor_sync(0xffffffffu, dot, 2);
-        const float a = relu(dot * sc[h]);
-        const float wt = counts ? a * a : 0.f;
-        z[h] += wt;
-#pragma unroll
-        for (int i = 0; i < NI; ++i)
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) o[h][i * VEC + e] = fmaf(wt, vf[i][e], o[h][i * VEC + e]);
+        for (int x = 1; x < LANES; x <<= 1) wt[h] += __shfl_xor_sync(0xffffffffu, wt[h], x);
+        const float a = relu(wt[h] * sc[h]);
+        wt[h] = here ? a * a : 0.f;
+        z[h] += wt[h];
       }
+#pragma unroll
+      for (int x = 0; x < E / kGroup; ++x) {
+        float f[kGroup];
+        group(1, x, f);
+#pragma unroll
+        for (int h = 0; h < HU; ++h)
+#pragma unroll
+          for (int e = 0; e < kGroup; e += 2) {
+            f32x2& to = o[h][(x * kGroup + e) / 2];
+            to = f2_fma(f2_make(wt[h], wt[h]), f2_make(f[e], f[e + 1]), to);
+          }
+      }
+      if constexpr (Sh::kRing) {
+        const int next = i + Sh::kStages - 1;
+        counts = (counts & ~(1u << (next & 31))) | (pg >= 0 ? 1u : 0u) << (next & 31);
+        issue(next, pg, row);  // over the stage that this lane read in the previous step
+        find(next + 1, pg, row);
+      }
+    }
+    if constexpr (Sh::kRing) {
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      __syncwarp();  // every lane has read its last stage before the sums go over the ring
     }
 #pragma unroll
     for (int h = 0; h < HU; ++h) {
 #pragma unroll
-      for (int x = 4; x < 32; x <<= 1) z[h] += __shfl_xor_sync(0xffffffffu, z[h], x);
+      for (int x = LANES; x < 32; x <<= 1) z[h] += __shfl_xor_sync(0xffffffffu, z[h], x);
       if (lane == 0) rz[warp * HU + h] = z[h];
 #pragma unroll
       for (int e = 0; e < E; ++e) {
+        float sum = e & 1 ? f2_hi(o[h][e / 2]) : f2_lo(o[h][e / 2]);
 #pragma unroll
-        for (int x = 4; x < 32; x <<= 1) o[h][e] += __shfl_xor_sync(0xffffffffu, o[h][e], x);
-        const int d = (e / VEC * 4 + c) * VEC + e % VEC;
-        if (r == 0 && d < p.D) red[(warp * HU + h) * ld + d] = o[h][e];
+        for (int x = LANES; x < 32; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+        const int d = (e / VEC * LANES + c) * VEC + e % VEC;
+        if (r == 0 && d < p.D) red[warp * red_warp + h * ld + d] = sum;
       }
     }
     __syncthreads();
@@ -682,7 +794,7 @@ __global__ void __launch_bounds__(kThreads) paged_born_general(const PagedParams
       for (int d = threadIdx.x; d < p.D; d += kThreads) {
         float os = 0.f;
 #pragma unroll
-        for (int x = 0; x < kWarps; ++x) os += red[(x * HU + h) * ld + d];
+        for (int x = 0; x < kWarps; ++x) os += red[x * red_warp + h * ld + d];
         if (w.whole())
           (static_cast<T*>(p.out) + w.s * p.os[0] + (head0 + h) * p.os[1])[d] =
               from_f32<T>(zs == 0.f ? 0.f : os / (zs + p.eps));
@@ -989,6 +1101,11 @@ struct PagedPlan {
   size_t workspace;
 };
 
+template <typename T> int general_ctas_per_sm(const PagedPlan& pl) {
+  constexpr int V = 16 / sizeof(T);
+  return pl.vec == 1 ? GenShape<T, 1, 4>::kCtasPerSm : GenShape<T, V, 4>::kCtasPerSm;
+}
+
 PagedPlan plan_paged(const fb_paged_args* a) {
   PagedPlan pl{};
   const int G = a->heads / a->kv_heads, size = a->dtype == FB_F32 ? 4 : 2;
@@ -999,7 +1116,7 @@ PagedPlan plan_paged(const fb_paged_args* a) {
   pl.pack = G <= 8;
   pl.vec = rows16 ? 16 / size : 1;
   pl.size_class = a->head_dim <= 64 ? 0 : a->head_dim <= 128 ? 1 : 2;
-  pl.HU = pl.tc ? (pl.pack ? 8 : 16) : 4 >> pl.size_class;
+  pl.HU = pl.tc ? (pl.pack ? 8 : 16) : pl.vec > 1 && G <= 2 ? G : 4;
   pl.chunks = (G + pl.HU - 1) / pl.HU;
   // The most keys a unit can have: the table's capacity, or the window and what its start is rounded down by
   int64_t cap = (int64_t)a->page_size * a->max_pages;
@@ -1012,7 +1129,9 @@ PagedPlan plan_paged(const fb_paged_args* a) {
   while (units * ((cap + tile - 1) / tile) > 0x7FFFFFFF) tile *= 2;
   pl.tile = (int)std::min<int64_t>(tile, 1 << 30);
   const int64_t tiles = units * std::max<int64_t>((cap + tile - 1) / tile, 1);
-  const int per_sm = pl.tc ? kWarps * (a->head_dim == 64 ? TcShape<64>::kCtasPerSm : TcShape<128>::kCtasPerSm) : 4;
+  // one wave of them
+  const int per_sm = pl.tc ? kWarps * (a->head_dim == 64 ? TcShape<64>::kCtasPerSm : TcShape<128>::kCtasPerSm)
+                     : size == 4 ? general_ctas_per_sm<float>(pl) : general_ctas_per_sm<__half>(pl);
   pl.W = (uint32_t)std::min<int64_t>(tiles, pl.join ? (int64_t)per_sm * sm_count() : 0x7FFFFFFF);
   pl.workspace = pl.join ? (size_t)pl.W * 2 * pl.HU * (a->head_dim + 1) * sizeof(float) : 0;
   return pl;
@@ -1037,21 +1156,29 @@ int check_paged(const fb_paged_args* a) {
   return FB_OK;
 }
 
+template <typename T, int VEC, int LANES, int HU>
+cudaError_t launch_general(const PagedParams& p, cudaStream_t st) {
+  using Sh = GenShape<T, VEC, LANES>;
+  const int sums = Sh::kRing ? Sh::kRingBytes : kWarps * HU * (p.D + 4) * (int)sizeof(float);
+  const int smem = sums + HU * LANES * Sh::E * (int)sizeof(float);
+  const auto kernel = &paged_born_general<T, VEC, LANES, HU>;
+  const cudaError_t e = set_smem_limit_once(reinterpret_cast<const void*>(kernel), smem);
+  if (e != cudaSuccess) return e;
+  kernel<<<p.W, kThreads, smem, st>>>(p);
+  return cudaGetLastError();
+}
+template <typename T, int VEC, int HU>
+cudaError_t launch_general(const PagedParams& p, const PagedPlan& pl, cudaStream_t st) {
+  if (pl.size_class == 0) return launch_general<T, VEC, 4, HU>(p, st);
+  if (pl.size_class == 1) return launch_general<T, VEC, 8, HU>(p, st);
+  return launch_general<T, VEC, 16, HU>(p, st);
+}
 template <typename T>
 cudaError_t launch_general(const PagedParams& p, const PagedPlan& pl, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T);
-  const int smem = (kWarps * p.HU * (p.D + 4) + p.HU * (64 << pl.size_class)) * (int)sizeof(float);
-  const dim3 grid(p.W), block(kThreads);
-  if (pl.vec > 1) {
-    if (pl.size_class == 0) paged_born_general<T, V, 16 / V, 4><<<grid, block, smem, st>>>(p);
-    else if (pl.size_class == 1) paged_born_general<T, V, 32 / V, 2><<<grid, block, smem, st>>>(p);
-    else paged_born_general<T, V, 64 / V, 1><<<grid, block, smem, st>>>(p);
-  } else {
-    if (pl.size_class == 0) paged_born_general<T, 1, 16, 4><<<grid, block, smem, st>>>(p);
-    else if (pl.size_class == 1) paged_born_general<T, 1, 32, 2><<<grid, block, smem, st>>>(p);
-    else paged_born_general<T, 1, 64, 1><<<grid, block, smem, st>>>(p);
-  }
-  return cudaGetLastError();
+  if (pl.vec == 1) return launch_general<T, 1, 4>(p, pl, st);
+  if (pl.HU == 1) return launch_general<T, V, 1>(p, pl, st);
+  return pl.HU == 2 ? launch_general<T, V, 2>(p, pl, st) : launch_general<T, V, 4>(p, pl, st);
 }
 
 // TMA maps of the pages, (B, H, T, D) = (page, kv head, row, dimension); false where TMA cannot take them:
