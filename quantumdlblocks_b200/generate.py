@@ -1,0 +1,199 @@
+"""Generating from the flash-Born GPT, scoring what it said, and a policy-gradient step on it.
+
+    python -m quantumdlblocks_b200.generate
+
+runs all three on a small random model.  The pieces are the package's own operators:
+
+* the prompts, packed into one row whatever their lengths, go through the training path's
+  ``flash_born_attention`` (document ids keep them apart) while ``paged_qkv_write`` fills the cache;
+* a step of all sequences' next tokens is ``paged_qkv_write`` + ``paged_born_attention`` per layer, then
+  ``token_logprobs`` of what was chosen;
+* ``policy_step`` differentiates ``token_logprobs`` over whole rows and clips with ``clip_grad_norm_``.
+"""
+from __future__ import annotations
+
+from typing import NamedTuple, Optional, Sequence
+
+import torch
+import torch.nn.functional as F
+
+from .gpt import BornGPT
+from .kernels.flash_born import flash_born_attention
+from .kernels.gradclip import clip_grad_norm_
+from .kernels.logprobs import token_logprobs
+from .kernels.paged import paged_born_attention, paged_qkv_write
+from .kernels.prologue import l2_normalize
+
+__all__ = ["Generation", "PagedKVCache", "PolicyStep", "generate", "policy_step"]
+
+
+class PagedKVCache:
+    """Key and value pages of all layers, and which of them each sequence has.
+
+    Every sequence gets the pages for ``capacities[s]`` tokens at once; ``pages`` is one tensor,
+    ``(layers, 2, num_pages, heads, page_size, head_dim)``, and its keys and values of a layer are what the
+    operators take.
+    """
+
+    def __init__(self, layers: int, heads: int, head_dim: int, capacities: Sequence[int], dtype: torch.dtype,
+                 device: torch.device, page_size: int = 64):
+        counts = [-(-c // page_size) for c in capacities]
+        self.page_size, self.capacities = page_size, list(capacities)
+        self.pages = torch.empty((layers, 2, sum(counts), heads, page_size, head_dim), dtype=dtype, device=device)
+        table = torch.full((len(counts), max(counts, default=0)), -1, dtype=torch.int32)
+        start = 0
+        for s, n in enumerate(counts):
+            table[s, :n] = torch.arange(start, start + n, dtype=torch.int32)
+            start += n
+        self.table = table.to(device)
+        self.lens = torch.zeros(len(counts), dtype=torch.int32, device=device)
+
+    def slots(self, seqs: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
+        """Cache slots of tokens at ``positions`` of sequences ``seqs`` (int64, both of one shape)."""
+        page = self.table[seqs, positions // self.page_size].to(torch.int64)
+        return page * self.page_size + positions % self.page_size
+
+    def layer(self, i: int) -> tuple[torch.Tensor, torch.Tensor]:
+        return self.pages[i, 0], self.pages[i, 1]
+
+
+class Generation(NamedTuple):
+    tokens: torch.Tensor  # (S, n) int64
+    logp: torch.Tensor  # (S, n) fp32, of the chosen tokens
+    entropy: torch.Tensor  # (S, n) fp32
+    top_logp: torch.Tensor  # (S, n, top_k) fp32
+    top_index: torch.Tensor  # (S, n, top_k) int64
+
+
+def _block(blk, x: torch.Tensor, attend) -> torch.Tensor:
+    """One transformer block on rows ``(N, d)``; ``attend(attn, qkv)`` gives the heads' outputs ``(N, d)``."""
+    attn = blk.attn
+    x = x + attn.out(attend(attn, attn.qkv(l2_normalize(x, attn.eps))))
+    return x + blk.proj(F.gelu(blk.fc(blk.norm(x)), approximate="tanh"))
+
+
+def _scale(attn) -> torch.Tensor:
+    return torch.clamp(attn.head_scale, min=1.0, max=100.0)
+
+
+def generate(model: BornGPT, prompts: Sequence[torch.Tensor], new_tokens: int, temperature: float = 0.0, top_k: int = 0,
+             generator: Optional[torch.Generator] = None, autocast_dtype: Optional[torch.dtype] = torch.bfloat16,
+             page_size: int = 64) -> Generation:
+    """``new_tokens`` for each of ``prompts`` (1-D int64 tensors, one token or more, of any lengths).
+
+    ``temperature`` 0 takes the likeliest token, else samples from ``softmax(logits / temperature)``; the log
+    probabilities, entropy and ``top_k`` alternatives returned are the model's own (temperature 1).  Positions
+    go up to the model's ``seq_len``.
+    """
+    cfg, device = model.cfg, model.emb.weight.device
+    if device.type != "cuda" or not model.native_loss:
+        raise RuntimeError("generate (B200): a CUDA model with the native attention is required; there is no CPU path")
+    lens = [int(p.numel()) for p in prompts]
+    if not lens or min(lens) < 1 or new_tokens < 1:
+        raise ValueError(f"generate takes one prompt or more, of one token or more, and new_tokens >= 1; got lengths "
+                         f"{lens}, new_tokens={new_tokens}")
+    if max(lens) + new_tokens > cfg.seq_len:
+        raise ValueError(f"{max(lens)} prompt tokens + {new_tokens} new ones exceed the model's {cfg.seq_len} positions")
+    S, H, hd = len(lens), cfg.n_heads, cfg.d_model // cfg.n_heads
+    cache = PagedKVCache(cfg.n_layers, H, hd, [n + new_tokens for n in lens], autocast_dtype or model.emb.weight.dtype,
+                         device, page_size)
+    counts = torch.tensor(lens, device=device)
+    seqs = torch.repeat_interleave(torch.arange(S, device=device), counts)
+    ends = counts.cumsum(0)
+    positions = torch.arange(int(sum(lens)), device=device) - torch.repeat_interleave(ends - counts, counts)
+    tokens = torch.cat([p.reshape(-1).to(device=device, dtype=torch.int64) for p in prompts])
+    got: list[list[torch.Tensor]] = [[], [], [], [], []]
+
+    with torch.no_grad(), torch.autocast("cuda", dtype=autocast_dtype, enabled=autocast_dtype is not None):
+        # the prompts as one packed row
+        slots, docs = cache.slots(seqs, positions), seqs.to(torch.int32)[None]
+        x = model.emb(tokens)
+        for i, blk in enumerate(model.blocks):
+            def attend(attn, qkv, i=i):
+                q, k, v = (y.transpose(0, 1)[None] for y in paged_qkv_write(
+                    qkv, attn.cos, attn.sin, positions, slots, *cache.layer(i), H, attn.eps, return_kv=True))
+                o = flash_born_attention(q, k, v, _scale(attn), is_causal=True, eps=attn.eps, doc_ids=docs, token_major=True)
+                return o.transpose(1, 2).reshape(-1, cfg.d_model)
+
+            x = _block(blk, x, attend)
+        cache.lens += counts.to(torch.int32)
+        x = x[ends - 1]
+        every = torch.arange(S, device=device)
+        for step in range(new_tokens):
+            logits = model.head(x)
+            if temperature > 0.0:
+                noise = torch.empty(logits.shape, dtype=torch.float32, device=device).exponential_(generator=generator)
+                chosen = (logits.float() / temperature - noise.log()).argmax(dim=1)
+                r = token_logprobs(logits, chosen, top_k)
+            else:
+                chosen = torch.argmax(logits, dim=1)
+                r = token_logprobs(logits, chosen, top_k)
+            for to, y in zip(got, (chosen, *r)):
+                to.append(y)
+            if step + 1 == new_tokens:
+                break
+            at = cache.lens.to(torch.int64)  # the chosen tokens' positions
+            slots = cache.slots(every, at)
+            cache.lens += 1
+            x = model.emb(chosen)
+            for i, blk in enumerate(model.blocks):
+                def attend(attn, qkv, i=i):
+                    q = paged_qkv_write(qkv, attn.cos, attn.sin, at, slots, *cache.layer(i), H, attn.eps)
+                    return paged_born_attention(q, *cache.layer(i), cache.table, cache.lens, _scale(attn),
+                                                eps=attn.eps).view(S, cfg.d_model)
+
+                x = _block(blk, x, attend)
+    return Generation(*(torch.stack(y, dim=1) for y in got))
+
+
+class PolicyStep(NamedTuple):
+    loss: torch.Tensor
+    entropy: torch.Tensor  # mean over the tokens that count
+    grad_norm: torch.Tensor  # before clipping
+
+
+def policy_step(model: BornGPT, opt: torch.optim.Optimizer, tokens: torch.Tensor, advantages: torch.Tensor,
+                entropy_weight: float = 0.0, max_norm: float = 1.0,
+                autocast_dtype: Optional[torch.dtype] = torch.bfloat16) -> PolicyStep:
+    """One policy-gradient step: ``-(mean of advantage * logp + entropy_weight * entropy)`` over the tokens of
+    ``tokens (B, T + 1)`` whose ``advantages (B, T)`` (of token t + 1 at t) are not 0, gradients clipped to ``max_norm``."""
+    inp, tgt = tokens[:, :-1], tokens[:, 1:].reshape(-1)
+    adv = advantages.reshape(-1).to(torch.float32)
+    counts = (adv != 0).to(torch.float32)
+    n = counts.sum().clamp_min(1.0)
+    with torch.autocast("cuda", dtype=autocast_dtype, enabled=autocast_dtype is not None):
+        logits = model.logits(inp)
+    r = token_logprobs(logits, tgt)
+    entropy = (counts * r.entropy).sum() / n
+    loss = -(adv * r.logp).sum() / n - entropy_weight * entropy
+    loss.backward()
+    norm = clip_grad_norm_([p.grad for p in model.parameters() if p.grad is not None], max_norm)
+    opt.step()
+    opt.zero_grad(set_to_none=True)
+    return PolicyStep(loss.detach(), entropy.detach(), norm)
+
+
+def main() -> None:
+    from .gpt import GPTConfig
+
+    torch.manual_seed(0)
+    cfg = GPTConfig(vocab_size=211, d_model=256, n_layers=2, n_heads=4, seq_len=128)
+    model = BornGPT(cfg).cuda()
+    opt = torch.optim.SGD(model.parameters(), lr=0.5)
+    prompts = [torch.randint(0, cfg.vocab_size, (n,)) for n in (1, 7, 30)]
+    for step in range(3):
+        g = generate(model, prompts, 24, temperature=1.0, top_k=3)
+        reward = (g.tokens % 2 == 0).float()  # what is asked for here: even tokens
+        tokens = torch.zeros((len(prompts), max(p.numel() for p in prompts) + 24), dtype=torch.int64, device="cuda")
+        adv = torch.zeros((len(prompts), tokens.shape[1] - 1), device="cuda")
+        for s, p in enumerate(prompts):
+            n = p.numel()
+            tokens[s, :n], tokens[s, n:n + 24] = p.cuda(), g.tokens[s]
+            adv[s, n - 1:n + 23] = reward[s] - 0.5
+        r = policy_step(model, opt, tokens, adv, entropy_weight=0.01)
+        print(f"step {step}: {float(reward.mean()):.2f} even, logp {float(g.logp.mean()):.3f}, entropy "
+              f"{float(g.entropy.mean()):.3f}, loss {float(r.loss):.4f}, gradient norm {float(r.grad_norm):.3f}")
+
+
+if __name__ == "__main__":
+    main()

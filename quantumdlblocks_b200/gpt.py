@@ -135,13 +135,20 @@ class BornGPT(nn.Module):
         self.blocks = nn.ModuleList(Block(cfg, attention, fused) for _ in range(cfg.n_layers))
         self.norm = nn.RMSNorm(cfg.d_model)
 
-    def forward(self, tokens: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
+    def head(self, x: torch.Tensor) -> torch.Tensor:
+        """Logits of hidden states ``(..., d_model)``: ``(rows, padded vocabulary)``, the padded columns at -inf."""
+        h = self.norm(x)
+        logits = F.linear(h, self.emb.weight, self.logit_mask.to(h.dtype))  # tied head, padded rows at -inf
+        return logits.view(-1, logits.shape[-1])
+
+    def logits(self, tokens: torch.Tensor) -> torch.Tensor:
         x = self.emb(tokens)
         for blk in self.blocks:
             x = blk(x)
-        h = self.norm(x)
-        logits = F.linear(h, self.emb.weight, self.logit_mask.to(h.dtype))  # tied head, padded rows at -inf
-        logits = logits.view(-1, logits.shape[-1])
+        return self.head(x)
+
+    def forward(self, tokens: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
+        logits = self.logits(tokens)
         if self.native_loss and logits.is_cuda and logits.dtype == torch.bfloat16:
             from .kernels.xent import cross_entropy
 
@@ -179,13 +186,19 @@ def make_ddp(model: nn.Module, device: torch.device, bucket_mb: float = 25.0):
 
 
 def train_step(model: nn.Module, opt: torch.optim.Optimizer, tokens: torch.Tensor,
-               autocast_dtype: Optional[torch.dtype] = torch.bfloat16) -> torch.Tensor:
-    """One optimiser step on ``tokens`` ``(B, T + 1)``; returns the loss (a device tensor)."""
+               autocast_dtype: Optional[torch.dtype] = torch.bfloat16, max_norm: Optional[float] = None) -> torch.Tensor:
+    """One optimiser step on ``tokens`` ``(B, T + 1)``; returns the loss (a device tensor).
+
+    ``max_norm`` clips the gradients' global norm first (CUDA models: ``clip_grad_norm_``)."""
     inp, tgt = tokens[:, :-1], tokens[:, 1:]
     dev_type = tokens.device.type
     with torch.autocast(dev_type, dtype=autocast_dtype, enabled=autocast_dtype is not None):
         loss = model(inp, tgt)
     loss.backward()
+    if max_norm is not None:
+        from .kernels.gradclip import clip_grad_norm_
+
+        clip_grad_norm_([p.grad for p in model.parameters() if p.grad is not None], max_norm)
     opt.step()
     opt.zero_grad(set_to_none=True)
     return loss.detach()

@@ -1,0 +1,152 @@
+"""GPU: generation from the flash-Born GPT against the model run over the whole text again, packed and ragged
+prompts against each alone, and a policy-gradient step against the same step of torch's operators."""
+from __future__ import annotations
+
+import copy
+
+import pytest
+import torch
+
+from quantumdlblocks_b200.generate import PagedKVCache, generate, policy_step
+from quantumdlblocks_b200.gpt import BornGPT, GPTConfig, train_step, zipf_tokens
+from quantumdlblocks_b200.kernels import flash_born as fbm
+from test_gpt_cpu import born_eager
+
+pytestmark = pytest.mark.gpu
+
+if not torch.cuda.is_available():
+    pytest.skip("CUDA device required", allow_module_level=True)
+
+CFG = GPTConfig(vocab_size=211, d_model=256, n_layers=2, n_heads=4, seq_len=160)
+
+
+def make_model(seed=0):
+    torch.manual_seed(seed)
+    model = BornGPT(CFG).cuda()
+    with torch.no_grad():  # logits with some spread: a fresh embedding's are all alike
+        model.emb.weight.mul_(2.0)  # the tied head's logits reach about 10
+    return model
+
+
+def prompts_of(lens, seed=3):
+    g = torch.Generator().manual_seed(seed)
+    return [torch.randint(0, CFG.vocab_size, (n,), generator=g) for n in lens]
+
+
+def again(model, prompt, said, dtype):
+    """Log-softmax rows (fp32) of the tokens `said` after `prompt`, from the whole text at once."""
+    text = torch.cat([prompt.cuda(), said])[None, :-1]
+    with torch.no_grad(), torch.autocast("cuda", dtype=dtype, enabled=dtype is not None):
+        logits = model.logits(text).float()
+    return torch.log_softmax(logits, dim=1)[prompt.numel() - 1:]
+
+
+@pytest.mark.parametrize("dtype,tol", [(None, 1e-3), (torch.bfloat16, 0.15)], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("temperature", [0.0, 1.0])
+def test_generate_agrees_with_the_whole_text(dtype, tol, temperature):
+    """fp32: two orders of fp32 sums through two layers; bf16: activations of a unit-scale residual stream round at
+    2^-8 on either path, logits of size ~10 differ by a few such roundings."""
+    model = make_model()
+    prompts = prompts_of([1, 37, 64, 100])
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    g = generate(model, prompts, 50, temperature=temperature, top_k=5, generator=gen, autocast_dtype=dtype, page_size=16)
+    assert g.tokens.shape == (4, 50) and g.top_index.shape == (4, 50, 5)
+    assert int(g.tokens.max()) < CFG.vocab_size  # never a padded row of the head
+    for s, p in enumerate(prompts):
+        ls = again(model, p, g.tokens[s], dtype)
+        assert float((ls.gather(1, g.tokens[s][:, None])[:, 0] - g.logp[s]).abs().max()) <= tol
+        prob = ls.exp()
+        ent = -torch.where(prob > 0, prob * ls, torch.zeros_like(ls)).sum(1)
+        assert float((ent - g.entropy[s]).abs().max()) <= tol * 4
+        assert float((ls.topk(5).values - g.top_logp[s]).abs().max()) <= tol
+        if temperature == 0.0:
+            assert torch.equal(g.tokens[s], g.top_index[s, :, 0])
+            if dtype is None:  # the likeliest token again, but where two are as likely
+                best = ls.topk(2).values
+                clear = best[:, 0] - best[:, 1] > 4 * tol
+                assert torch.equal(ls.argmax(1)[clear], g.tokens[s][clear]) and clear.float().mean() > 0.5
+    assert fbm.device_status() == (0, 0)
+
+
+def test_prompts_packed_or_alone():
+    model = make_model(1)
+    prompts = prompts_of([3, 90, 17])
+    together = generate(model, prompts, 20, autocast_dtype=None)
+    for s, p in enumerate(prompts):
+        alone = generate(model, [p], 20, autocast_dtype=None, page_size=32)
+        assert torch.equal(alone.tokens[0], together.tokens[s])
+        torch.testing.assert_close(alone.logp[0], together.logp[s], rtol=0, atol=1e-3)
+
+
+def test_sampling_follows_the_generator():
+    model = make_model(2)
+    prompts = prompts_of([5, 6])
+    a, b, c = (generate(model, prompts, 12, temperature=1.0, generator=torch.Generator(device="cuda").manual_seed(x))
+               for x in (1, 1, 2))
+    assert torch.equal(a.tokens, b.tokens) and not torch.equal(a.tokens, c.tokens)
+
+
+def test_cache_pages_are_disjoint():
+    cache = PagedKVCache(1, 2, 8, [1, 64, 65, 130], torch.float32, torch.device("cuda"), page_size=64)
+    used = cache.table[cache.table >= 0]
+    assert used.numel() == 1 + 1 + 2 + 3 == cache.pages.shape[2] and used.unique().numel() == used.numel()
+    seqs = torch.tensor([3, 3, 2], device="cuda")
+    pos = torch.tensor([0, 129, 64], device="cuda")
+    assert cache.slots(seqs, pos).tolist() == [4 * 64, 6 * 64 + 1, 3 * 64]
+
+
+def test_policy_step_matches_torch():
+    """The native model's step against the eager attention's with torch's log-softmax and clipping, from the same
+    weights: fp32, plain gradient descent, a clipped norm."""
+    torch.manual_seed(0)
+    ref = BornGPT(CFG, attention=born_eager).cuda()
+    model = BornGPT(CFG).cuda()
+    model.load_state_dict(copy.deepcopy(ref.state_dict()))
+    tokens = torch.from_numpy(zipf_tokens(3, 65, CFG.vocab_size, seed=4)).cuda()
+    adv = torch.randn(3, 65, generator=torch.Generator().manual_seed(5)).cuda()
+    adv[:, :10] = 0  # the prompt
+    lr, most, weight = 0.5, 0.05, 0.02
+    got = policy_step(model, torch.optim.SGD(model.parameters(), lr=lr), tokens, adv, weight, most, autocast_dtype=None)
+    ls = torch.log_softmax(ref.logits(tokens[:, :-1]), dim=1)
+    p = ls.exp()
+    logp = ls.gather(1, tokens[:, 1:].reshape(-1, 1))[:, 0]
+    ent = -torch.where(p > 0, p * ls.clamp_min(-1e4), torch.zeros_like(p)).sum(1)
+    m = (adv.reshape(-1) != 0).float()
+    entropy = (m * ent).sum() / m.sum()
+    loss = -(adv.reshape(-1) * logp).sum() / m.sum() - weight * entropy
+    opt = torch.optim.SGD(ref.parameters(), lr=lr)
+    loss.backward()
+    norm = torch.nn.utils.clip_grad_norm_(ref.parameters(), most)
+    opt.step()
+    assert float(norm) > 2 * most  # the step is a clipped one
+    torch.testing.assert_close(got.loss, loss.detach(), rtol=1e-4, atol=1e-5)
+    torch.testing.assert_close(got.entropy, entropy.detach(), rtol=1e-4, atol=1e-5)
+    torch.testing.assert_close(got.grad_norm, norm.detach(), rtol=1e-3, atol=1e-6)
+    # a clipped step moves all parameters together by lr * most: agreement is asked for within 1 % of that
+    for (name, a), (_, b) in zip(model.named_parameters(), ref.named_parameters()):
+        assert float((a - b).detach().norm()) <= 0.01 * lr * most, name
+
+
+def test_train_step_clips():
+    torch.manual_seed(0)
+    a = BornGPT(CFG).cuda()
+    b = copy.deepcopy(a)
+    tokens = torch.from_numpy(zipf_tokens(2, 64, CFG.vocab_size, seed=1)).cuda()
+    before = torch.cat([p.detach().reshape(-1).clone() for p in a.parameters()])
+    train_step(a, torch.optim.SGD(a.parameters(), lr=1.0), tokens, autocast_dtype=None, max_norm=1e-3)
+    moved = torch.cat([p.detach().reshape(-1) for p in a.parameters()]) - before
+    assert abs(float(moved.norm()) - 1e-3) <= 2e-5  # lr 1: the step is the clipped gradient
+    la = train_step(b, torch.optim.SGD(b.parameters(), lr=1.0), tokens, autocast_dtype=None, max_norm=1e9)
+    assert torch.isfinite(la)
+
+
+def test_refusals():
+    model = make_model()
+    p = prompts_of([4])
+    for bad in (([], 3), ([p[0][:0]], 3), (p, 0), (prompts_of([150]), 11)):
+        with pytest.raises(ValueError):
+            generate(model, *bad)
+    with pytest.raises(RuntimeError):
+        generate(BornGPT(CFG, attention=born_eager).cuda(), p, 3)
+    with pytest.raises(RuntimeError):
+        generate(BornGPT(CFG), p, 3)
