@@ -100,15 +100,15 @@ template <typename T, int N> struct Span {
   }
 };
 
-// The tensor that holds a chunk (the last that starts at or before it: tensors without elements have none)
-__device__ __forceinline__ int tensor_of(const ClipParams& p, uint32_t chunk) {
-  int a = 0, b = p.count;  // t[a].chunk0 <= chunk, t[b].chunk0 > chunk
-  while (b - a > 1) {
-    const int m = (a + b) / 2;
-    if (p.t[m].chunk0 <= chunk) a = m;
-    else b = m;
+// The tensor that holds a chunk, searched from the one that held an earlier (or, DOWN, a later) chunk
+template <bool DOWN>
+__device__ __forceinline__ int tensor_of(const ClipParams& p, uint32_t chunk, int from) {
+  if (DOWN) {
+    while (p.t[from].chunk0 > chunk) --from;
+  } else {
+    while (from + 1 < p.count && p.t[from + 1].chunk0 <= chunk) ++from;
   }
-  return a;
+  return from;
 }
 
 template <typename T>
@@ -141,8 +141,10 @@ __device__ __forceinline__ double block_sum(double d) {
 __global__ void __launch_bounds__(kThreads, kCtasPerSm) clip_sum(const __grid_constant__ ClipParams p) {
   asm volatile("griddepcontrol.launch_dependents;");
   double sum = 0.0;
+  int at = 0;
   for (uint32_t chunk = blockIdx.x; chunk < p.chunks; chunk += gridDim.x) {
-    const Tensor& t = p.t[tensor_of(p, chunk)];
+    at = tensor_of<false>(p, chunk, at);
+    const Tensor& t = p.t[at];
     if (t.dtype == FB_F32) sum += squares<float>(t, chunk);
     else if (t.dtype == FB_BF16) sum += squares<__nv_bfloat16>(t, chunk);
     else sum += squares<__half>(t, chunk);
@@ -189,9 +191,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) clip_scale(const __grid_
   float c = p.max_norm / (norm + p.eps);
   if (c >= 1.f) c = 1.f;  // a NaN norm stays NaN
   if (c == 1.f && p.in_place) return;
+  int at = p.count - 1;
   for (uint32_t i = blockIdx.x; i < p.chunks; i += gridDim.x) {
     const uint32_t chunk = p.chunks - 1 - i;
-    const Tensor& t = p.t[tensor_of(p, chunk)];
+    at = tensor_of<true>(p, chunk, at);
+    const Tensor& t = p.t[at];
     if (t.dtype == FB_F32) scale<float, float>(t, chunk, c);
     else if (t.dtype == FB_BF16 && t.out_dtype == FB_BF16) scale<__nv_bfloat16, __nv_bfloat16>(t, chunk, c);
     else if (t.dtype == FB_BF16) scale<__nv_bfloat16, float>(t, chunk, c);
