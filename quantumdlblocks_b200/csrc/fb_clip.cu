@@ -3,7 +3,7 @@
 //   norm = sqrt(sum g^2),  c = min(1, max_norm / (norm + eps)),  out = c g
 //
 // Two kernels, whatever the tensors' number and types.  All tensors' elements are cut into chunks of
-// kChunkBytes, the table of tensors travels in the kernel's parameters (kTensors to a launch; more take
+// kSumBytes or kScaleBytes, the table of tensors travels in the kernel's parameters (kTensors to a launch; more take
 // more launches), and CTA b of a launch takes chunks b, b + grid, ...:
 //
 //   clip_sum    each CTA's sum of squares: fp32 for the 16 or 32 squares of a thread and chunk, fp64 beyond
@@ -20,22 +20,29 @@
 #include <type_traits>
 
 #include "fb_common.cuh"
+#include "fb_sm100.cuh"
 
 namespace fb {
 namespace {
 
+using namespace sm100;  // packed fp32 pairs
+
 constexpr int kThreads = 256;
-constexpr int kUnroll = 4;                                // 16-byte loads a thread has under way
-constexpr int kChunkBytes = kThreads * kUnroll * 16;      // 16 KB
-constexpr int kTensors = 96;                              // per launch: the table stays under 4 KB
-constexpr int kCtasPerSm = 6;
+// The summing kernel takes 16 KB at a time (four 16-byte loads under way per thread), the scaling one, whose
+// stores want more CTAs than loads want bytes, 8 KB (127 M fp32 summed: 85 us, with 8 KB 91; 40 M bf16 into
+// fp32: 59 us, with 16 KB 61)
+constexpr int kSumBytes = 16 * 1024, kSumCtas = 6;      // per chunk; CTAs per SM
+constexpr int kScaleBytes = 8 * 1024, kScaleCtas = 8;
+constexpr int kTensors = 96;                            // per launch: the table stays under 4 KB
 
 struct Tensor {
   const void* g;
   void* out;
   int64_t n;
-  uint32_t chunk0;    // its first chunk in the launch
+  uint32_t chunk0;        // its first chunk in the launch
+  uint32_t full0, fulls;  // chunks [full0, full0 + fulls) of the launch are wholly its own
   uint8_t dtype, out_dtype;
+  bool out_aligned;       // element 0 of the first vector would be stored to a 16-byte boundary
 };
 
 struct ClipParams {
@@ -50,53 +57,65 @@ struct ClipParams {
 };
 static_assert(sizeof(ClipParams) <= 4096, "kernel parameters");
 
-// Elements of a chunk: vectors of N elements of memory from the 16-byte boundary at or before the tensor, so that
-// every load is aligned; the tensor's first and last vector may be partly its own.
-template <typename T, int N> struct Span {
+__device__ __forceinline__ void unpack(const uint4& w, f32x2 (&f)[2], const float*) {
+  f[0] = f2_make(__uint_as_float(w.x), __uint_as_float(w.y));
+  f[1] = f2_make(__uint_as_float(w.z), __uint_as_float(w.w));
+}
+template <typename W, int P>
+__device__ __forceinline__ void unpack(const W& w, f32x2 (&f)[P], const __nv_bfloat16*) {
+#pragma unroll
+  for (int i = 0; i < P; ++i) f[i] = f2_make(bf16_lo((&w.x)[i]), bf16_hi((&w.x)[i]));
+}
+template <typename W, int P>
+__device__ __forceinline__ void unpack(const W& w, f32x2 (&f)[P], const __half*) {
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    const uint32_t b = (&w.x)[i];
+    const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&b));
+    f[i] = f2_make(v.x, v.y);
+  }
+}
+
+// A chunk's vectors of N elements, counted from the 16-byte boundary at or before the tensor, so that every load
+// is aligned; the tensor's first and last vector may be partly its own.
+template <typename T, int N, int BYTES> struct Span {
   using W = typename std::conditional<N * sizeof(T) == 16, uint4, uint2>::type;
-  static constexpr int kVectors = kChunkBytes / sizeof(W), kEach = kVectors / kThreads;  // of a chunk, of a thread
-  const T* base;
-  int64_t lo, hi;  // the tensor's elements from there
+  static constexpr int kVectors = BYTES / sizeof(W), kEach = kVectors / kThreads;  // of a chunk, of a thread
+  const Tensor& t;
+  int shift;       // the tensor's first element, from the boundary
   int64_t v0;      // the thread's first vector
   bool full;       // the whole chunk is the tensor's
-  __device__ Span(const Tensor& t, uint32_t chunk) {
-    const int shift = (int)((reinterpret_cast<uintptr_t>(t.g) & 15) / sizeof(T));
-    base = static_cast<const T*>(t.g) - shift;
-    lo = shift;
-    hi = shift + t.n;
-    v0 = (int64_t)(chunk - t.chunk0) * kVectors;
-    full = v0 * N >= lo && (v0 + kVectors) * N <= hi;
-    v0 += threadIdx.x;
+  __device__ Span(const Tensor& tensor, uint32_t chunk) : t(tensor) {
+    shift = (int)((reinterpret_cast<uintptr_t>(t.g) & 15) / sizeof(T));
+    v0 = (int64_t)(chunk - t.chunk0) * kVectors + threadIdx.x;
+    full = chunk - t.full0 < t.fulls;
   }
-  __device__ const W* at(int i) const { return reinterpret_cast<const W*>(base) + v0 + i * kThreads; }
-  __device__ bool has(int64_t element) const { return element >= lo && element < hi; }
-  // the thread's vectors as floats, 0 where the tensor has none
-  __device__ void load(float (&f)[kEach][N]) const {
+  __device__ const T* base() const { return static_cast<const T*>(t.g) - shift; }
+  __device__ bool has(int64_t element) const { return element >= shift && element < shift + t.n; }
+  // the thread's vectors as pairs of floats, 0 where the tensor has none
+  __device__ void load(f32x2 (&f)[kEach][N / 2]) const {
+    const W* from = reinterpret_cast<const W*>(base()) + v0;
     W w[kEach];
     if (full) {
 #pragma unroll
-      for (int i = 0; i < kEach; ++i) w[i] = *at(i);
+      for (int i = 0; i < kEach; ++i) w[i] = from[i * kThreads];
     } else {
 #pragma unroll
       for (int i = 0; i < kEach; ++i) {
         const int64_t e0 = (v0 + i * kThreads) * N;
         if (has(e0) && has(e0 + N - 1)) {
-          w[i] = *at(i);
+          w[i] = from[i * kThreads];
         } else {
           w[i] = W{};
           T* e = reinterpret_cast<T*>(&w[i]);
 #pragma unroll
           for (int x = 0; x < N; ++x)
-            if (has(e0 + x)) e[x] = base[e0 + x];
+            if (has(e0 + x)) e[x] = base()[e0 + x];
         }
       }
     }
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      const T* e = reinterpret_cast<const T*>(&w[i]);
-#pragma unroll
-      for (int x = 0; x < N; ++x) f[i][x] = to_f32(e[x]);
-    }
+    for (int i = 0; i < kEach; ++i) unpack(w[i], f[i], static_cast<const T*>(nullptr));
   }
 };
 
@@ -114,15 +133,15 @@ __device__ __forceinline__ int tensor_of(const ClipParams& p, uint32_t chunk, in
 template <typename T>
 __device__ __forceinline__ float squares(const Tensor& t, uint32_t chunk) {
   constexpr int N = 16 / sizeof(T);
-  using S = Span<T, N>;
+  using S = Span<T, N, kSumBytes>;
   const S s(t, chunk);
-  float f[S::kEach][N], sum = 0.f;
+  f32x2 f[S::kEach][N / 2], sum = f2_make(0.f, 0.f);
   s.load(f);
 #pragma unroll
   for (int i = 0; i < S::kEach; ++i)
 #pragma unroll
-    for (int e = 0; e < N; ++e) sum = fmaf(f[i][e], f[i][e], sum);
-  return sum;
+    for (int e = 0; e < N / 2; ++e) sum = f2_fma(f[i][e], f[i][e], sum);
+  return f2_lo(sum) + f2_hi(sum);
 }
 
 // The sum over the block, in every thread
@@ -138,7 +157,7 @@ __device__ __forceinline__ double block_sum(double d) {
   return d;
 }
 
-__global__ void __launch_bounds__(kThreads, kCtasPerSm) clip_sum(const __grid_constant__ ClipParams p) {
+__global__ void __launch_bounds__(kThreads, kSumCtas) clip_sum(const __grid_constant__ ClipParams p) {
   asm volatile("griddepcontrol.launch_dependents;");
   double sum = 0.0;
   int at = 0;
@@ -153,35 +172,52 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) clip_sum(const __grid_co
   if (threadIdx.x == 0) p.part[blockIdx.x] = d;
 }
 
+__device__ __forceinline__ uint4 pack(const f32x2 (&f)[2], const float*) {
+  return make_uint4(__float_as_uint(f2_lo(f[0])), __float_as_uint(f2_hi(f[0])), __float_as_uint(f2_lo(f[1])),
+                    __float_as_uint(f2_hi(f[1])));
+}
+__device__ __forceinline__ uint4 pack(const f32x2 (&f)[4], const __nv_bfloat16*) {
+  return make_uint4(f2_bf16(f[0]), f2_bf16(f[1]), f2_bf16(f[2]), f2_bf16(f[3]));
+}
+__device__ __forceinline__ uint4 pack(const f32x2 (&f)[4], const __half*) {
+  uint4 w;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __half2 v = __floats2half2_rn(f2_lo(f[i]), f2_hi(f[i]));
+    (&w.x)[i] = *reinterpret_cast<const uint32_t*>(&v);
+  }
+  return w;
+}
+
 // 16 bytes stored per thread and vector, neighbours next to one another: 16-bit gradients on their way to fp32 are
 // taken 8 bytes at a time (with 16, a warp's stores left every other 16 bytes for the next: 54 us against 41)
 template <typename T, typename U>
 __device__ __forceinline__ void scale(const Tensor& t, uint32_t chunk, float c) {
   constexpr int N = 16 / sizeof(U);
-  using S = Span<T, N>;
+  using S = Span<T, N, kScaleBytes>;
   const S s(t, chunk);
-  U* out = static_cast<U*>(t.out) - s.lo;  // element i of the span goes to out[i]
-  const bool aligned = (reinterpret_cast<uintptr_t>(out) & 15) == 0;
-  float f[S::kEach][N];
+  U* out = static_cast<U*>(t.out) - s.shift + s.v0 * N;  // the thread's first element
+  f32x2 f[S::kEach][N / 2];
   s.load(f);
 #pragma unroll
   for (int i = 0; i < S::kEach; ++i) {
     const int64_t e0 = (s.v0 + i * kThreads) * N;
-    uint4 w;
-    U* e = reinterpret_cast<U*>(&w);
 #pragma unroll
-    for (int x = 0; x < N; ++x) e[x] = from_f32<U>(f[i][x] * c);
-    if (aligned && (s.full || (s.has(e0) && s.has(e0 + N - 1)))) {
-      *reinterpret_cast<uint4*>(out + e0) = w;
+    for (int x = 0; x < N / 2; ++x) f[i][x] = f2_mul(f[i][x], f2_make(c, c));
+    const uint4 w = pack(f[i], static_cast<const U*>(nullptr));
+    U* to = out + i * kThreads * N;
+    if (t.out_aligned && (s.full || (s.has(e0) && s.has(e0 + N - 1)))) {
+      *reinterpret_cast<uint4*>(to) = w;
     } else {
+      const U* e = reinterpret_cast<const U*>(&w);
 #pragma unroll
       for (int x = 0; x < N; ++x)
-        if (s.has(e0 + x)) out[e0 + x] = e[x];
+        if (s.has(e0 + x)) to[x] = e[x];
     }
   }
 }
 
-__global__ void __launch_bounds__(kThreads, kCtasPerSm) clip_scale(const __grid_constant__ ClipParams p) {
+__global__ void __launch_bounds__(kThreads, kScaleCtas) clip_scale(const __grid_constant__ ClipParams p) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;");
   double d = 0.0;
@@ -192,8 +228,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) clip_scale(const __grid_
   if (c >= 1.f) c = 1.f;  // a NaN norm stays NaN
   if (c == 1.f && p.in_place) return;
   int at = p.count - 1;
-  for (uint32_t i = blockIdx.x; i < p.chunks; i += gridDim.x) {
-    const uint32_t chunk = p.chunks - 1 - i;
+  // the CTA's chunks from the last to the first: what was summed last may still be in L2
+  const uint32_t mine = blockIdx.x < p.chunks ? (p.chunks - 1 - blockIdx.x) / gridDim.x + 1 : 0;
+  for (uint32_t i = mine; i-- > 0;) {
+    const uint32_t chunk = blockIdx.x + i * gridDim.x;
     at = tensor_of<true>(p, chunk, at);
     const Tensor& t = p.t[at];
     if (t.dtype == FB_F32) scale<float, float>(t, chunk, c);
@@ -219,16 +257,10 @@ int sm_count() {
 bool bad_dtype(int d) { return d != FB_F32 && d != FB_F16 && d != FB_BF16; }
 int size_of(int dtype) { return dtype == FB_F32 ? 4 : 2; }
 
-uint64_t chunks_of(const void* g, int64_t n, int dtype) {
-  if (n == 0) return 0;
-  const uint64_t bytes = (uint64_t)n * size_of(dtype) + (reinterpret_cast<uintptr_t>(g) & 15);
-  return (bytes + kChunkBytes - 1) / kChunkBytes;
-}
-
-// Every launch leaves at most kCtasPerSm sums per SM
+// Every launch leaves at most kSumCtas sums per SM
 size_t workspace_size(const fb_clip_args* a) {
   const size_t launches = (size_t)std::max(1, (a->count + kTensors - 1) / kTensors);
-  return launches * kCtasPerSm * sm_count() * sizeof(double);
+  return launches * kSumCtas * sm_count() * sizeof(double);
 }
 
 int check(const fb_clip_args* a) {
@@ -252,30 +284,34 @@ int check(const fb_clip_args* a) {
   return FB_OK;
 }
 
-// The launch's table: tensors [i0, i1)
-void fill(ClipParams* p, const fb_clip_args* a, int i0, int i1) {
+// The table of launch l, in chunks of `bytes`
+void fill(ClipParams* p, const fb_clip_args* a, int l, uint32_t bytes) {
   p->count = 0;
   p->chunks = 0;
   p->in_place = true;
-  for (int i = i0; i < i1; ++i) {
-    const uint64_t n = chunks_of(a->grads[i], a->numel[i], a->dtype[i]);
-    if (n == 0) continue;
+  for (int i = l * kTensors; i < std::min(a->count, (l + 1) * kTensors); ++i) {
+    if (a->numel[i] == 0) continue;
     Tensor& t = p->t[p->count++];
     t.g = a->grads[i];
     t.out = a->out != nullptr ? a->out[i] : nullptr;
-    p->in_place = p->in_place && t.out == t.g;
     t.n = a->numel[i];
-    t.chunk0 = p->chunks;
     t.dtype = (uint8_t)a->dtype[i];
     t.out_dtype = (uint8_t)(a->out_dtype != nullptr ? a->out_dtype[i] : a->dtype[i]);
-    p->chunks += (uint32_t)n;
+    const uint64_t shift = reinterpret_cast<uintptr_t>(t.g) & 15, end = shift + (uint64_t)t.n * size_of(t.dtype);
+    t.chunk0 = p->chunks;
+    t.full0 = t.chunk0 + (shift > 0);
+    t.fulls = (uint32_t)std::max<int64_t>((int64_t)(end / bytes) - (shift > 0), 0);
+    t.out_aligned =
+        (reinterpret_cast<uintptr_t>(t.out) - shift / size_of(t.dtype) * size_of(t.out_dtype)) % 16 == 0;
+    p->in_place = p->in_place && t.out == t.g;
+    p->chunks += (uint32_t)((end + bytes - 1) / bytes);
   }
 }
 
 int clip(const fb_clip_args* a, cudaStream_t s) {
   const int rc = check(a);
   if (rc != FB_OK) return rc;
-  const int most = kCtasPerSm * sm_count(), launches = std::max(1, (a->count + kTensors - 1) / kTensors);
+  const int sms = sm_count(), launches = std::max(1, (a->count + kTensors - 1) / kTensors);
   ClipParams p{};
   p.max_norm = a->max_norm;
   p.eps = a->eps;
@@ -283,23 +319,22 @@ int clip(const fb_clip_args* a, cudaStream_t s) {
   int parts = 0;
   cudaError_t e = cudaSuccess;
   for (int l = 0; l < launches && e == cudaSuccess; ++l) {
-    fill(&p, a, l * kTensors, std::min(a->count, (l + 1) * kTensors));
-    const int grid = (int)std::max<uint32_t>(1, std::min<uint32_t>(p.chunks, most));
+    fill(&p, a, l, kSumBytes);
+    const int grid = (int)std::max<uint32_t>(1, std::min<uint32_t>(p.chunks, kSumCtas * sms));
     p.part = sums + parts;
     parts += grid;
     clip_sum<<<grid, kThreads, 0, s>>>(p);
     e = cudaGetLastError();
   }
-  // one launch: its table still is in p
   p.part = sums;
   p.parts = parts;
   int n = launches;
   for (int l = 0; l < (a->out != nullptr ? launches : 1) && e == cudaSuccess; ++l, ++n) {
-    if (launches > 1) fill(&p, a, l * kTensors, std::min(a->count, (l + 1) * kTensors));
+    if (a->out != nullptr) fill(&p, a, l, kScaleBytes);
+    else p.chunks = 0;
     p.norm = l == 0 ? a->norm : nullptr;
-    if (a->out == nullptr) p.chunks = 0;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(std::max<uint32_t>(1, std::min<uint32_t>(p.chunks, most)));
+    cfg.gridDim = dim3(std::max<uint32_t>(1, std::min<uint32_t>(p.chunks, kScaleCtas * sms)));
     cfg.blockDim = dim3(kThreads);
     cfg.stream = s;
     cudaLaunchAttribute at{};

@@ -14,6 +14,8 @@ import torch
 
 from .. import _lib
 
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch.cuda.current_device
 _FORMAT = {ctypes.c_int32: "i", ctypes.c_int64: "q", ctypes.c_float: "f", ctypes.c_void_p: "P", ctypes.c_size_t: "N"}
 
 
@@ -31,21 +33,24 @@ def packer(cls: type[ctypes.Structure]) -> Callable[..., ctypes.Structure]:
 
 def launch(fn: Callable, args: ctypes.Structure, index: int, what: str) -> None:
     """fn(args, stream) on device `index`'s current stream; a status other than FB_OK raises."""
-    if torch.cuda.current_device() == index:
-        rc = fn(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(index))
+    if _current_device() == index:
+        rc = fn(args, _raw_stream(index))  # the C side takes a pointer: ctypes passes the struct's address
     else:
         with torch.cuda.device(index):
-            rc = fn(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(index))
+            rc = fn(args, _raw_stream(index))
     if rc:
         _lib.check(rc, what)
 
 
 def same_device(what: str, *tensors: torch.Tensor) -> int:
     """The CUDA device index that all tensors are on; raises where they are not on one."""
-    index = tensors[0].get_device()
-    for t in tensors:
-        if t.get_device() != index or index < 0:
-            if all(x.is_cuda for x in tensors):
-                raise RuntimeError(f"{what}: all tensors must be on one device; got {[str(x.device) for x in tensors]}")
-            raise RuntimeError(f"{what} (B200): CUDA tensors required; there is no CPU path")
-    return index
+    first, *rest = [t.get_device() for t in tensors]
+    for index in rest:
+        if index != first:
+            break
+    else:
+        if first >= 0:
+            return first
+    if all(t.is_cuda for t in tensors):
+        raise RuntimeError(f"{what}: all tensors must be on one device; got {[str(t.device) for t in tensors]}")
+    raise RuntimeError(f"{what} (B200): CUDA tensors required; there is no CPU path")

@@ -29,15 +29,16 @@ _write_args = packer(_lib.FbPagedWriteArgs)
 
 
 def _check_pages(what: str, x: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor) -> None:
+    dtype = x.dtype
     if k_pages.dim() != 4 or k_pages.shape != v_pages.shape:
         raise ValueError(f"{what}: pages must be two (num_pages, kv_heads, page_size, head_dim) tensors of one shape; "
                          f"got {tuple(k_pages.shape)}, {tuple(v_pages.shape)}")
-    if x.dtype not in _DTYPE_CODE or k_pages.dtype != x.dtype or v_pages.dtype != x.dtype:
-        raise ValueError(f"{what}: one dtype of float32 / float16 / bfloat16 for all; got {x.dtype}, {k_pages.dtype}, "
+    if dtype not in _DTYPE_CODE or k_pages.dtype is not dtype or v_pages.dtype is not dtype:
+        raise ValueError(f"{what}: one dtype of float32 / float16 / bfloat16 for all; got {dtype}, {k_pages.dtype}, "
                          f"{v_pages.dtype}")
-    if k_pages.shape[3] > 1 and (k_pages.stride(3) != 1 or v_pages.stride(3) != 1):
+    if (k_pages.stride(3) != 1 or v_pages.stride(3) != 1) and k_pages.shape[3] > 1:
         raise ValueError(f"{what}: pages must have a unit inner stride (they are not copied)")
-    if torch.is_grad_enabled() and (x.requires_grad or k_pages.requires_grad or v_pages.requires_grad):
+    if (x.requires_grad or k_pages.requires_grad or v_pages.requires_grad) and torch.is_grad_enabled():
         raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad()")
 
 
