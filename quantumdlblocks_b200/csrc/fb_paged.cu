@@ -49,6 +49,7 @@ struct PagedParams {
   int HU, chunks, U;  // query heads per unit, units per kv head, units per sequence
   int tile;           // keys, a multiple of 2 kSub where units are cut
   uint32_t W;         // workers that share the tiles (all units' tiles are below 2^31)
+  uint2* ends;        // [S U] first and last worker of each unit
   float* part;        // [W][2][HU][D] sums of p v, then [W][2][HU] sums of p
   int* status;        // device status word
 };
@@ -153,6 +154,14 @@ struct Walk {
     if (t >= t1) return false;
     piece(p);
     return true;
+  }
+  // Where the unit begins in this share: its first and last worker, for the join (a unit in one share needs none
+  // but that its two are alike).  pre: tile_prefix's.
+  template <int N>
+  __device__ void tell_ends(const PagedParams& p, const uint32_t* pre, uint32_t worker) const {
+    if (p.ends == nullptr || a != 0) return;
+    const uint32_t last = b == k.tiles ? worker : Shares(pre[N - 1], p.W).owner(t + k.tiles - 1);
+    p.ends[(int64_t)s * p.U + unit] = make_uint2(worker, last);
   }
   __device__ int first_key(const PagedParams& p) const { return k.base + (int)a * p.tile; }
   __device__ int end_key(const PagedParams& p) const { return b == k.tiles ? k.hi : k.base + (int)b * p.tile; }
@@ -358,6 +367,7 @@ __global__ void __launch_bounds__(kThreads, TcShape<D>::kCtasPerSm)
   do {
     const int kvh = w.unit / p.chunks, h0 = w.unit % p.chunks * p.HU, nh = min(p.HU, p.G - h0);
     const int head0 = kvh * p.G + h0;
+    if (lane == 0) w.tell_ends<kThreads>(p, pre, worker);
     // Q: heads r (and r + 8) of the unit, zero where it has fewer
     uint32_t qf[D / 32][kHeads][4];
     float sc[kHeads];
@@ -622,6 +632,7 @@ __global__ void __launch_bounds__(kThreads, (GenShape<T, VEC, LANES>::kCtasPerSm
   do {
     const int kvh = w.unit / p.chunks, h0 = w.unit % p.chunks * HU, nh = min(HU, p.G - h0);
     const int head0 = kvh * p.G + h0;
+    if (threadIdx.x == 0) w.tell_ends<kThreads>(p, pre, blockIdx.x);
     const int32_t* table = p.table + w.s * p.table_stride;
     const T* kbase = static_cast<const T*>(p.k) + kvh * p.ks[1];
     const T* vbase = static_cast<const T*>(p.v) + kvh * p.vs[1];
@@ -813,27 +824,16 @@ __global__ void __launch_bounds__(kThreads, (GenShape<T, VEC, LANES>::kCtasPerSm
 // ------------------------------------------------------------------------------------------
 template <typename T, int THREADS>
 __global__ void __launch_bounds__(THREADS) paged_join(const PagedParams p, int ways) {
-  __shared__ uint32_t pre[THREADS];
   __shared__ float so[THREADS], sz[THREADS / 32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, slices = (p.D + 31) / 32;
-  const int per = tile_prefix<THREADS>(p, pre);
   const uint32_t item = blockIdx.x * (THREADS / 32 / ways) + warp / ways, row = item / slices;
   const bool work = row < (uint32_t)(p.S * p.H);
   const int way = warp & (ways - 1), d = (int)(item - row * slices) * 32 + lane;
   const int s = work ? (int)(row / p.H) : 0, head = work ? (int)(row % p.H) : 0;
   const int kvh = head / p.G, chunk = head % p.G / p.HU, h = head % p.G % p.HU;
-  // tiles before sequence s: those of the groups before its own, and of the sequences before it in that
-  const int g = s / per;
-  uint32_t before = 0;
-  for (int x = g * per + lane; x < s; x += 32) before += keys_of(p, x).tiles * p.U;
-#pragma unroll
-  for (int x = 16; x > 0; x >>= 1) before += __shfl_xor_sync(0xffffffffu, before, x);
-  if (g > 0) before += pre[g - 1];
-  const uint32_t n = keys_of(p, s).tiles;
-  const uint32_t t0 = before + (uint32_t)(kvh * p.chunks + chunk) * n;
-  const Shares sh(pre[THREADS - 1], p.W);
-  const uint32_t w0 = sh.owner(t0), w1 = sh.owner(t0 + n - 1);
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  const uint2 ends = p.ends[(int64_t)s * p.U + kvh * p.chunks + chunk];
+  const uint32_t w0 = ends.x, w1 = ends.y;  // alike: finished by that worker
   float o = 0.f, z = 0.f;
   if (work && w0 != w1 && d < p.D) {
     const float* zs = slot_z(p);
@@ -1089,6 +1089,10 @@ bool aligned16(const void* p, const int64_t* s, int n, int size) {
   return ok;
 }
 
+// The units' ends come first in the workspace, an even number of them: the sums behind them are stored 16 bytes at
+// a time.
+int64_t even_units(int64_t units) { return (units + 1) & ~1ll; }
+
 // What a call launches, from sizes, types and alignment alone.
 struct PagedPlan {
   bool tc;         // the tensor-core kernel
@@ -1133,7 +1137,7 @@ PagedPlan plan_paged(const fb_paged_args* a) {
   const int per_sm = pl.tc ? kWarps * (a->head_dim == 64 ? TcShape<64>::kCtasPerSm : TcShape<128>::kCtasPerSm)
                      : size == 4 ? general_ctas_per_sm<float>(pl) : general_ctas_per_sm<__half>(pl);
   pl.W = (uint32_t)std::min<int64_t>(tiles, pl.join ? (int64_t)per_sm * sm_count() : 0x7FFFFFFF);
-  pl.workspace = pl.join ? (size_t)pl.W * 2 * pl.HU * (a->head_dim + 1) * sizeof(float) : 0;
+  pl.workspace = pl.join ? (size_t)pl.W * 2 * pl.HU * (a->head_dim + 1) * sizeof(float) + (size_t)even_units(units) * sizeof(uint2) : 0;
   return pl;
 }
 
@@ -1209,7 +1213,7 @@ cudaError_t launch_tc(const PagedParams& p, const PagedPlan& pl, cudaStream_t st
 
 template <typename T, int THREADS>
 cudaError_t launch_join(const PagedParams& p, int ways, cudaStream_t st) {
-  // its CTAs start while the last shares still run (what they need of the lengths is read meanwhile), and wait
+  // its CTAs start where the last shares leave room, and wait for them
   const int64_t items = (int64_t)p.S * p.H * ((p.D + 31) / 32), each = THREADS / 32 / ways;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)((items + each - 1) / each));
@@ -1249,6 +1253,7 @@ int paged_fwd(const fb_paged_args* a, cudaStream_t st) {
   }
   const PagedPlan pl = plan_paged(a);
   if (pl.workspace > 0 && (a->workspace == nullptr || a->workspace_bytes < pl.workspace)) return FB_ERR_WORKSPACE;
+  if (pl.workspace > 0 && (reinterpret_cast<uintptr_t>(a->workspace) & 15) != 0) return FB_ERR_ALIGN;
   PagedParams p{};
   p.S = a->seqs; p.H = a->heads; p.Hkv = a->kv_heads; p.G = a->heads / a->kv_heads; p.D = a->head_dim;
   p.page = a->page_size; p.pages = a->num_pages;
@@ -1260,7 +1265,10 @@ int paged_fwd(const fb_paged_args* a, cudaStream_t st) {
   for (int i = 0; i < 4; ++i) p.ks[i] = a->k_stride[i], p.vs[i] = a->v_stride[i];
   p.table = a->table; p.table_stride = a->table_stride; p.lens = a->lens;
   p.HU = pl.HU; p.chunks = pl.chunks; p.U = p.Hkv * p.chunks; p.tile = pl.tile; p.W = pl.W;
-  p.part = static_cast<float*>(a->workspace);
+  if (pl.join) {
+    p.ends = static_cast<uint2*>(a->workspace);
+    p.part = reinterpret_cast<float*>(p.ends + even_units((int64_t)p.S * p.U));
+  }
   p.status = device_status_word(&rc);
   if (rc != FB_OK) return rc;
   cudaError_t e;
