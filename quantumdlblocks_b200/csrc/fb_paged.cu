@@ -530,7 +530,8 @@ __global__ void __launch_bounds__(kThreads, TcShape<D>::kCtasPerSm)
       if (h >= nh) continue;
       const bool whole = w.whole();
       const bool none = z[y] == 0.f;  // no key with weight: 0, also where eps is 0
-      const float norm = none ? 1.f : z[y] + p.eps;
+      const float norm = none ? 1.f : z[y] + p.eps, inv = 1.f / norm;
+      const bool tiny = norm < 1e-30f;  // its reciprocal may overflow
       T* out = static_cast<T*>(p.out) + w.s * p.os[0] + (head0 + h) * p.os[1];
       const int64_t slot = slot_of(worker, w.a == 0);
       float* part = p.part + (slot * p.HU + h) * D;
@@ -545,7 +546,7 @@ __global__ void __launch_bounds__(kThreads, TcShape<D>::kCtasPerSm)
           if (whole) {
             T t[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) t[e] = from_f32<T>(none ? 0.f : x[e] / norm);
+            for (int e = 0; e < 8; ++e) t[e] = from_f32<T>(none ? 0.f : tiny ? x[e] / norm : x[e] * inv);
             uint4 packed;
             memcpy(&packed, t, 16);
             *reinterpret_cast<uint4*>(out + d) = packed;
