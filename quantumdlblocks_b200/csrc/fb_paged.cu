@@ -820,45 +820,53 @@ __global__ void __launch_bounds__(kThreads, (GenShape<T, VEC, LANES>::kCtasPerSm
 }
 
 // ------------------------------------------------------------------------------------------
-// The pieces of units that span several shares, added in share order.  `ways` warps (a power of two) on
-// 32 dimensions of a query head, one on every ways-th piece; blocks of max(8, ways) warps.
+// The pieces of units that span several shares, added in share order: `ways` warps (a power of two) on a query
+// head, one on every ways-th piece.  Blocks of max(8, ways) warps; a block's heads are of one sequence.
 // ------------------------------------------------------------------------------------------
-template <typename T, int THREADS>
-__global__ void __launch_bounds__(THREADS) paged_join(const PagedParams p, int ways) {
-  __shared__ float so[THREADS], sz[THREADS / 32];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, slices = (p.D + 31) / 32;
-  const uint32_t item = blockIdx.x * (THREADS / 32 / ways) + warp / ways, row = item / slices;
-  const bool work = row < (uint32_t)(p.S * p.H);
-  const int way = warp & (ways - 1), d = (int)(item - row * slices) * 32 + lane;
-  const int s = work ? (int)(row / p.H) : 0, head = work ? (int)(row % p.H) : 0;
-  const int kvh = head / p.G, chunk = head % p.G / p.HU, h = head % p.G % p.HU;
+template <typename T, int SLICES>  // of 32 dimensions
+__global__ void __launch_bounds__(1024) paged_join(const PagedParams p, int ways) {
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  float* so = reinterpret_cast<float*>(smem_raw);  // [warps][SLICES * 32], then [warps]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  float* sz = so + warps * SLICES * 32;
+  const int s = blockIdx.x, head = (blockIdx.y * warps + warp) / ways, way = warp & (ways - 1);
+  const bool work = head < p.H;
+  const int kvh = head / p.G, chunk = (head - kvh * p.G) / p.HU, h = head - kvh * p.G - chunk * p.HU;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const uint2 ends = p.ends[(int64_t)s * p.U + kvh * p.chunks + chunk];
-  const uint32_t w0 = ends.x, w1 = ends.y;  // alike: finished by that worker
-  float o = 0.f, z = 0.f;
-  if (work && w0 != w1 && d < p.D) {
+  uint2 ends = make_uint2(0, 0);  // alike: finished by that worker
+  if (work) ends = p.ends[(int64_t)s * p.U + kvh * p.chunks + chunk];
+  float o[SLICES], z = 0.f;
+#pragma unroll
+  for (int i = 0; i < SLICES; ++i) o[i] = 0.f;
+  if (ends.x != ends.y) {
     const float* zs = slot_z(p);
-#pragma unroll 8
-    for (uint32_t w = w0 + way; w <= w1; w += ways) {
-      const int64_t slot = slot_of(w, w == w0);
-      o += p.part[(slot * p.HU + h) * p.D + d];
-      z += zs[slot * p.HU + h];
+#pragma unroll 4
+    for (uint32_t w = ends.x + way; w <= ends.y; w += ways) {
+      const int64_t row = slot_of(w, w == ends.x) * p.HU + h;
+      const float* part = p.part + row * p.D;
+#pragma unroll
+      for (int i = 0; i < SLICES; ++i)
+        if (i * 32 + lane < p.D) o[i] += part[i * 32 + lane];
+      z += zs[row];
     }
   }
   if (ways > 1) {
-    so[threadIdx.x] = o;
+#pragma unroll
+    for (int i = 0; i < SLICES; ++i) so[(warp * SLICES + i) * 32 + lane] = o[i];
     if (lane == 0) sz[warp] = z;
     __syncthreads();
-    if (way == 0)
-      for (int x = 1; x < ways; ++x) {
-        o += so[threadIdx.x + 32 * x];
-        z += sz[warp + x];
-      }
+    if (way != 0) return;
+    for (int x = 1; x < ways; ++x) {
+#pragma unroll
+      for (int i = 0; i < SLICES; ++i) o[i] += so[((warp + x) * SLICES + i) * 32 + lane];
+      z += sz[warp + x];
+    }
   }
-  if (work && w0 != w1 && d < p.D && way == 0) {
-    T* out = static_cast<T*>(p.out) + s * p.os[0] + head * p.os[1];
-    out[d] = from_f32<T>(z == 0.f ? 0.f : o / (z + p.eps));
-  }
+  if (ends.x == ends.y) return;
+  T* out = static_cast<T*>(p.out) + s * p.os[0] + head * p.os[1];
+#pragma unroll
+  for (int i = 0; i < SLICES; ++i)
+    if (i * 32 + lane < p.D) out[i * 32 + lane] = from_f32<T>(z == 0.f ? 0.f : o[i] / (z + p.eps));
 }
 
 struct WriteParams {
@@ -1144,7 +1152,7 @@ PagedPlan plan_paged(const fb_paged_args* a) {
 
 int check_paged(const fb_paged_args* a) {
   if (a == nullptr) return FB_ERR_ARG;
-  if (a->seqs < 0 || a->heads < 1 || a->kv_heads < 1 || a->heads % a->kv_heads != 0 || a->heads > 65535 ||
+  if (a->seqs < 0 || a->heads < 1 || a->kv_heads < 1 || a->heads % a->kv_heads != 0 || a->heads > 16384 ||
       a->head_dim < 1 || a->head_dim > 256 || a->page_size < 1 || a->num_pages < 0 || a->max_pages < 0 ||
       (int64_t)a->page_size * a->max_pages > 0x7FFFFFFF - 256 || (int64_t)a->seqs * a->heads > 0x0FFFFFFF)
     return FB_ERR_SHAPE;
@@ -1212,20 +1220,21 @@ cudaError_t launch_tc(const PagedParams& p, const PagedPlan& pl, cudaStream_t st
   return tma ? launch_tc<T, D, false, true>(p, k, v, st) : launch_tc<T, D, false, false>(p, k, v, st);
 }
 
-template <typename T, int THREADS>
+template <typename T, int SLICES>
 cudaError_t launch_join(const PagedParams& p, int ways, cudaStream_t st) {
   // its CTAs start where the last shares leave room, and wait for them
-  const int64_t items = (int64_t)p.S * p.H * ((p.D + 31) / 32), each = THREADS / 32 / ways;
+  const int warps = std::max(8, ways);
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)((items + each - 1) / each));
-  cfg.blockDim = dim3(THREADS);
+  cfg.gridDim = dim3((unsigned)p.S, (unsigned)((p.H * ways + warps - 1) / warps));
+  cfg.blockDim = dim3(warps * 32);
+  cfg.dynamicSmemBytes = (size_t)warps * (SLICES * 32 + 1) * sizeof(float);
   cfg.stream = st;
   cudaLaunchAttribute at{};
   at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, paged_join<T, THREADS>, p, ways);
+  return cudaLaunchKernelEx(&cfg, paged_join<T, SLICES>, p, ways);
 }
 
 template <typename T>
@@ -1237,12 +1246,14 @@ cudaError_t launch_paged(const PagedParams& p, const PagedPlan& pl, cudaStream_t
     e = launch_general<T>(p, pl, st);
   }
   if (e != cudaSuccess || !pl.join) return e;
-  // A warp has eight pieces' loads under way at a time: a warp on an output for every eight of the pieces that a
+  // A warp has four pieces' loads under way at a time: a warp on an output for every eight of the pieces that a
   // unit would have were the lengths alike (49 pieces of 192 units: 27 us with 32 warps each, 5 us with 8)
   const uint32_t pieces = p.W / ((uint32_t)p.S * p.U) + 1;
   int ways = 1;
   while (ways < 32 && ways * 8 < (int)pieces) ways *= 2;
-  return ways <= 8 ? launch_join<T, 256>(p, ways, st) : launch_join<T, 1024>(p, ways, st);
+  if (p.D <= 32) return launch_join<T, 1>(p, ways, st);
+  if (p.D <= 64) return launch_join<T, 2>(p, ways, st);
+  return p.D <= 128 ? launch_join<T, 4>(p, ways, st) : launch_join<T, 8>(p, ways, st);
 }
 
 int paged_fwd(const fb_paged_args* a, cudaStream_t st) {
