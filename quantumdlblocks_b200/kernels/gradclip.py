@@ -7,6 +7,7 @@ their number, sizes and types.  CUDA only, like every op here.
 from __future__ import annotations
 
 import array
+from operator import attrgetter
 from typing import Iterable, Optional, Sequence
 
 import torch
@@ -19,16 +20,20 @@ __all__ = ["clip_grad_norm_", "grad_norm"]
 
 
 _clip_args = packer(_lib.FbClipArgs)
+# mapped over dozens of tensors a step: unbound methods, no bytecode per tensor
+_data_ptr, _numel, _get_device, _is_contiguous = (getattr(torch.Tensor, n) for n in
+                                                  ("data_ptr", "numel", "get_device", "is_contiguous"))
+_dtype, _shape = attrgetter("dtype"), attrgetter("shape")
 
 
 def _codes(what: str, tensors: Sequence[torch.Tensor], index: int) -> array.array:
     """The tensors' dtype codes; raises where one is not a float tensor on device `index`."""
-    if any(t.get_device() != index for t in tensors):
+    if set(map(_get_device, tensors)) != {index}:
         if all(t.is_cuda for t in tensors):
             raise RuntimeError(f"{what}: all tensors must be on one device; got {sorted({str(t.device) for t in tensors})}")
         raise RuntimeError(f"{what} (B200): CUDA tensors required; there is no CPU path")
     try:
-        return array.array("i", [_DTYPE_CODE[t.dtype] for t in tensors])
+        return array.array("i", map(_DTYPE_CODE.__getitem__, map(_dtype, tensors)))
     except KeyError:
         raise ValueError(f"{what}: gradients are dense float32 / float16 / bfloat16; got "
                          f"{sorted({str(t.dtype) for t in tensors})}") from None
@@ -41,12 +46,12 @@ def _run(grads: Sequence[torch.Tensor], out: Optional[Sequence[torch.Tensor]], m
     first = grads[0]
     index = max(first.get_device(), 0)
     codes = _codes(what, grads, index)
-    ptrs = array.array("Q", [g.data_ptr() for g in grads])
-    numel = array.array("q", [g.numel() for g in grads])
+    ptrs = array.array("Q", map(_data_ptr, grads))
+    numel = array.array("q", map(_numel, grads))
     out_ptrs, out_codes = ptrs, codes  # in place
     if out is not None and out is not grads:
         out_codes = _codes(what, out, index)
-        out_ptrs = array.array("Q", [o.data_ptr() for o in out])
+        out_ptrs = array.array("Q", map(_data_ptr, out))
     norm = torch.empty((), dtype=torch.float32, device=first.device)
     a = _clip_args(len(grads), ptrs.buffer_info()[0], out_ptrs.buffer_info()[0] if out is not None else 0,
                    numel.buffer_info()[0], codes.buffer_info()[0], out_codes.buffer_info()[0], max_norm, eps,
@@ -103,15 +108,15 @@ def clip_grad_norm_(
     to = gs if out is None else list(out)
     if len(to) != len(gs):
         raise ValueError(f"clip_grad_norm_: {len(gs)} gradients, but out has {len(to)} tensors")
-    plain = all([g.is_contiguous() for g in gs])
+    plain = all(map(_is_contiguous, gs))
     if not plain:
         for g in gs:
             if not _dense(g):
                 raise ValueError(f"clip_grad_norm_: gradients must be dense; got strides {g.stride()} for {tuple(g.shape)}")
     if to is not gs:
-        alike = [g.shape for g in gs] == [o.shape for o in to]
-        alike = alike and (all([o.is_contiguous() for o in to]) if plain else [g.stride() for g in gs] == [o.stride() for o in to])
-        if not alike or any([o.dtype is not torch.float32 and o.dtype is not g.dtype for g, o in zip(gs, to)]):
+        alike = list(map(_shape, gs)) == list(map(_shape, to))
+        alike = alike and (all(map(_is_contiguous, to)) if plain else [g.stride() for g in gs] == [o.stride() for o in to])
+        if not alike or any(o not in (torch.float32, g) for g, o in set(zip(map(_dtype, gs), map(_dtype, to)))):
             raise ValueError("clip_grad_norm_: each of out must match its gradient's shape and memory order, and have its "
                              "dtype or float32; got "
                              f"{[(tuple(o.shape), o.stride(), o.dtype) for o in to]} for "

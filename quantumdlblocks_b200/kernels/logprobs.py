@@ -11,6 +11,7 @@ from __future__ import annotations
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from .. import _lib
 from ._host import launch, packer, same_device
@@ -66,6 +67,7 @@ class _TokenLogprobs(torch.autograd.Function):
         return logp, entropy, top_logp, top_index
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, g_logp: Optional[torch.Tensor], g_entropy: Optional[torch.Tensor],
                  g_top: Optional[torch.Tensor], _g_index):
         logits, targets, entropy, stats, top_index = ctx.saved_tensors

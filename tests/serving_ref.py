@@ -76,8 +76,8 @@ def logprobs(logits, targets, top_k):
     x = logits.detach().double()
     N, V = x.shape
     m = x.max(dim=1, keepdim=True).values
-    lse = m + torch.log(torch.exp(x - m).sum(1, keepdim=True))
-    lp = x - lse
+    # (x - m) - log s, not x - (m + log s): m may be the lowest value of a type, beside which log s is lost
+    lp = (x - m) - torch.log(torch.exp(x - m).sum(1, keepdim=True))
     p = torch.exp(lp)
     ent = -torch.where(x == -math.inf, p, p * lp).sum(1)  # p is 0 where x is -inf (or the row is NaN)
     ok = (targets >= 0) & (targets < V)

@@ -135,6 +135,23 @@ def test_runs_on_the_current_stream():
     check(norm, new, want_norm, want)
 
 
+def test_clip_replays_from_a_graph():
+    gs = make([5000, 300, 7], [F32, BF16])
+    new = [torch.zeros_like(g) for g in gs]
+    clip_grad_norm_([g.clone() for g in gs], 1.0)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        norm = clip_grad_norm_(new, 1.0)
+    for seed in (0, 1):
+        want_norm, want = ref.clip(make([5000, 300, 7], [F32, BF16], seed), 1.0)
+        for a, b in zip(new, make([5000, 300, 7], [F32, BF16], seed)):
+            a.copy_(b)
+        graph.replay()
+        torch.cuda.synchronize()
+        check(norm, new, want_norm, want)
+
+
 def test_refusals():
     g = torch.ones(8, device="cuda")
     for args in (([], 1.0), ([g], -1.0), ([g], math.nan), ([g.double()], 1.0), ([g.int()], 1.0)):

@@ -113,6 +113,69 @@ def test_rows_without_a_distribution(dtype):
 
 
 @TYPES
+@pytest.mark.parametrize("V", [500, 50304])
+def test_masks_of_the_lowest_value(dtype, V):
+    """Columns masked by the type's lowest finite number: no probability beside live ones; a row of nothing else is
+    uniform over them, with -inf columns left out; forward and gradient."""
+    low = torch.finfo(dtype).min
+    x, t = make(4, V, dtype)
+    x[0, V // 3:] = low
+    x[1] = low
+    x[2] = low
+    x[2, 100:] = -math.inf
+    x[3, 5:] = low / 2
+    t[0], t[2], t[3] = 7, 50, 4
+    r = token_logprobs(x, t, top_k=4)
+    logp, ent, top, order = ref.logprobs(x, t, 4)
+    assert torch.equal(r.top_index, order)
+    torch.testing.assert_close(r.logp.double(), logp, rtol=1e-6, atol=2e-5)
+    torch.testing.assert_close(r.entropy.double(), ent, rtol=1e-5, atol=2e-5)
+    torch.testing.assert_close(r.top_logp.double(), top, rtol=1e-6, atol=2e-5)
+    assert abs(float(r.logp[1]) + math.log(V)) <= 2e-5 and abs(float(r.logp[2]) + math.log(100)) <= 2e-5
+    g = torch.Generator(device="cuda").manual_seed(0)
+    gl, ge = (torch.randn(4, generator=g, device="cuda") for _ in range(2))
+    gt = torch.randn(4, 4, generator=g, device="cuda")
+    leaf = x.clone().requires_grad_(True)
+    r = token_logprobs(leaf, t, top_k=4)
+    (dx,) = torch.autograd.grad([r.logp, r.entropy, r.top_logp], [leaf], [gl, ge, gt])
+    want = ref.logprobs_grad(x, t, order, gl, ge, gt)
+    size = float((gl.abs() + gt.abs().sum(1) + ge.abs() * (30 + math.log(V))).max())
+    tol = ref.ROUND[dtype] * 1.01 * want.abs() + 2e-5 * size * torch.softmax(x.double(), 1) + 3e-7 * size
+    assert bool(((dx.double() - want).abs() <= tol).all())
+
+
+def test_replays_from_a_graph_and_refuses_second_derivatives():
+    x, t = make(3, 5000, BF16)
+    leaf = x.clone().requires_grad_(True)
+    up = torch.tensor([1.0, -2.0, 0.5], device="cuda")
+
+    def step():
+        r = token_logprobs(leaf, t, top_k=3)
+        (dx,) = torch.autograd.grad([r.logp], [leaf], [up])
+        return r.logp.detach(), r.top_index, dx
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    y, _ = make(3, 5000, BF16, seed=9)
+    with torch.no_grad():
+        leaf.copy_(y)
+    graph.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(got, step()):
+        assert torch.equal(a, b)
+    r = token_logprobs(leaf, t)
+    (dx,) = torch.autograd.grad([r.logp.sum()], [leaf], create_graph=True)
+    with pytest.raises(RuntimeError):
+        dx.float().sum().backward()
+
+
+@TYPES
 def test_strides_and_index_types(dtype):
     x, t = make(9, 1003, dtype)
     wide = torch.full((9, 1100), math.nan, dtype=dtype, device="cuda")
