@@ -48,7 +48,7 @@ def check_forward(r, x, t, K):
 
 
 SHAPES = [(1, 1, 0), (3, 2, 0), (5, 7, 3), (2, 64, 0), (37, 259, 59), (4, 1000, 333), (3, 4099, 0), (2, 50257, 0),
-          (2, 50304, 47), (1, 131075, 0), (200, 513, 0)]
+          (2, 50304, 47), (1, 131075, 0), (200, 513, 0), (1300, 77, 5)]
 
 
 @TYPES
@@ -192,7 +192,8 @@ def test_strides_and_index_types(dtype):
 
 
 @TYPES
-@pytest.mark.parametrize("N,V,masked", [(1, 1, 0), (5, 7, 3), (37, 259, 59), (3, 4099, 0), (2, 50304, 47), (3, 50257, 0), (150, 640, 0)])
+@pytest.mark.parametrize("N,V,masked", [(1, 1, 0), (5, 7, 3), (37, 259, 59), (3, 4099, 0), (2, 50304, 47), (3, 50257, 0), (150, 640, 0),
+                                        (1300, 77, 5)])
 @pytest.mark.parametrize("K", [0, 6])
 def test_gradient_matches_formula(N, V, masked, K, dtype):
     K = min(K, V - masked)
