@@ -49,33 +49,42 @@ def _forward(logits: torch.Tensor, targets: torch.Tensor, top_k: int, index: int
     return logp, entropy, top_logp.view(n, top_k), top_index, stats
 
 
+def _f32(g: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    if g is None or (g.dtype is torch.float32 and g.is_contiguous()):
+        return g
+    return g.to(torch.float32).contiguous()
+
+
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits: torch.Tensor, targets: torch.Tensor, top_k: int, index: int):
-        # tensors of their own: a caller may change a result in place
-        n, opts = logits.shape[0], dict(dtype=torch.float32, device=logits.device)
-        logp, entropy, top_logp = torch.empty(n, **opts), torch.empty(n, **opts), torch.empty((n, top_k), **opts)
-        stats = torch.empty((n, 2), **opts)
-        top_index = torch.empty((n, top_k), dtype=torch.int64, device=logits.device)
-        a = _args(logits, targets, top_k, logp.data_ptr(), entropy.data_ptr(), stats.data_ptr(),
-                  top_logp.data_ptr(), top_index.data_ptr())
+        # results are tensors of their own: a caller may change one in place
+        n, device = logits.shape[0], logits.device
+        logp = torch.empty(n, dtype=torch.float32, device=device)
+        entropy, top_logp, stats = torch.empty_like(logp), logp.new_empty((n, top_k)), logp.new_empty((n, 2))
+        top_index = torch.empty((n, top_k), dtype=torch.int64, device=device)
+        a = _args(logits, targets, top_k, logp.data_ptr(), entropy.data_ptr(), stats.data_ptr(), top_logp.data_ptr(),
+                  top_index.data_ptr())
         launch(_lib.load().fb_logprob_fwd, a, index, "token log probabilities")
-        ctx.save_for_backward(logits, targets, entropy, stats, top_index)
+        if top_k:
+            ctx.save_for_backward(logits, targets, entropy, stats, top_index)
+        else:
+            ctx.save_for_backward(logits, targets, entropy, stats)
         ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(top_index)
-        ctx.index = index
+        ctx.top_k, ctx.index = top_k, index
         return logp, entropy, top_logp, top_index
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g_logp: Optional[torch.Tensor], g_entropy: Optional[torch.Tensor],
                  g_top: Optional[torch.Tensor], _g_index):
-        logits, targets, entropy, stats, top_index = ctx.saved_tensors
+        logits, targets, entropy, stats, *top_index = ctx.saved_tensors
         grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        given = [g if g is None else g.to(torch.float32).contiguous() for g in (g_logp, g_entropy, g_top)]
-        ptrs = [0 if g is None else g.data_ptr() for g in given]
-        a = _args(logits, targets, top_index.shape[1], 0, entropy.data_ptr(), stats.data_ptr(), 0, top_index.data_ptr(),
-                  *ptrs, grad.data_ptr())
+        g_logp, g_entropy, g_top = _f32(g_logp), _f32(g_entropy), _f32(g_top) if ctx.top_k else None
+        a = _args(logits, targets, ctx.top_k, 0, entropy.data_ptr(), stats.data_ptr(), 0,
+                  top_index[0].data_ptr() if top_index else 0, *[0 if g is None else g.data_ptr() for g in (g_logp, g_entropy, g_top)],
+                  grad.data_ptr())
         launch(_lib.load().fb_logprob_bwd, a, ctx.index, "token log probabilities backward")
         return grad, None, None, None
 
