@@ -399,7 +399,7 @@ typedef struct fb_paged_args {
   void* out;           int64_t out_stride[3]; /* (seqs, heads, head_dim) */
   const int32_t* table; int64_t table_stride; /* elements between the table's rows */
   const int32_t* lens;
-  void* workspace;     size_t workspace_bytes;
+  void* workspace;     size_t workspace_bytes; /* fb_paged_workspace_size bytes, 16-byte aligned */
 } fb_paged_args;
 
 FB_API size_t fb_paged_workspace_size(const fb_paged_args* args);

@@ -15,8 +15,8 @@
 // under way while the first runs.
 //
 // Measured: 127 M fp32 in place below the limit 76 us a call (6.65 TB/s; the sum's kernel 6.85), 40 M bf16 of odd
-// sizes into fp32 57 us of kernels (240 MB by the formula's need, 320 MB with the second read of what did not
-// stay in L2: 5.6 TB/s), 12 tensors of 99 K elements 8 to 10 us, the two launches.
+// sizes into fp32 57 us of kernels (240 MB by the formula's need; about 270 MB of DRAM traffic, since 47 of the
+// second read's 80 MB did not stay in L2), 12 tensors of 99 K elements 8 to 10 us, the two launches.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -194,7 +194,7 @@ __device__ __forceinline__ uint4 pack(const f32x2 (&f)[4], const __half*) {
 }
 
 // 16 bytes stored per thread and vector, neighbours next to one another: 16-bit gradients on their way to fp32 are
-// taken 8 bytes at a time (with 16, a warp's stores left every other 16 bytes for the next: 54 us against 41)
+// taken 8 bytes at a time (with 16, a warp's stores left every other 16 bytes for the next: 70 us against 60 in all)
 template <typename T, typename U>
 __device__ __forceinline__ void scale(const Tensor& t, uint32_t chunk, float c) {
   constexpr int N = 16 / sizeof(U);

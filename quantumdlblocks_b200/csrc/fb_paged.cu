@@ -256,8 +256,9 @@ struct Feed {
 // No barrier between warps; the ring runs on into the next piece while one is finished.
 //
 // mma.sync, not tcgen05: 16 rows are all there are, the tensor pipe is 20 % busy at 6 TB/s, and an accumulator in
-// registers goes from S to P without a round trip.  Before the warps had shares and rings of their own (one
-// share per CTA, its warps' sums joined in shared memory at each piece's end) the batch of 48 took 63 us.
+// registers goes from S to P without a round trip.  With one share per CTA, its warps' sums joined in shared
+// memory at each piece's end, and rows copied by all lanes the batch of 48 sequences took 63 us; shares and TMA
+// rings of a warp's own and the rest of P in free operand rows made that 37, a lighter join and four CTAs 30.
 template <typename T, int D, bool PACK, bool TMA>
 __global__ void __launch_bounds__(kThreads, TcShape<D>::kCtasPerSm)
     paged_born_tc(const PagedParams p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
@@ -943,8 +944,8 @@ __device__ __forceinline__ uint4 pack_pairs(const sm100::f32x2 (&f)[4], const __
 // makes `accesses` of them, all of one token, ACC at a time.  The turn's other half of a piece is LPH / 2 lanes
 // away (one exchange of the raw words), the norm a sum over the head's lanes.  Reads and writes every element
 // once: HBM bandwidth bounds it, and for a batch's new tokens latency (one access a warp spreads them over more).
-// 16,389 tokens of 32 + 4 + 4 heads of 128, bf16, 344 MB: 67 us, 5.1 TB/s (a warp per four accesses instead of per
-// token, each with its own slot, position and angles: 100 us); 48 tokens of 16 + 8 + 8 heads of 64: 4.5 us.
+// 16,389 tokens of 32 + 4 + 4 heads of 128, bf16, 344 MB: 67 us, 5.1 TB/s (72 us with three CTAs per SM, and
+// then 100 us with a warp per four accesses, each with its own slot, position and angles); 48 tokens of 16 + 8 + 8 heads of 64: 4.5 us.
 template <typename T, int LPH, int ACC>
 __global__ void __launch_bounds__(256, 4) paged_write_vec(const WriteParams p, int warps_per_token, int accesses) {
   using namespace sm100;
@@ -1260,7 +1261,8 @@ cudaError_t launch_paged(const PagedParams& p, const PagedPlan& pl, cudaStream_t
   }
   if (e != cudaSuccess || !pl.join) return e;
   // A warp has four pieces' loads under way at a time: a warp on an output for every eight of the pieces that a
-  // unit would have were the lengths alike (49 pieces of 192 units: 27 us with 32 warps each, 5 us with 8)
+  // unit would have were the lengths alike (by ncu, cold: 27 us with 32 warps on each of 768 outputs of 49 pieces;
+  // 9.5 us with 32 on each of 64 heads of 148 pieces, as here)
   const uint32_t pieces = p.W / ((uint32_t)p.S * p.U) + 1;
   int ways = 1;
   while (ways < 32 && ways * 8 < (int)pieces) ways *= 2;

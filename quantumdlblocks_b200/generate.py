@@ -125,9 +125,10 @@ def generate(model: BornGPT, prompts: Sequence[torch.Tensor], new_tokens: int, t
                 noise = torch.empty(logits.shape, dtype=torch.float32, device=device).exponential_(generator=generator)
                 chosen = (logits.float() / temperature - noise.log()).argmax(dim=1)
                 r = token_logprobs(logits, chosen, top_k)
-            else:
-                chosen = torch.argmax(logits, dim=1)
-                r = token_logprobs(logits, chosen, top_k)
+            else:  # the first alternative is the choice
+                r = token_logprobs(logits, torch.zeros_like(counts), max(top_k, 1))
+                chosen = r.top_index[:, 0]
+                r = r._replace(logp=r.top_logp[:, 0], top_logp=r.top_logp[:, :top_k], top_index=r.top_index[:, :top_k])
             for to, y in zip(got, (chosen, *r)):
                 to.append(y)
             if step + 1 == new_tokens:
@@ -155,7 +156,7 @@ class PolicyStep(NamedTuple):
 def policy_step(model: BornGPT, opt: torch.optim.Optimizer, tokens: torch.Tensor, advantages: torch.Tensor,
                 entropy_weight: float = 0.0, max_norm: float = 1.0,
                 autocast_dtype: Optional[torch.dtype] = torch.bfloat16) -> PolicyStep:
-    """One policy-gradient step: ``-(mean of advantage * logp + entropy_weight * entropy)`` over the tokens of
+    """One policy-gradient step of a plain ``BornGPT`` (no data-parallel wrapper): ``-(mean of advantage * logp + entropy_weight * entropy)`` over the tokens of
     ``tokens (B, T + 1)`` whose ``advantages (B, T)`` (of token t + 1 at t) are not 0, gradients clipped to ``max_norm``."""
     inp, tgt = tokens[:, :-1], tokens[:, 1:].reshape(-1)
     adv = advantages.reshape(-1).to(torch.float32)
