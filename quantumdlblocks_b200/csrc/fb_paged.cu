@@ -77,7 +77,7 @@ __device__ __forceinline__ Keys keys_of(const PagedParams& p, int s) {
   k.hi = min(max(p.lens[s], 0), p.page * p.width);
   k.lo = p.window > 0 ? max(k.hi - p.window, 0) : 0;
   k.base = k.lo & ~(kSub - 1);
-  k.tiles = max((uint32_t)(k.hi - k.base + p.tile - 1) / (uint32_t)p.tile, 1u);
+  k.tiles = max(((uint32_t)(k.hi - k.base) + (uint32_t)p.tile - 1) / (uint32_t)p.tile, 1u);
   return k;
 }
 

@@ -73,6 +73,11 @@ CASES = [
     (3, 3, 7, 5, [33, 6], 4),
     (4, 2, 256, 16, [70, 300], 0),
     (9, 3, 80, 32, [640, 31], 100),
+    (12, 1, 64, 24, [100, 0, 700], 0),
+    (9, 1, 128, 5, [60, 333], 50),
+    (4, 2, 128, 24, [500, 24], 0),
+    (2, 2, 200, 16, [300, 17], 0),
+    (2, 1, 128, 64, [2000], 0),
     (1, 1, 1, 3, [10], 0),
 ]
 
@@ -197,6 +202,32 @@ def test_offsets_past_32_bits(dtype):
     slots = torch.tensor([P * page - 1, P * page], device="cuda")
     paged_qkv_write(qkv, cos, sin, torch.tensor([0, 1], device="cuda"), slots, k, v, 8)
     assert torch.equal(v[P - 1, :, page - 1], qkv[0].view(24, D)[16:])
+
+
+@pytest.mark.parametrize("H,Hkv,D,dtype", [(4, 2, 64, BF16), (4, 2, 48, F32)])
+def test_tables_far_wider_than_the_lengths(H, Hkv, D, dtype):
+    """2^30 keys' worth of table columns for 64 sequences of at most 300: tiles, counted in 31 bits, get coarser."""
+    page, width, S = 1024, 1 << 20, 64
+    k, v, one, _ = make_cache([1000], Hkv, D, page, dtype)
+    table = torch.full((1, width), -1, dtype=torch.int32, device="cuda")
+    table[0, 0] = one[0, 0]
+    lens = [(37 * s) % 301 for s in range(S)]
+    q = make_q(S, H, D, dtype)
+    n = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    got = paged_born_attention(q, k, v, table.expand(S, width), n, 8.0)
+    check(got, ref.paged_attention(q, k, v, table[:, :1].expand(S, 1), lens, [8.0] * H), v, dtype)
+
+
+@pytest.mark.parametrize("D,dtype", [(64, BF16), (128, F16), (64, F32)])
+def test_many_sequences(D, dtype):
+    """More sequences than threads that sum their tiles, most of them empty or of a few keys, one long."""
+    lens = [(7 * s * s) % 23 if s % 3 else 0 for s in range(700)]
+    lens[411] = 3000
+    k, v, table, n = make_cache(lens, 2, D, 16, dtype)
+    q = make_q(len(lens), 4, D, dtype)
+    for window in (0, 5):
+        got = paged_born_attention(q, k, v, table, n, 8.0, window_size=window)
+        check(got, ref.paged_attention(q, k, v, table, lens, [8.0] * 4, window=window), v, dtype)
 
 
 def test_runs_on_the_current_stream():
