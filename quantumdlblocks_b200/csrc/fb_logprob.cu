@@ -623,15 +623,18 @@ int parts_of(const LogprobParams& p, int chunk, int most) {
   return parts;
 }
 
-bool many(const LogprobParams& p) { return p.rows >= 8 * sm_count(); }
+// Rows enough for the smaller CTAs: so many per SM.  With alternatives 256 threads win over 512 from 3 on (800 x
+// 50304 bf16: 26.7 us against 32.9; 500: 19.7 against 22.6), without them 128 from 5 on (800: 24.1 against 25.0;
+// 500: 20.8 against 17.4).
+bool many(const LogprobParams& p, int per_sm) { return p.rows >= per_sm * sm_count(); }
 
 template <typename T>
 cudaError_t launch_fwd(const LogprobParams& p, cudaStream_t s) {
   const unsigned n = (unsigned)p.rows;
   const int parts = parts_of(p, 16 / sizeof(T), kMaxCluster);
   if (parts == 1) {
-    if (many(p) && p.K == 0) logprob_fwd_kernel<T, kManyPlain, false><<<n, kManyPlain, 0, s>>>(p);
-    else if (many(p)) logprob_fwd_kernel<T, kMany, false><<<n, kMany, 0, s>>>(p);
+    if (p.K == 0 && many(p, 5)) logprob_fwd_kernel<T, kManyPlain, false><<<n, kManyPlain, 0, s>>>(p);
+    else if (p.K > 0 && many(p, 3)) logprob_fwd_kernel<T, kMany, false><<<n, kMany, 0, s>>>(p);
     else logprob_fwd_kernel<T, kFew, false><<<n, kFew, 0, s>>>(p);
     return cudaGetLastError();
   }
@@ -651,7 +654,7 @@ cudaError_t launch_fwd(const LogprobParams& p, cudaStream_t s) {
 template <typename T>
 cudaError_t launch_bwd(const LogprobParams& p, cudaStream_t s) {
   const dim3 grid((unsigned)p.rows, parts_of(p, 16 / sizeof(T), 1024));
-  if (many(p)) logprob_bwd_kernel<T, kMany><<<grid, kMany, 0, s>>>(p);
+  if (many(p, 8)) logprob_bwd_kernel<T, kMany><<<grid, kMany, 0, s>>>(p);
   else logprob_bwd_kernel<T, kFew><<<grid, kFew, 0, s>>>(p);
   return cudaGetLastError();
 }
