@@ -280,16 +280,16 @@ int check(const fb_clip_args* a) {
     if (a->numel[i] == 0) continue;
     if (a->grads[i] == nullptr || (a->out != nullptr && a->out[i] == nullptr)) return FB_ERR_ARG;
     const int out_size = a->out_dtype != nullptr ? size_of(a->out_dtype[i]) : size_of(a->dtype[i]);
-    if (reinterpret_cast<uintptr_t>(a->grads[i]) % size_of(a->dtype[i]) != 0 ||
-        (a->out != nullptr && reinterpret_cast<uintptr_t>(a->out[i]) % out_size != 0))
+    if ((reinterpret_cast<uintptr_t>(a->grads[i]) & (size_of(a->dtype[i]) - 1)) != 0 ||
+        (a->out != nullptr && (reinterpret_cast<uintptr_t>(a->out[i]) & (out_size - 1)) != 0))
       return FB_ERR_ALIGN;
   }
   if (a->workspace == nullptr || a->workspace_bytes < workspace_size(a)) return FB_ERR_WORKSPACE;
   return FB_OK;
 }
 
-// The table of launch l, in chunks of `bytes`
-void fill(ClipParams* p, const fb_clip_args* a, int l, uint32_t bytes) {
+// The table of launch l, in chunks of BYTES
+template <uint32_t BYTES> void fill(ClipParams* p, const fb_clip_args* a, int l) {
   p->count = 0;
   p->chunks = 0;
   p->in_place = true;
@@ -304,11 +304,11 @@ void fill(ClipParams* p, const fb_clip_args* a, int l, uint32_t bytes) {
     const uint64_t shift = reinterpret_cast<uintptr_t>(t.g) & 15, end = shift + (uint64_t)t.n * size_of(t.dtype);
     t.chunk0 = p->chunks;
     t.full0 = t.chunk0 + (shift > 0);
-    t.fulls = (uint32_t)std::max<int64_t>((int64_t)(end / bytes) - (shift > 0), 0);
+    t.fulls = (uint32_t)std::max<int64_t>((int64_t)(end / BYTES) - (shift > 0), 0);
     t.out_aligned =
-        (reinterpret_cast<uintptr_t>(t.out) - shift / size_of(t.dtype) * size_of(t.out_dtype)) % 16 == 0;
+        ((reinterpret_cast<uintptr_t>(t.out) - (t.dtype == t.out_dtype ? shift : shift * 2)) & 15) == 0;  // 16 bits to 32
     p->in_place = p->in_place && t.out == t.g;
-    p->chunks += (uint32_t)((end + bytes - 1) / bytes);
+    p->chunks += (uint32_t)((end + BYTES - 1) / BYTES);
   }
 }
 
@@ -323,7 +323,7 @@ int clip(const fb_clip_args* a, cudaStream_t s) {
   int parts = 0;
   cudaError_t e = cudaSuccess;
   for (int l = 0; l < launches && e == cudaSuccess; ++l) {
-    fill(&p, a, l, kSumBytes);
+    fill<kSumBytes>(&p, a, l);
     const int grid = (int)std::max<uint32_t>(1, std::min<uint32_t>(p.chunks, kSumCtas * sms));
     p.part = sums + parts;
     parts += grid;
@@ -334,7 +334,7 @@ int clip(const fb_clip_args* a, cudaStream_t s) {
   p.parts = parts;
   int n = launches;
   for (int l = 0; l < (a->out != nullptr ? launches : 1) && e == cudaSuccess; ++l, ++n) {
-    if (a->out != nullptr) fill(&p, a, l, kScaleBytes);
+    if (a->out != nullptr) fill<kScaleBytes>(&p, a, l);
     else p.chunks = 0;
     p.norm = l == 0 ? a->norm : nullptr;
     cudaLaunchConfig_t cfg{};

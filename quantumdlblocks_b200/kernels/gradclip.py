@@ -7,7 +7,7 @@ their number, sizes and types.  CUDA only, like every op here.
 from __future__ import annotations
 
 import array
-from operator import attrgetter
+from operator import attrgetter, eq
 from typing import Iterable, Optional, Sequence
 
 import torch
@@ -114,7 +114,7 @@ def clip_grad_norm_(
             if not _dense(g):
                 raise ValueError(f"clip_grad_norm_: gradients must be dense; got strides {g.stride()} for {tuple(g.shape)}")
     if to is not gs:
-        alike = list(map(_shape, gs)) == list(map(_shape, to))
+        alike = all(map(eq, map(_shape, gs), map(_shape, to)))
         alike = alike and (all(map(_is_contiguous, to)) if plain else [g.stride() for g in gs] == [o.stride() for o in to])
         if not alike or any(o not in (torch.float32, g) for g, o in set(zip(map(_dtype, gs), map(_dtype, to)))):
             raise ValueError("clip_grad_norm_: each of out must match its gradient's shape and memory order, and have its "
