@@ -457,10 +457,12 @@ __global__ void __launch_bounds__(THREADS, threads_per_sm(THREADS) / THREADS) lo
     const float ls = log2f(all.s);
     auto logp_of = [&](float x) { return (x - all.m) - kLn2 * ls; };
     if (threadIdx.x == 0) {
-      p.stats[2 * r] = all.m;
-      p.stats[2 * r + 1] = ls;
+      const float h = kLn2 * (ls - all.u / all.s);
+      p.stats[3 * r] = all.m;
+      p.stats[3 * r + 1] = ls;
+      p.stats[3 * r + 2] = h;
       p.logp[r] = logp_of(target);
-      p.entropy[r] = kLn2 * (ls - all.u / all.s);
+      p.entropy[r] = h;
     }
     for (int i = threadIdx.x; i < p.K; i += THREADS) {
       p.top_index[r * p.K + i] = key_column(top[i]);
@@ -509,7 +511,7 @@ __global__ void __launch_bounds__(THREADS, 1280 / THREADS) logprob_bwd_kernel(co
   const bool same = in.shift == out.shift;
   int j0, j1;
   out.part_of(blockIdx.y, gridDim.y, j0, j1);
-  float m = p.stats[2 * r], ls = p.stats[2 * r + 1];
+  float m = p.stats[3 * r], ls = p.stats[3 * r + 1];
   const int64_t t = p.targets[r];
   const float g = p.g_logp ? p.g_logp[r] : 0.f, gh = p.g_entropy ? p.g_entropy[r] : 0.f;
   // the weight of -p: the gradients of all log probabilities taken (NaN where the target has none), and
@@ -522,7 +524,7 @@ __global__ void __launch_bounds__(THREADS, 1280 / THREADS) logprob_bwd_kernel(co
       none = none && x == 0.f;
       c0 += x;
     }
-  if (gh != 0.f) c0 = fmaf(gh, p.entropy[r], c0);
+  if (gh != 0.f) c0 = fmaf(gh, p.stats[3 * r + 2], c0);
   if (none) m = ls = 0.f;  // which may be NaN
   const float c1 = gh * kLn2;
   auto value = [&](float x) {
@@ -670,8 +672,8 @@ int logprob(const fb_logprob_args* a, void* stream, bool backward) {
     set_last_launch_count(0);
     return FB_OK;
   }
-  if (a->logits == nullptr || a->targets == nullptr || a->stats == nullptr || a->entropy == nullptr) return FB_ERR_ARG;
-  if (!backward && a->logp == nullptr) return FB_ERR_ARG;
+  if (a->logits == nullptr || a->targets == nullptr || a->stats == nullptr) return FB_ERR_ARG;
+  if (!backward && (a->logp == nullptr || a->entropy == nullptr)) return FB_ERR_ARG;
   if (!backward && a->top_k > 0 && (a->top_logp == nullptr || a->top_index == nullptr)) return FB_ERR_ARG;
   if (backward && a->grad == nullptr) return FB_ERR_ARG;
   if (backward && a->top_k > 0 && a->g_top != nullptr && a->top_index == nullptr) return FB_ERR_ARG;

@@ -40,8 +40,8 @@ def _args(logits: torch.Tensor, targets: torch.Tensor, top_k: int, logp: int = 0
 def _forward(logits: torch.Tensor, targets: torch.Tensor, top_k: int, index: int) -> tuple[torch.Tensor, ...]:
     n = logits.shape[0]
     # one allocation where nothing needs the results as tensors of their own
-    logp, entropy, top_logp, stats = torch.empty(n * (4 + top_k), dtype=torch.float32, device=logits.device).split_with_sizes(
-        (n, n, n * top_k, 2 * n))
+    logp, entropy, top_logp, stats = torch.empty(n * (5 + top_k), dtype=torch.float32, device=logits.device).split_with_sizes(
+        (n, n, n * top_k, 3 * n))
     top_index = torch.empty((n, top_k), dtype=torch.int64, device=logits.device)
     a = _args(logits, targets, top_k, logp.data_ptr(), entropy.data_ptr(), stats.data_ptr(), top_logp.data_ptr(),
               top_index.data_ptr())
@@ -61,15 +61,15 @@ class _TokenLogprobs(torch.autograd.Function):
         # results are tensors of their own: a caller may change one in place
         n, device = logits.shape[0], logits.device
         logp = torch.empty(n, dtype=torch.float32, device=device)
-        entropy, top_logp, stats = torch.empty_like(logp), logp.new_empty((n, top_k)), logp.new_empty((n, 2))
+        entropy, top_logp, stats = torch.empty_like(logp), logp.new_empty((n, top_k)), logp.new_empty((n, 3))
         top_index = torch.empty((n, top_k), dtype=torch.int64, device=device)
         a = _args(logits, targets, top_k, logp.data_ptr(), entropy.data_ptr(), stats.data_ptr(), top_logp.data_ptr(),
                   top_index.data_ptr())
         launch(_lib.load().fb_logprob_fwd, a, index, "token log probabilities")
         if top_k:
-            ctx.save_for_backward(logits, targets, entropy, stats, top_index)
+            ctx.save_for_backward(logits, targets, stats, top_index)
         else:
-            ctx.save_for_backward(logits, targets, entropy, stats)
+            ctx.save_for_backward(logits, targets, stats)
         ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(top_index)
         ctx.top_k, ctx.index = top_k, index
@@ -79,10 +79,10 @@ class _TokenLogprobs(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, g_logp: Optional[torch.Tensor], g_entropy: Optional[torch.Tensor],
                  g_top: Optional[torch.Tensor], _g_index):
-        logits, targets, entropy, stats, *top_index = ctx.saved_tensors
+        logits, targets, stats, *top_index = ctx.saved_tensors
         grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         g_logp, g_entropy, g_top = _f32(g_logp), _f32(g_entropy), _f32(g_top) if ctx.top_k else None
-        a = _args(logits, targets, ctx.top_k, 0, entropy.data_ptr(), stats.data_ptr(), 0,
+        a = _args(logits, targets, ctx.top_k, 0, 0, stats.data_ptr(), 0,
                   top_index[0].data_ptr() if top_index else 0, *[0 if g is None else g.data_ptr() for g in (g_logp, g_entropy, g_top)],
                   grad.data_ptr())
         launch(_lib.load().fb_logprob_bwd, a, ctx.index, "token log probabilities backward")

@@ -261,6 +261,21 @@ def test_gradient_matches_differences():
     assert abs(slope - want) <= 2e-3 * max(1.0, abs(want)), (slope, want)
 
 
+def test_results_may_change_before_the_backward():
+    """The backward keeps what it needs itself: results altered in place do not alter the gradient."""
+    x, t = make(5, 300, F32)
+    want = ref.logprobs_grad(x, t, torch.zeros(5, 0, dtype=torch.int64, device="cuda"), torch.ones(5, device="cuda"),
+                             torch.ones(5, device="cuda"), torch.zeros(5, 0, device="cuda"))
+    leaf = x.clone().requires_grad_(True)
+    r = token_logprobs(leaf, t)
+    loss = (r.logp + r.entropy).sum()
+    with torch.no_grad():
+        r.entropy.zero_()
+        r.logp.fill_(7.0)
+    loss.backward()
+    assert float((leaf.grad.double() - want).abs().max()) <= 1e-4
+
+
 @TYPES
 def test_targets_out_of_range(dtype):
     x, t = make(5, 130, dtype)
