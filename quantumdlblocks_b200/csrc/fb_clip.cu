@@ -9,7 +9,7 @@
 //   clip_sum    each CTA's sum of squares: fp32 for the 16 or 32 squares of a thread and chunk, fp64 beyond
 //   clip_scale  each CTA adds all CTAs' sums, in order, to the norm (the same bits everywhere and every time),
 //               and scales its chunks; in place with c = 1 there is nothing to do.  It takes the chunks from the
-//               last to the first: what clip_sum read last is still in L2.
+//               last to the first, for what of clip_sum's last reads is still in L2.
 //
 // Both are bound by HBM bandwidth for many elements; for few by the two launches, the second of which is
 // under way while the first runs.
